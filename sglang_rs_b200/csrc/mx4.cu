@@ -1,0 +1,174 @@
+// Rows into the microscaled four-bit format of mx4.cuh and back.
+//
+//   srb_mx4_quantize     per block of 32 entries: e = floor(log2(largest magnitude)) - 2, at least -127; s = e + 127; an entry is
+//                        x / 2^e rounded to the nearest value, ties to the even mantissa, magnitudes above 6 to 6 (the OCP
+//                        specification's conversion).  x / 2^e is exact, so the codes are a function of the numbers alone.  A block
+//                        that holds an infinity or something that is not a number has s = 255 and codes of zero.
+//   srb_mx4_dequantize   the values, in bfloat16 (which holds every one of them exactly) or float.
+//
+// Both are bound by the bytes of the wide side.  A row's 128 entries are the work of 16 lanes, 8 entries (16 bytes of bfloat16) each; 4 lanes
+// are a block.
+#include "common.cuh"
+#include "mx4.cuh"
+
+SRB_DEFINE_LAST_ERROR()
+SRB_DEFINE_PDL_SWITCH()
+
+#define MX4_THREADS 256
+
+__device__ __forceinline__ void mx4_unpack_bf16(const uint4& raw, float (&v)[8]) {
+  const unsigned w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    v[2 * i] = __uint_as_float(w[i] << 16);
+    v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+  }
+}
+
+// Four scaled entries to two bytes each, nearest with ties to even, magnitudes above 6 to 6; the first entry in the low half.
+__device__ __forceinline__ unsigned mx4_pack_eight(const float (&v)[8]) {
+  unsigned out;
+  asm("{\n.reg .b8 a, b, c, d;\n"
+      "cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\ncvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n"
+      "cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\ncvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n"
+      "mov.b32 %0, {a, b, c, d};\n}\n"
+      : "=r"(out) : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]));
+  return out;
+}
+
+template <typename T, bool WIDE>
+__global__ void __launch_bounds__(MX4_THREADS)
+mx4_quantize_kernel(const T* __restrict__ x, size_t pitch, size_t matrix_pitch, int rows, int width, unsigned* __restrict__ codes,
+                    unsigned* __restrict__ scales) {
+  srb_launch_dependents();
+  srb_grid_dependency_wait();
+  const int k_tiles = mx4_tiles(width), row_tiles = mx4_tiles(rows);
+  const int lane = threadIdx.x & 15;                         // of the 16 that share 128 entries of a row
+  const long long item = (long long)blockIdx.x * (MX4_THREADS / 16) + (threadIdx.x >> 4);
+  const int row = (int)(item / k_tiles), kt = (int)(item % k_tiles), matrix = blockIdx.y;
+  const bool inside = row < row_tiles * 128, live = row < rows;
+  const int k = kt * 128 + lane * 8;
+  float v[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = 0.f;
+  if (live) {
+    const T* src = x + (size_t)matrix * matrix_pitch + (size_t)row * pitch + k;
+    if (WIDE && k + 8 <= width) {
+      if (sizeof(T) == 2) mx4_unpack_bf16(*reinterpret_cast<const uint4*>(src), v);
+      else {
+        const float4 a = reinterpret_cast<const float4*>(src)[0], b = reinterpret_cast<const float4*>(src)[1];
+        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (k + i < width) v[i] = srb_to_float(src[i]);
+    }
+  }
+  // magnitudes as their bits: the largest bits are the largest magnitude, and whatever is not finite is above all that is
+  unsigned most = 0u;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) most = max(most, __float_as_uint(v[i]) & 0x7fffffffu);
+  most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
+  most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
+  const bool finite = most < 0x7f800000u;
+  const int exponent = max((int)(most >> 23) - 129, -127);   // a subnormal's field is 0: the least scale
+  const unsigned s = finite ? (unsigned)(exponent + 127) : 255u;
+  const float inverse = __uint_as_float((unsigned)(127 - exponent) << 23);      // 2^-exponent, between 2^-125 and 2^127
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = finite ? v[i] * inverse : 0.f;
+  const unsigned packed = mx4_pack_eight(v);
+  // the scales of the four blocks, a byte each, in one word; blocks behind the row's end and rows behind the last get 127
+  unsigned word = live && kt * 128 + (lane >> 2) * 32 < width ? s : 127u;
+  word = (lane & 3) == 0 ? word << (8 * (lane >> 2)) : 0u;
+  word |= __shfl_xor_sync(0xffffffffu, word, 4);
+  word |= __shfl_xor_sync(0xffffffffu, word, 8);
+  if (!inside) return;
+  if (live) codes[((size_t)matrix * rows + row) * (mx4_pitch(width) / 4) + kt * 16 + lane] = packed;
+  if (lane == 0) scales[((size_t)matrix * row_tiles * k_tiles * MX4_TILE_BYTES + mx4_scale_word(row, kt, k_tiles)) / 4] = word;
+}
+
+template <typename T, bool WIDE>
+__global__ void __launch_bounds__(MX4_THREADS)
+mx4_dequantize_kernel(const unsigned* __restrict__ codes, const unsigned* __restrict__ scales, int rows, int width, T* __restrict__ out) {
+  srb_launch_dependents();
+  srb_grid_dependency_wait();
+  const int k_tiles = mx4_tiles(width), row_tiles = mx4_tiles(rows);
+  const int lane = threadIdx.x & 15;
+  const long long item = (long long)blockIdx.x * (MX4_THREADS / 16) + (threadIdx.x >> 4);
+  const int row = (int)(item / k_tiles), kt = (int)(item % k_tiles), matrix = blockIdx.y;
+  if (row >= rows) return;
+  const unsigned packed = codes[((size_t)matrix * rows + row) * (mx4_pitch(width) / 4) + kt * 16 + lane];
+  const unsigned word = scales[((size_t)matrix * row_tiles * k_tiles * MX4_TILE_BYTES + mx4_scale_word(row, kt, k_tiles)) / 4];
+  const float scale = mx4_scale_value((word >> (8 * (lane >> 2))) & 255u);
+  const int k = kt * 128 + lane * 8;
+  T* dst = out + ((size_t)matrix * rows + row) * width + k;
+  float v[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = mx4_code_value((packed >> (4 * i)) & 15u) * scale;
+  if (WIDE && k + 8 <= width) {
+    if (sizeof(T) == 2) {
+      unsigned w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const __nv_bfloat162 pair = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+        w[i] = *reinterpret_cast<const unsigned*>(&pair);
+      }
+      *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
+    } else {
+      reinterpret_cast<float4*>(dst)[0] = make_float4(v[0], v[1], v[2], v[3]);
+      reinterpret_cast<float4*>(dst)[1] = make_float4(v[4], v[5], v[6], v[7]);
+    }
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (k + i < width) dst[i] = srb_from_float<T>(v[i]);
+}
+
+static int mx4_grid(int matrices, long long rows, int width, dim3* grid) {
+  const long long items = rows * mx4_tiles(width), blocks = (items + MX4_THREADS / 16 - 1) / (MX4_THREADS / 16);
+  if (blocks > 0x7fffffffll || matrices > 65535) SRB_FAIL("mx4: %d matrices of %lld rows of %d entries are too many", matrices, rows, width);
+  *grid = dim3((unsigned)blocks, (unsigned)matrices);
+  return SRB_OK;
+}
+
+// x: `matrices` matrices, `matrix_pitch` elements apart, of `rows` rows, `pitch` elements apart, of `width` entries.
+extern "C" int srb_mx4_quantize(const void* x, long long pitch, long long matrix_pitch, int matrices, int rows, int width, void* codes,
+                                void* scales, int dtype, void* stream) {
+  if (matrices <= 0 || rows <= 0 || width <= 0) return SRB_OK;
+  dim3 grid;
+  if (mx4_grid(matrices, (long long)mx4_tiles(rows) * 128, width, &grid) != SRB_OK) return SRB_ERR_INVALID;
+  const int element = dtype == SRB_DTYPE_F32 ? 4 : 2;
+  const bool wide = ((uintptr_t)x & 15) == 0 && pitch * element % 16 == 0 && matrix_pitch * element % 16 == 0;
+  cudaStream_t s = (cudaStream_t)stream;
+  if (dtype == SRB_DTYPE_F32)
+    SRB_CUDA_CALL(srb_launch(wide ? mx4_quantize_kernel<float, true> : mx4_quantize_kernel<float, false>, grid, dim3(MX4_THREADS), 0, s,
+                             (const float*)x, (size_t)pitch, (size_t)matrix_pitch, rows, width, (unsigned*)codes, (unsigned*)scales));
+  else if (dtype == SRB_DTYPE_BF16)
+    SRB_CUDA_CALL(srb_launch(wide ? mx4_quantize_kernel<__nv_bfloat16, true> : mx4_quantize_kernel<__nv_bfloat16, false>, grid, dim3(MX4_THREADS), 0,
+                             s, (const __nv_bfloat16*)x, (size_t)pitch, (size_t)matrix_pitch, rows, width, (unsigned*)codes, (unsigned*)scales));
+  else
+    SRB_FAIL("mx4_quantize: unknown dtype %d", dtype);
+  SRB_LAUNCH_CHECK("mx4_quantize");
+  return SRB_OK;
+}
+
+extern "C" int srb_mx4_dequantize(const void* codes, const void* scales, int matrices, int rows, int width, void* out, int dtype, void* stream) {
+  if (matrices <= 0 || rows <= 0 || width <= 0) return SRB_OK;
+  dim3 grid;
+  if (mx4_grid(matrices, rows, width, &grid) != SRB_OK) return SRB_ERR_INVALID;
+  const int element = dtype == SRB_DTYPE_F32 ? 4 : 2;
+  const bool wide = ((uintptr_t)out & 15) == 0 && (long long)width * element % 16 == 0;
+  cudaStream_t s = (cudaStream_t)stream;
+  if (dtype == SRB_DTYPE_F32)
+    SRB_CUDA_CALL(srb_launch(wide ? mx4_dequantize_kernel<float, true> : mx4_dequantize_kernel<float, false>, grid, dim3(MX4_THREADS), 0, s,
+                             (const unsigned*)codes, (const unsigned*)scales, rows, width, (float*)out));
+  else if (dtype == SRB_DTYPE_BF16)
+    SRB_CUDA_CALL(srb_launch(wide ? mx4_dequantize_kernel<__nv_bfloat16, true> : mx4_dequantize_kernel<__nv_bfloat16, false>, grid,
+                             dim3(MX4_THREADS), 0, s, (const unsigned*)codes, (const unsigned*)scales, rows, width, (__nv_bfloat16*)out));
+  else
+    SRB_FAIL("mx4_dequantize: unknown dtype %d", dtype);
+  SRB_LAUNCH_CHECK("mx4_dequantize");
+  return SRB_OK;
+}

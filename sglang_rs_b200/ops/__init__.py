@@ -1911,3 +1911,9 @@ def count_picked(counts: torch.Tensor, index: torch.Tensor, picked: torch.Tensor
     _need(counts, "counts", torch.int32); _need(index, "index", torch.int32); _need(picked, "picked", torch.int32)
     lib = load_library("sampling")
     _check(lib, lib.srb_count_picked(_ptr(counts), counts.shape[1], _ptr(index), _ptr(picked), picked.numel(), _stream()))
+
+
+# --------------------------------------------------------------------------- matrices in four bits
+
+from .mx4 import (MX4_BLOCK, Mx4, choose_experts, chosen_experts_mx4, dequantize_mx4, linear_mx4, mx4_from_rows,  # noqa: E402,F401
+                  quantize_mx4)
