@@ -126,6 +126,59 @@ mx4_dequantize_kernel(const unsigned* __restrict__ codes, const unsigned* __rest
     if (k + i < width) dst[i] = srb_from_float<T>(v[i]);
 }
 
+// Rows of bfloat16 as the two eight-bit parts of mx4.cuh: parts [2, rows, 128 * column tiles] bytes, zero behind a row's last entry, and
+// their scales [2, row tiles, column tiles, 512] in the tiles of mx4.cuh (those of rows behind the last are not written: they are read,
+// but only for sums that nobody stores).
+template <bool WIDE>
+__global__ void __launch_bounds__(MX4_THREADS)
+mx4_split_kernel(const __nv_bfloat16* __restrict__ x, size_t pitch, int rows, int width, uint8_t* __restrict__ parts, uint8_t* __restrict__ scales) {
+  srb_launch_dependents();
+  srb_grid_dependency_wait();
+  const int k_tiles = mx4_tiles(width);
+  const int lane = threadIdx.x & 15;
+  const long long item = (long long)blockIdx.x * (MX4_THREADS / 16) + (threadIdx.x >> 4);
+  const int row = (int)(item / k_tiles), kt = (int)(item % k_tiles);
+  const bool live = row < rows;
+  const int k = kt * 128 + lane * 8;
+  float v[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = 0.f;
+  if (live) {
+    const __nv_bfloat16* src = x + (size_t)row * pitch + k;
+    if (WIDE && k + 8 <= width) mx4_unpack_bf16(*reinterpret_cast<const uint4*>(src), v);
+    else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (k + i < width) v[i] = srb_to_float(src[i]);
+    }
+  }
+  unsigned most = 0u;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) most = max(most, __float_as_uint(v[i]) & 0x7fffffffu);
+  most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
+  most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
+  const unsigned high = mx8_scale_high(most), low = mx8_scale_low(high);
+  unsigned h[4], l[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) mx8_split(v[2 * i], v[2 * i + 1], high, low, h[i], l[i]);
+  unsigned high_word = (lane & 3) == 0 ? high << (8 * (lane >> 2)) : 0u, low_word = (lane & 3) == 0 ? low << (8 * (lane >> 2)) : 0u;
+#pragma unroll
+  for (int offset = 4; offset <= 8; offset <<= 1) {
+    high_word |= __shfl_xor_sync(0xffffffffu, high_word, offset);
+    low_word |= __shfl_xor_sync(0xffffffffu, low_word, offset);
+  }
+  if (!live) return;
+  const size_t part = (size_t)rows * k_tiles * 128, scale_part = (size_t)mx4_tiles(rows) * k_tiles * MX4_TILE_BYTES;
+  uint8_t* dst = parts + (size_t)row * k_tiles * 128 + k;
+  *reinterpret_cast<uint2*>(dst) = make_uint2(h[0] | h[1] << 16, h[2] | h[3] << 16);
+  *reinterpret_cast<uint2*>(dst + part) = make_uint2(l[0] | l[1] << 16, l[2] | l[3] << 16);
+  if (lane == 0) {
+    uint8_t* word = scales + mx4_scale_word(row, kt, k_tiles);
+    *reinterpret_cast<unsigned*>(word) = high_word;
+    *reinterpret_cast<unsigned*>(word + scale_part) = low_word;
+  }
+}
+
 static int mx4_grid(int matrices, long long rows, int width, dim3* grid) {
   const long long items = rows * mx4_tiles(width), blocks = (items + MX4_THREADS / 16 - 1) / (MX4_THREADS / 16);
   if (blocks > 0x7fffffffll || matrices > 65535) SRB_FAIL("mx4: %d matrices of %lld rows of %d entries are too many", matrices, rows, width);
@@ -170,5 +223,16 @@ extern "C" int srb_mx4_dequantize(const void* codes, const void* scales, int mat
   else
     SRB_FAIL("mx4_dequantize: unknown dtype %d", dtype);
   SRB_LAUNCH_CHECK("mx4_dequantize");
+  return SRB_OK;
+}
+
+extern "C" int srb_mx4_split(const void* x, long long pitch, int rows, int width, void* parts, void* scales, void* stream) {
+  if (rows <= 0 || width <= 0) return SRB_OK;
+  dim3 grid;
+  if (mx4_grid(1, rows, width, &grid) != SRB_OK) return SRB_ERR_INVALID;
+  const bool wide = ((uintptr_t)x & 15) == 0 && pitch % 8 == 0;
+  SRB_CUDA_CALL(srb_launch(wide ? mx4_split_kernel<true> : mx4_split_kernel<false>, grid, dim3(MX4_THREADS), 0, (cudaStream_t)stream,
+                           (const __nv_bfloat16*)x, (size_t)pitch, rows, width, (uint8_t*)parts, (uint8_t*)scales));
+  SRB_LAUNCH_CHECK("mx4_split");
   return SRB_OK;
 }

@@ -33,3 +33,29 @@ __device__ __forceinline__ float mx4_code_value(unsigned code) {
   const float v = magnitude < 2u ? 0.5f * (float)magnitude : __uint_as_float(((126u + (magnitude >> 1)) << 23) | ((magnitude & 1u) << 22));
   return code & 8u ? -v : v;
 }
+
+// ---- a float as two parts of eight bits -----------------------------------------------------------------------------
+// The block-scaled products multiply four-bit entries with eight-bit ones (e4m3: four significant bits), so a row of more bits goes in as
+// two parts: the entries of a block over 2^(E - 7), E = floor(log2(largest magnitude)), rounded to e4m3, and what is left over a scale 2^5
+// less, rounded once more.  Four and four significant bits and the second part's sign hold the eight of a bfloat16: exactly, where an
+// entry is at least 2^-14 of its block's largest (below, e4m3 runs out of exponents); every entry to 2^-22 of the largest.
+__device__ __forceinline__ unsigned mx8_scale_high(unsigned largest_bits) {
+  return largest_bits >= 0x7f800000u ? 255u : (unsigned)max((int)(largest_bits >> 23) - 7, 0);
+}
+__device__ __forceinline__ unsigned mx8_scale_low(unsigned high) { return high == 255u ? 255u : (unsigned)max((int)high - 5, 0); }
+// Two entries: each part's bytes, the first entry's in the low half.  `high` and `low` are the parts' scales.
+__device__ __forceinline__ void mx8_split(float a, float b, unsigned high, unsigned low, unsigned& high_bytes, unsigned& low_bytes) {
+  if (high == 255u) { high_bytes = low_bytes = 0u; return; }
+  const float inverse = __uint_as_float((254u - high) << 23), onward = __uint_as_float((127u + high - low) << 23);
+  a *= inverse;
+  b *= inverse;
+  unsigned short h, l;
+  unsigned back;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %2, %1;" : "=h"(h) : "f"(a), "f"(b));
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(back) : "h"(h));
+  float back_a, back_b;
+  asm("{\n.reg .b16 x, y;\nmov.b32 {x, y}, %2;\ncvt.f32.f16 %0, x;\ncvt.f32.f16 %1, y;\n}\n" : "=f"(back_a), "=f"(back_b) : "r"(back));
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %2, %1;" : "=h"(l) : "f"((a - back_a) * onward), "f"((b - back_b) * onward));
+  high_bytes = h;
+  low_bytes = l;
+}

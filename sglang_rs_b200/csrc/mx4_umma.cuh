@@ -1,0 +1,41 @@
+// The block-scaled tensor-core instructions of sm_100 (tcgen05.mma ... block_scale) and what feeds them.
+//
+// Operands lie in shared memory in rows of 128 bytes with the 128-byte swizzle, as for the plain products; a step takes 32 bytes of a row: 64
+// four-bit entries (kind mxf4), or 32 entries of eight bits (kind mxf8f6f4), where four-bit entries stand 16 to 16 bytes, eight bytes of
+// codes and eight that are not read.  Scales lie in tensor memory: row r's in lane r % 32 (of every quarter of the lanes) and
+// column r / 32, a byte for each of four consecutive blocks of 32 entries; the instruction descriptor says which bytes a step takes.
+#pragma once
+#include "tcgen05_helpers.cuh"
+
+#define MX_E4M3 0u
+#define MX_E2M1 5u       // among the types of kind mxf8f6f4
+
+// kind mxf8f6f4: scales of 2^n, both operands K-major, M = 128.  The scale byte `k` of a word is ORed in by mx_idesc_step.
+__device__ __forceinline__ unsigned mx_idesc(unsigned a_type, unsigned b_type, int m, int n) {
+  return (a_type << 7) | (b_type << 10) | ((unsigned)(n >> 3) << 17) | (1u << 23) | ((unsigned)(m >> 4) << 24);
+}
+__device__ __forceinline__ unsigned mx_idesc_step(unsigned idesc, unsigned byte) { return idesc | (byte << 4) | (byte << 29); }
+
+__device__ __forceinline__ void umma_mx8(unsigned tmem_d, unsigned long long a_desc, unsigned long long b_desc, unsigned idesc, unsigned a_scales,
+                                         unsigned b_scales, unsigned accumulate) {
+  asm volatile(
+      "{\n.reg .pred p;\nsetp.ne.b32 p, %6, 0;\n"
+      "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n}\n"
+      ::"r"(tmem_d), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(a_scales), "r"(b_scales), "r"(accumulate) : "memory");
+}
+// 512 bytes of shared memory, 32 rows of 16, to four columns of all lanes (every quarter gets the 32 rows)
+__device__ __forceinline__ void tmem_copy_scales(unsigned tmem, unsigned long long desc) {
+  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
+}
+// rows of 16 bytes without swizzle, groups of eight rows 128 bytes apart
+__device__ __forceinline__ unsigned long long scales_descriptor(unsigned address) {
+  return (unsigned long long)((address & 0x3ffffu) >> 4) | ((unsigned long long)(128u >> 4) << 32) | (1ull << 46);
+}
+__device__ __forceinline__ void tmem_load_8(unsigned address, float (&v)[8]) {
+  unsigned r[8];
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]) : "r"(address) : "memory");
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(r[i]);
+}

@@ -138,6 +138,16 @@ def dequantize_mx4(q: Mx4, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     return out
 
 
+def _split(x: torch.Tensor):
+    """bfloat16 rows as the two eight-bit parts (and their scales) that multiply four-bit entries (csrc/mx4.cuh)."""
+    rows, width = x.shape
+    parts = torch.empty((2, rows, 128 * _tiles(width)), dtype=torch.uint8, device=x.device)
+    scales = torch.empty((2, _tiles(rows), _tiles(width), 512), dtype=torch.uint8, device=x.device)
+    lib = load_library("mx4")
+    _check(lib, lib.srb_mx4_split(_ptr(x), ctypes.c_longlong(x.stride(0)), rows, width, _ptr(parts), _ptr(scales), _stream()))
+    return parts, scales
+
+
 @traced("gemm")
 def linear_mx4(x, weight: Mx4, error_word: torch.Tensor, *, bias: Optional[torch.Tensor] = None,
                out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
@@ -168,10 +178,10 @@ def linear_mx4(x, weight: Mx4, error_word: torch.Tensor, *, bias: Optional[torch
     out = torch.empty((rows, weight.rows), dtype=out_dtype, device=weight.device)
     if out.numel():
         lib = load_library("gemm_mx4")
-        _check(lib, lib.srb_mx4_linear(_ptr(x.codes if four else x), _ptr(x.scales) if four else None,
-                                       ctypes.c_longlong(x.codes.stride(0) if four else x.stride(0)), _ptr(weight.codes), _ptr(weight.scales),
-                                       _ptr(bias), _ptr(out), ctypes.c_longlong(out.stride(0)), rows, weight.rows, width,
-                                       int(out_dtype == torch.float32), _ptr(error_word), _stream()))
+        held, scales = (x.codes, x.scales) if four else _split(x)
+        _check(lib, lib.srb_mx4_linear(_ptr(held), _ptr(scales), int(four), _ptr(weight.codes), _ptr(weight.scales), _ptr(bias), _ptr(out),
+                                       ctypes.c_longlong(out.stride(0)), rows, weight.rows, width, int(out_dtype == torch.float32),
+                                       _ptr(error_word), _stream()))
     return out
 
 
@@ -238,15 +248,19 @@ def chosen_experts_mx4(h: torch.Tensor, chosen: torch.Tensor, weights: torch.Ten
     plan = torch.empty(moe.srb_moe_plan_ints_of(rows, top, experts, tile), dtype=torch.int32, device=device)
     slot_row = torch.empty(entries, dtype=torch.int32, device=device)
     entry_slot = torch.empty(entries, dtype=torch.int32, device=device)
-    act = torch.empty((entries, inner), dtype=torch.bfloat16, device=device)
+    act = torch.empty((2, entries, 128 * _tiles(inner)), dtype=torch.uint8, device=device)
+    act_scales = torch.empty((2, _tiles(entries), _tiles(inner), 512), dtype=torch.uint8, device=device)
     y = torch.empty((entries, width), dtype=torch.float32, device=device)
     _check(moe, moe.srb_moe_plan_of(_ptr(chosen), rows, top, experts, tile, _ptr(plan), _ptr(slot_row), _ptr(entry_slot), None, None,
                                     _ptr(error_word), stream))
-    tiles = moe.srb_moe_max_tiles_of(rows, top, experts, tile)
-    _check(lib, lib.srb_mx4_experts(_ptr(h), ctypes.c_longlong(width), _ptr(slot_row), _ptr(w_gate_up.codes), _ptr(w_gate_up.scales), _ptr(act),
-                                    _ptr(plan), tiles, experts, inner, width, GEMM_MODES["gated" if gated else "act"], act_code,
-                                    ctypes.c_float(activation_param), _ptr(error_word), stream))
-    _check(lib, lib.srb_mx4_experts(_ptr(act), ctypes.c_longlong(inner), None, _ptr(w_down.codes), _ptr(w_down.scales), _ptr(y),
-                                    _ptr(plan), tiles, experts, width, inner, GEMM_MODES["f32"], 0, ctypes.c_float(0.0), _ptr(error_word), stream))
+    # a tile has a slot at least
+    tiles = min(entries, moe.srb_moe_max_tiles_of(rows, top, experts, tile))
+    parts, scales = _split(h)
+    _check(lib, lib.srb_mx4_experts(_ptr(parts), _ptr(scales), rows, _ptr(slot_row), _ptr(w_gate_up.codes), _ptr(w_gate_up.scales), _ptr(act),
+                                    _ptr(act_scales), _ptr(plan), tiles, entries, experts, inner, width, GEMM_MODES["gated" if gated else "act"],
+                                    act_code, ctypes.c_float(activation_param), _ptr(error_word), stream))
+    _check(lib, lib.srb_mx4_experts(_ptr(act), _ptr(act_scales), entries, None, _ptr(w_down.codes), _ptr(w_down.scales), _ptr(y), None,
+                                    _ptr(plan), tiles, entries, experts, width, inner, GEMM_MODES["f32"], 0, ctypes.c_float(0.0),
+                                    _ptr(error_word), stream))
     _check(lib, lib.srb_mx4_combine(_ptr(y), _ptr(entry_slot), _ptr(weights), rows, top, width, _ptr(out), stream))
     return out
