@@ -1,0 +1,564 @@
+// Y = X W^T with W in the microscaled four-bit format of mx4.cuh for many rows: tiles of 256 rows of X x 192 rows of W on pairs of CTAs
+// (tcgen05.mma.cta_group::2 with block scales), in a persistent loop.
+//
+// Two kinds of rows.  FOUR: X in four bits too; both operands and their scales come by TMA as they lie, a step is 256 entries, four
+// products of kind mxf4 (64 entries each, four times bfloat16's rate).  Otherwise X is the two eight-bit parts of a bfloat16 (mx4.cuh): a
+// step is 128 entries, four products of kind mxf8f6f4 for each part into the same sums (each at twice bfloat16's rate); they want the codes of W
+// eight bytes to each 16, so four warps bring those, and the scales of W, by cp.async.  Nothing is unpacked in either.
+//
+// CTA r of a pair has 128 rows of X (the M side) and 96 rows of W (half of the N side) in shared memory, and in tensor memory two
+// buffers of 192 columns of sums for its rows of X, a row a lane, beside 128 columns of scales (256 columns of sums twice would leave none).  Scales
+// go from shared to tensor memory ahead of a step's products, in the same queue; steps use places in turn.
+//
+// Over experts (GROUPED) a tile is up to 256 slots of one expert (the plan of csrc/moe.cu); X and the parts that the gated mode leaves have room
+// for 256 rows a tile, so that a tile's scales are whole tiles.  Gated: the even CTA brings gate rows, the odd one the up rows of the same 96 features.
+//
+// Warps: 0 TMA, 1 products (even CTA) and tensor memory, then four for W where X is parts, then twelve of the epilogue: a quarter of the lanes
+// and a third of the columns each.  Waits are bounded; one that runs out flags SRB_FLAG_WAIT_TIMEOUT.
+#include "common.cuh"
+#include "activations.cuh"
+#include "mx4.cuh"
+#include "mx4_umma.cuh"
+#include <algorithm>
+#include <mutex>
+
+SRB_DEFINE_LAST_ERROR()
+SRB_DEFINE_PDL_SWITCH()
+
+#define MXP_ROWS 128             // rows of X of a CTA
+#define MXP_TILE 256             // ... of a pair
+#define MXP_N 192                // rows of W of a pair
+#define MXP_HALF 96
+#define MXP_EPILOGUE_WARPS 12
+#define MXP_BOX_BYTES 2048       // a warp's piece of the output: 32 rows x 64 bytes, swizzled
+#define MXP_A_BYTES (MXP_ROWS * 128)
+#define MXP_B_BYTES (MXP_HALF * 128)
+#define MXP_COPIES_AHEAD 2       // steps of W that the copy warps have issued beyond the one that they hand over
+#define MXP_SUMS 384             // columns of tensor memory: scales lie behind
+#define MXP_BF16 0
+#define MXP_F32 1
+#define MXP_GATED 2
+#define MXP_ACT 5
+
+template <bool FOUR> struct PairShape {
+  static constexpr int STAGES = FOUR ? 6 : 4;
+  static constexpr int PARTS = FOUR ? 1 : 2;
+  static constexpr int B_AT = PARTS * MXP_A_BYTES;
+  static constexpr int XS_AT = B_AT + MXP_B_BYTES;           // scales of X: two column tiles, or a tile of each part
+  static constexpr int WS_AT = XS_AT + 1024;                 // of W: two row tiles of each column tile, or 192 rows in order
+  static constexpr int STAGE_BYTES = WS_AT + (FOUR ? 2048 : 1024);
+  static constexpr int TMA_BYTES = FOUR ? STAGE_BYTES : 2 * MXP_A_BYTES + 1024;    // a CTA's by TMA
+  static constexpr int COPY_WARPS = FOUR ? 0 : 4;
+  static constexpr int THREADS = 32 * (2 + COPY_WARPS + MXP_EPILOGUE_WARPS);
+  static constexpr int PLACE_COLUMNS = FOUR ? 24 : 16;       // of scales of a step
+  static constexpr int PLACES = FOUR ? 5 : 4;
+};
+
+struct PairMx4Args {
+  const uint8_t* w;
+  const uint8_t* w_scales;
+  const float* bias;
+  void* out;
+  uint8_t* out_scales;           // of parts
+  size_t ldo;                    // elements; bytes of parts
+  size_t out_part, os_part;
+  int rows, features, w_rows, k_tiles;
+  int x_lo_row, xs_lo_tile;      // where the second part's rows and tiles of scales begin
+  int tiles_t, tiles_f;
+  int activation;
+  float act_param;
+  int* error_word;
+  const int* plan;               // GROUPED
+  int experts;
+};
+
+__device__ __forceinline__ void cp_async_8(unsigned dst, const void* src, int bytes) {
+  asm volatile("cp.async.ca.shared.global.L2::128B [%0], [%1], 8, %2;\n" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async_4(unsigned dst, const void* src, int bytes) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;\n" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void pair_tmem_alloc(unsigned holder) {
+  asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(holder), "r"(512) : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void pair_tmem_dealloc(unsigned address) {
+  asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(address), "r"(512) : "memory");
+}
+// arrives on the barrier at this offset in both CTAs once the products and copies issued so far are done
+__device__ __forceinline__ void pair_commit(unsigned bar) {
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+               ::"r"(bar), "h"((unsigned short)3) : "memory");
+}
+// a copy whose bytes count on the even CTA's barrier (bit 24 of a shared address names the odd CTA)
+__device__ __forceinline__ void pair_tma_load(unsigned dst, const CUtensorMap* map, unsigned bar, int x, int y) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+      ::"r"(dst), "l"(map), "r"(bar & 0xFEFFFFFFu), "r"(x), "r"(y) : "memory");
+}
+__device__ __forceinline__ void arrive_at(unsigned bar, unsigned rank) {
+  asm volatile("{\n.reg .b32 remote;\nmapa.shared::cluster.u32 remote, %0, %1;\n"
+               "mbarrier.arrive.release.cluster.shared::cluster.b64 _, [remote];\n}\n" ::"r"(bar), "r"(rank) : "memory");
+}
+__device__ __forceinline__ void pair_tma_store(const CUtensorMap* map, unsigned src, int x, int y) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];"
+               ::"l"(map), "r"(src), "r"(x), "r"(y) : "memory");
+  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+__device__ __forceinline__ void pair_stores_have_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+__device__ __forceinline__ void store_16(unsigned at, unsigned a, unsigned b, unsigned c, unsigned d) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+__device__ __forceinline__ unsigned two_bf16(float low, float high) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(low, high);
+  return *reinterpret_cast<const unsigned*>(&v);
+}
+
+// What a tile is, the same in every role of both CTAs.
+struct PairMx4Tile {
+  int feature0;                  // the first output feature
+  int x_row0;                    // the first row of X (of the padded ones, over experts)
+  int out_row0, limit;           // the first row (or slot) of the result, and where the tile's rows end
+  int matrix;
+};
+template <int MODE, bool GROUPED>
+__device__ __forceinline__ PairMx4Tile pair_mx4_tile(const PairMx4Args& a, int tile) {
+  constexpr int FEATURES = MODE == MXP_GATED ? MXP_HALF : MXP_N;
+  PairMx4Tile t;
+  if (GROUPED) {
+    // the features of a row tile follow one another: its rows stay in L2, and an expert's weights are streamed once
+    const int* first_slot = a.plan + 1;
+    const int* tiles = first_slot + a.experts + 1;
+    const int rt = tile / a.tiles_f;
+    t.matrix = tiles[2 * rt];
+    t.feature0 = (tile % a.tiles_f) * FEATURES;
+    t.x_row0 = rt * MXP_TILE;
+    t.out_row0 = tiles[2 * rt + 1];
+    t.limit = min(t.out_row0 + MXP_TILE, first_slot[t.matrix + 1]);
+  } else {
+    t.matrix = 0;
+    t.feature0 = tile / a.tiles_t * FEATURES;
+    t.x_row0 = t.out_row0 = tile % a.tiles_t * MXP_TILE;
+    t.limit = a.rows;
+  }
+  return t;
+}
+
+template <bool FOUR, int MODE, bool GROUPED>
+__global__ void __launch_bounds__(PairShape<FOUR>::THREADS, 1)
+mx4_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_xs, const __grid_constant__ CUtensorMap map_w,
+                const __grid_constant__ CUtensorMap map_ws, const __grid_constant__ CUtensorMap map_out, const PairMx4Args a) {
+  using Shape = PairShape<FOUR>;
+  constexpr int STAGES = Shape::STAGES;
+  constexpr bool GATED = MODE == MXP_GATED, PARTS = MODE == MXP_GATED || MODE == MXP_ACT;
+  extern __shared__ unsigned char smem_unaligned[];
+  unsigned char* smem = reinterpret_cast<unsigned char*>(((uintptr_t)smem_unaligned + 1023) & ~(uintptr_t)1023);
+  __shared__ __align__(8) unsigned long long full_bar[STAGES], empty_bar[STAGES], acc_full[2], acc_empty[2];
+  __shared__ unsigned tmem_holder;
+  __shared__ int abort_flag;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const unsigned rank = srb_cluster_rank();                  // 0: the CTA that issues the products
+  const int pair = blockIdx.x >> 1, num_pairs = gridDim.x >> 1;
+  const int steps = FOUR ? (a.k_tiles + 1) / 2 : a.k_tiles;
+
+  if (threadIdx.x == 0) {
+    abort_flag = 0;
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(smem_u32(&full_bar[s]), 1 + 2 * Shape::COPY_WARPS);
+      mbar_init(smem_u32(&empty_bar[s]), 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(smem_u32(&acc_full[b]), 1);
+      mbar_init(smem_u32(&acc_empty[b]), 2 * MXP_EPILOGUE_WARPS);
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) pair_tmem_alloc(smem_u32(&tmem_holder));
+  tc_fence_before();
+  srb_cluster_sync();
+  tc_fence_after();
+  const unsigned tmem = tmem_holder;
+  srb_launch_dependents();
+  srb_grid_dependency_wait();
+  const int num_tiles = GROUPED ? a.plan[0] * a.tiles_f : a.tiles_t * a.tiles_f;
+
+  if (warp == 0) {
+    // ---- TMA: each CTA its own halves; the bytes count on the even CTA's barrier
+    int issued = 0;
+    unsigned round = 0;
+    bool ok = true;
+    for (int tile = pair; tile < num_tiles && ok; tile += num_pairs) {
+      const PairMx4Tile t = pair_mx4_tile<MODE, GROUPED>(a, tile);
+      const int x_row = t.x_row0 + (int)rank * MXP_ROWS, xs_tile = (x_row >> 7) * a.k_tiles;
+      const int w_row = t.feature0 + (int)rank * MXP_HALF, ws_tile = (t.feature0 >> 7) * a.k_tiles;
+      for (int i = 0; i < steps && ok; ++i, ++round) {
+        const int s = (int)(round % STAGES);
+        ok = mbar_wait_warp(smem_u32(&empty_bar[s]), ((round / STAGES) & 1u) ^ 1u, &abort_flag);
+        if (!ok) break;
+        const unsigned bar = smem_u32(&full_bar[s]), stage = smem_u32(smem) + s * Shape::STAGE_BYTES;
+        if (elect_one()) {
+          if (rank == 0) mbar_expect_tx(bar, 2 * Shape::TMA_BYTES);
+          pair_tma_load(stage, &map_x, bar, i * 128, x_row);
+          if (FOUR) {
+            pair_tma_load(stage + Shape::B_AT, &map_w, bar, i * 128, w_row);
+            pair_tma_load(stage + Shape::XS_AT, &map_xs, bar, 0, xs_tile + 2 * i);
+            pair_tma_load(stage + Shape::WS_AT, &map_ws, bar, 0, ws_tile + 2 * i);
+            pair_tma_load(stage + Shape::WS_AT + 1024, &map_ws, bar, 0, ws_tile + a.k_tiles + 2 * i);
+          } else {
+            pair_tma_load(stage + MXP_A_BYTES, &map_x, bar, i * 128, a.x_lo_row + x_row);
+            pair_tma_load(stage + Shape::XS_AT, &map_xs, bar, 0, xs_tile + i);
+            pair_tma_load(stage + Shape::XS_AT + 512, &map_xs, bar, 0, a.xs_lo_tile + xs_tile + i);
+          }
+        }
+        ++issued;
+      }
+    }
+    // copies in flight when a wait ran out write into this CTA's memory: give them time to land
+    if (abort_flag && issued > 0) {
+      const long long start = clock64();
+      while (clock64() - start < 4000000ll) {}
+    }
+  } else if (warp == 1) {
+    if (rank == 0) {
+      // ---- products of the pair
+      const unsigned idesc = FOUR ? mx_idesc_four(2 * MXP_ROWS, MXP_N) : mx_idesc(MX_E4M3, MX_E2M1, 2 * MXP_ROWS, MXP_N);
+      unsigned round = 0;
+      int local = 0;
+      bool ok = true;
+      for (int tile = pair; tile < num_tiles && ok; tile += num_pairs, ++local) {
+        const int b = local & 1;
+        ok = mbar_wait_warp_cluster(smem_u32(&acc_empty[b]), (((unsigned)local >> 1) & 1u) ^ 1u, &abort_flag);
+        if (!ok) break;
+        tc_fence_after();
+        const unsigned acc = tmem + b * MXP_N;
+        // a tile of W that starts in the middle of a tile of scales
+        const unsigned shift = FOUR ? (unsigned)(pair_mx4_tile<MODE, GROUPED>(a, tile).feature0 & 127) >> 5 : 0u;
+        for (int i = 0; i < steps && ok; ++i, ++round) {
+          const int s = (int)(round % STAGES);
+          ok = mbar_wait_warp_cluster(smem_u32(&full_bar[s]), (round / STAGES) & 1u, &abort_flag);
+          if (!ok) break;
+          tc_fence_after();
+          const unsigned stage = smem_u32(smem) + s * Shape::STAGE_BYTES;
+          const unsigned place = tmem + MXP_SUMS + (round % Shape::PLACES) * Shape::PLACE_COLUMNS;
+          const unsigned long long a_desc = smem_descriptor(stage), b_desc = smem_descriptor(stage + Shape::B_AT);
+          if (elect_one()) {
+            const unsigned long long xs = scales_descriptor(stage + Shape::XS_AT), ws = scales_descriptor(stage + Shape::WS_AT);
+            tmem_copy_scales_pair(place, xs);
+            tmem_copy_scales_pair(place + 4, xs + (512 >> 4));
+            if (FOUR) {
+              // rows of the first row tile, of the second; this column tile, the next
+              tmem_copy_scales_pair(place + 8, ws);
+              tmem_copy_scales_pair(place + 12, ws + (1024 >> 4));
+              tmem_copy_scales_pair(place + 16, ws + (512 >> 4));
+              tmem_copy_scales_pair(place + 20, ws + (1536 >> 4));
+              const unsigned products = 2 * i + 1 < a.k_tiles ? 4u : 2u;
+#pragma unroll
+              for (unsigned k = 0; k < 4; ++k)
+                if (k < products)
+                  umma_mx4_pair(acc, a_desc + 2 * k, b_desc + 2 * k, mx_idesc_step(idesc, 2 * (k & 1)), place + 4 * (k >> 1),
+                                place + 8 + 8 * (k >> 1) + shift, (i > 0 || k > 0) ? 1u : 0u);
+            } else {
+              tmem_copy_scales_pair(place + 8, ws);
+              tmem_copy_scales_pair(place + 12, ws + (512 >> 4));
+#pragma unroll
+              for (unsigned k = 0; k < 8; ++k)
+                umma_mx8_pair(acc, a_desc + (k >> 2) * (MXP_A_BYTES >> 4) + 2 * (k & 3), b_desc + 2 * (k & 3), mx_idesc_step(idesc, k & 3),
+                              place + 4 * (k >> 2), place + 8, (i > 0 || k > 0) ? 1u : 0u);
+            }
+            pair_commit(smem_u32(&empty_bar[s]));
+            if (i == steps - 1) pair_commit(smem_u32(&acc_full[b]));
+          }
+          __syncwarp();
+        }
+      }
+    }
+  } else if (warp < 2 + Shape::COPY_WARPS) {
+    // ---- codes of W, eight bytes to each 16, and the scales of all 192 rows: chunk t % 8 of rows t / 8 + 16 i, scales of row t (and 128 + t)
+    const int t = threadIdx.x - 64, chunk = t & 7, sub = t >> 3;
+    const unsigned to = (unsigned)(chunk ^ (sub & 7)) << 4;
+    const size_t w_pitch = (size_t)a.k_tiles * 64;
+    unsigned round = 0, landed = 0;
+    bool ok = true;
+    auto land = [&]() {
+      fence_proxy_async_shared();
+      __syncwarp();
+      if (lane == 0) arrive_at(smem_u32(&full_bar[landed % STAGES]), 0);
+      ++landed;
+    };
+    for (int tile = pair; tile < num_tiles && ok; tile += num_pairs) {
+      const PairMx4Tile tl = pair_mx4_tile<MODE, GROUPED>(a, tile);
+      const uint8_t* w = a.w + (size_t)tl.matrix * a.w_rows * w_pitch;
+      const uint8_t* w_scales = a.w_scales + (size_t)tl.matrix * mx4_tiles(a.w_rows) * a.k_tiles * MX4_TILE_BYTES;
+      // row n of the N side
+      auto w_row = [&](int n, bool& live) {
+        const int feature = tl.feature0 + (GATED && n >= MXP_HALF ? n - MXP_HALF : n);
+        live = feature < a.features;
+        return !live ? 0 : GATED && n >= MXP_HALF ? a.features + feature : feature;
+      };
+      const uint8_t* w_at[6];
+      unsigned live = 0u;
+#pragma unroll
+      for (int i = 0; i < 6; ++i) {
+        bool here;
+        w_at[i] = w + (size_t)w_row((int)rank * MXP_HALF + sub + 16 * i, here) * w_pitch + chunk * 8;
+        live |= (unsigned)here << i;
+      }
+      bool first_live, second_live;
+      const size_t first_word = mx4_scale_word(w_row(t, first_live), 0, a.k_tiles);
+      const size_t second_word = mx4_scale_word(w_row(128 + (t & 63), second_live), 0, a.k_tiles);
+      for (int i = 0; i < steps; ++i, ++round) {
+        const int s = (int)(round % STAGES);
+        ok = mbar_wait_warp(smem_u32(&empty_bar[s]), ((round / STAGES) & 1u) ^ 1u, &abort_flag);
+        if (!ok) break;
+        const unsigned stage = smem_u32(smem) + s * Shape::STAGE_BYTES;
+#pragma unroll
+        for (int j = 0; j < 6; ++j)
+          cp_async_8(stage + Shape::B_AT + (sub + 16 * j) * 128 + to, w_at[j] + (size_t)i * 64, (live >> j) & 1u ? 8 : 0);
+        const unsigned word = stage + Shape::WS_AT + lane * 16 + ((t >> 5) << 2);
+        cp_async_4(word, w_scales + first_word + (size_t)i * MX4_TILE_BYTES, first_live ? 4 : 0);
+        if (t < 64) cp_async_4(word + 512, w_scales + second_word + (size_t)i * MX4_TILE_BYTES, second_live ? 4 : 0);
+        asm volatile("cp.async.commit_group;\n" ::: "memory");
+        if (round >= MXP_COPIES_AHEAD) {
+          asm volatile("cp.async.wait_group %0;\n" ::"n"(MXP_COPIES_AHEAD) : "memory");
+          land();
+        }
+      }
+    }
+    asm volatile("cp.async.wait_group 0;\n" ::: "memory");
+    if (ok)
+      while (landed < round) land();
+  } else {
+    // ---- epilogue: warp w has lanes 32 * (w % 4) .. + 31 of its CTA's tensor memory, a row of X a lane, and a third of the columns
+    const int quarter = warp & 3, third = (warp - 2 - Shape::COPY_WARPS) >> 2;
+    const unsigned lane_address = tmem + ((unsigned)(quarter * 32) << 16);
+    const unsigned box = smem_u32(smem) + STAGES * Shape::STAGE_BYTES + (warp - 2 - Shape::COPY_WARPS) * MXP_BOX_BYTES;
+    int local = 0;
+    for (int tile = pair; tile < num_tiles; tile += num_pairs, ++local) {
+      const int b = local & 1;
+      const PairMx4Tile t = pair_mx4_tile<MODE, GROUPED>(a, tile);
+      const int first = t.out_row0 + (int)rank * MXP_ROWS + quarter * 32, live = min(t.limit - first, 32);
+      if (!mbar_wait_warp(smem_u32(&acc_full[b]), ((unsigned)local >> 1) & 1u, &abort_flag)) break;
+      tc_fence_after();
+      const unsigned sums = lane_address + b * MXP_N;
+      if (live > 0) {
+        if (PARTS) {
+          // a lane's 32 features are a block of the next product's rows
+#pragma unroll 1
+          for (int part = 0; part < (GATED ? 1 : 2); ++part) {
+            const int column = GATED ? third * 32 : third * 64 + part * 32, feature = t.feature0 + column;
+            if (feature >= (int)a.ldo) continue;
+            float v[32];
+            tmem_load_32(sums + column, v);
+            if (GATED) {
+              float up[32];
+              tmem_load_32(sums + MXP_HALF + column, up);
+#pragma unroll
+              for (int j = 0; j < 32; ++j) v[j] = srb_gated<true>(a.activation, lane < live ? v[j] : 1.0f, up[j], a.act_param);
+            } else {
+#pragma unroll
+              for (int j = 0; j < 32; ++j) v[j] = srb_gated<true>(a.activation, lane < live ? v[j] : 1.0f, 1.0f, a.act_param);
+            }
+            if (feature + 32 > a.features) {
+#pragma unroll
+              for (int j = 0; j < 32; ++j)
+                if (feature + j >= a.features) v[j] = 0.f;   // the part that pads the parts' rows
+            }
+            if (lane < live) {
+              unsigned most = 0u;
+#pragma unroll
+              for (int j = 0; j < 32; ++j) most = max(most, __float_as_uint(v[j]) & 0x7fffffffu);
+              const unsigned high = mx8_scale_high(most), low = mx8_scale_low(high);
+              unsigned h[8], l[8];
+#pragma unroll
+              for (int j = 0; j < 8; ++j) {
+                unsigned h0, l0, h1, l1;
+                mx8_split(v[4 * j], v[4 * j + 1], high, low, h0, l0);
+                mx8_split(v[4 * j + 2], v[4 * j + 3], high, low, h1, l1);
+                h[j] = h0 | h1 << 16;
+                l[j] = l0 | l1 << 16;
+              }
+              const int row = t.x_row0 + (int)rank * MXP_ROWS + quarter * 32 + lane;
+              uint8_t* dst = reinterpret_cast<uint8_t*>(a.out) + (size_t)row * a.ldo + feature;
+              reinterpret_cast<uint4*>(dst)[0] = make_uint4(h[0], h[1], h[2], h[3]);
+              reinterpret_cast<uint4*>(dst)[1] = make_uint4(h[4], h[5], h[6], h[7]);
+              reinterpret_cast<uint4*>(dst + a.out_part)[0] = make_uint4(l[0], l[1], l[2], l[3]);
+              reinterpret_cast<uint4*>(dst + a.out_part)[1] = make_uint4(l[4], l[5], l[6], l[7]);
+              uint8_t* scale = a.out_scales + mx4_scale_word(row, feature >> 7, (int)(a.ldo / 128)) + ((feature >> 5) & 3);
+              scale[0] = (uint8_t)high;
+              scale[a.os_part] = (uint8_t)low;
+            }
+          }
+        } else {
+#pragma unroll 1
+          for (int part = 0; part < 2; ++part) {
+            const int column = third * 64 + part * 32, feature = t.feature0 + column;
+            if (feature >= a.features) continue;
+            float v[32];
+            tmem_load_32(sums + column, v);
+            if (a.bias) {
+#pragma unroll
+              for (int j = 0; j < 32; ++j) v[j] += feature + j < a.features ? __ldg(a.bias + feature + j) : 0.f;
+            }
+            if (GROUPED && live < 32) {
+              // the rows behind the expert's last slot belong to the next one
+              float* dst = reinterpret_cast<float*>(a.out) + (size_t)(first + lane) * a.ldo + feature;
+              if (lane < live) {
+#pragma unroll
+                for (int j = 0; j < 32; ++j)
+                  if (feature + j < a.features) dst[j] = v[j];
+              }
+              continue;
+            }
+            // 64 bytes of a row: 32 features in bfloat16, 16 in float; a 16-byte piece goes where the store's 64-byte swizzle wants it
+            const unsigned row = box + lane * 64;
+            const unsigned turn = (unsigned)(lane >> 1) & 3u;
+#pragma unroll
+            for (int half = 0; half < (MODE == MXP_F32 ? 2 : 1); ++half) {
+              if (lane == 0) pair_stores_have_read();
+              __syncwarp();
+#pragma unroll
+              for (unsigned i = 0; i < 4; ++i) {
+                if (MODE == MXP_F32) {
+                  const float* q = v + 16 * half + 4 * i;
+                  store_16(row + ((i ^ turn) << 4), __float_as_uint(q[0]), __float_as_uint(q[1]), __float_as_uint(q[2]), __float_as_uint(q[3]));
+                } else {
+                  const float* q = v + 8 * i;
+                  store_16(row + ((i ^ turn) << 4), two_bf16(q[0], q[1]), two_bf16(q[2], q[3]), two_bf16(q[4], q[5]), two_bf16(q[6], q[7]));
+                }
+              }
+              fence_proxy_async_shared();
+              __syncwarp();
+              if (lane == 0 && feature + 16 * half < a.features) pair_tma_store(&map_out, box, feature + 16 * half, first);
+            }
+          }
+        }
+      }
+      // the buffer is free for the tile after next
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) arrive_at(smem_u32(&acc_empty[b]), 0);
+    }
+    if (lane == 0) pair_stores_have_read();                  // before this block's shared memory goes
+    tc_fence_before();
+  }
+  __syncwarp();
+  srb_cluster_sync();                                        // nobody leaves while the other CTA may still signal or read
+  if (threadIdx.x == 0 && abort_flag) atomicOr(a.error_word, SRB_FLAG_WAIT_TIMEOUT);
+  if (warp == 1) {
+    tc_fence_after();
+    pair_tmem_dealloc(tmem);
+  }
+}
+
+// ------------------------------------------------------------------------------- host side
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                  const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+static EncodeTiledFn encode_tiled() {
+  static EncodeTiledFn fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* entry = nullptr;
+    cudaDriverEntryPointQueryResult result;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &entry, 12000, cudaEnableDefault, &result) == cudaSuccess &&
+        result == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<EncodeTiledFn>(entry);
+  });
+  return fn;
+}
+
+// A matrix [rows, columns] of elements of `type`, `pitch` bytes apart, cut into boxes.
+static int make_map(CUtensorMap* map, CUtensorMapDataType type, const void* base, long long rows, long long columns, long long pitch,
+                    int box_rows, int box_columns, CUtensorMapSwizzle swizzle) {
+  EncodeTiledFn fn = encode_tiled();
+  if (!fn) SRB_FAIL("gemm_mx4_pair: the driver does not offer cuTensorMapEncodeTiled");
+  const cuuint64_t dims[2] = {(cuuint64_t)columns, (cuuint64_t)rows};
+  const cuuint64_t strides[1] = {(cuuint64_t)pitch};
+  const cuuint32_t box[2] = {(cuuint32_t)box_columns, (cuuint32_t)box_rows};
+  const cuuint32_t element[2] = {1, 1};
+  const CUresult status = fn(map, type, 2, const_cast<void*>(base), dims, strides, box, element, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+                             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (status != CUDA_SUCCESS) SRB_FAIL("gemm_mx4_pair: cuTensorMapEncodeTiled failed with %d", (int)status);
+  return SRB_OK;
+}
+static int make_bytes_map(CUtensorMap* map, const void* base, long long rows, long long bytes, int box_rows) {
+  return make_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, base, rows, bytes, bytes, box_rows, 128, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+static int make_scales_map(CUtensorMap* map, const void* base, long long tiles, int at_once) {
+  return make_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, base, tiles, 128, MX4_TILE_BYTES, at_once, 128, CU_TENSOR_MAP_SWIZZLE_NONE);
+}
+
+template <bool FOUR, int MODE, bool GROUPED>
+static int launch_pair(const CUtensorMap (&maps)[5], const PairMx4Args& a, int max_tiles, cudaStream_t s) {
+  using Shape = PairShape<FOUR>;
+  const int pairs = std::max(1, std::min(srb_sm_count() / 2, max_tiles));
+  const size_t smem = (size_t)Shape::STAGES * Shape::STAGE_BYTES + MXP_EPILOGUE_WARPS * MXP_BOX_BYTES + 1024;
+  auto kernel = mx4_pair_kernel<FOUR, MODE, GROUPED>;
+  SRB_CUDA_CALL(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  SRB_CUDA_CALL(srb_launch_clustered(kernel, dim3(2 * pairs), dim3(Shape::THREADS), smem, s, dim3(2), maps[0], maps[1], maps[2], maps[3], maps[4], a));
+  SRB_LAUNCH_CHECK("mx4_pair");
+  return SRB_OK;
+}
+
+// As srb_mx4_linear of gemm_mx4.cu, for many rows; out's rows are `ldo` elements apart, a multiple of 16 bytes.
+extern "C" int srb_mx4_linear_pair(const void* x, const void* x_scales, int four, const void* w, const void* w_scales, const float* bias,
+                                   void* out, long long ldo, int rows, int features, int width, int out_float, int* error_word, void* stream) {
+  if (rows <= 0 || features <= 0) return SRB_OK;
+  if (width <= 0) SRB_FAIL("mx4_linear_pair: inner size %d must be positive", width);
+  if (((uintptr_t)out & 15) || ldo * (out_float ? 4 : 2) % 16) SRB_FAIL("mx4_linear_pair: rows of the result must start on 16-byte borders");
+  PairMx4Args a = {};
+  a.w = (const uint8_t*)w; a.w_scales = (const uint8_t*)w_scales; a.bias = bias; a.out = out; a.ldo = ldo; a.rows = rows;
+  a.features = a.w_rows = features; a.k_tiles = mx4_tiles(width); a.error_word = error_word;
+  a.x_lo_row = rows; a.xs_lo_tile = mx4_tiles(rows) * a.k_tiles;
+  a.tiles_t = (rows + MXP_TILE - 1) / MXP_TILE; a.tiles_f = (features + MXP_N - 1) / MXP_N;
+  const long long row_tiles = mx4_tiles(rows), tiles = (long long)a.tiles_t * a.tiles_f;
+  if (tiles > 0x3fffffff || 2ll * row_tiles * 128 > 0x7fffffff) SRB_FAIL("mx4_linear_pair: %d rows x %d features are too many", rows, features);
+  CUtensorMap maps[5];
+  if (make_bytes_map(&maps[0], x, four ? rows : 2ll * rows, a.k_tiles * (four ? 64 : 128), MXP_ROWS) != SRB_OK ||
+      make_scales_map(&maps[1], x_scales, (four ? 1 : 2) * row_tiles * a.k_tiles, four ? 2 : 1) != SRB_OK ||
+      make_bytes_map(&maps[2], w, features, a.k_tiles * 64, MXP_HALF) != SRB_OK ||
+      make_scales_map(&maps[3], w_scales, (long long)mx4_tiles(features) * a.k_tiles, 2) != SRB_OK ||
+      make_map(&maps[4], out_float ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, out, rows, features, ldo * (out_float ? 4 : 2),
+               32, out_float ? 16 : 32, CU_TENSOR_MAP_SWIZZLE_64B) != SRB_OK)
+    return SRB_ERR_INVALID;
+  cudaStream_t s = (cudaStream_t)stream;
+  if (four) return out_float ? launch_pair<true, MXP_F32, false>(maps, a, (int)tiles, s) : launch_pair<true, MXP_BF16, false>(maps, a, (int)tiles, s);
+  return out_float ? launch_pair<false, MXP_F32, false>(maps, a, (int)tiles, s) : launch_pair<false, MXP_BF16, false>(maps, a, (int)tiles, s);
+}
+
+// The experts' products over the plan's tiles of 256 slots.  x: parts [2, 256 max_tiles, 128 k_tiles] and their scales, 256 rows a tile.  Mode gated /
+// act: out parts [2, 256 max_tiles, 128 ceil(features / 128)], out_scales theirs; float: out [slots, features], rows on 16-byte borders.
+extern "C" int srb_mx4_experts_pair(const void* x, const void* x_scales, const void* w, const void* w_scales, void* out, void* out_scales,
+                                    const int* plan, int max_tiles, int slots, int experts, int features, int width, int mode, int activation,
+                                    float act_param, int* error_word, void* stream) {
+  if (max_tiles <= 0 || features <= 0) return SRB_OK;
+  if (width <= 0) SRB_FAIL("mx4_experts_pair: inner size %d must be positive", width);
+  if (activation < 0 || activation >= SRB_ACT_COUNT) SRB_FAIL("mx4_experts_pair: unknown activation %d", activation);
+  if (mode != MXP_F32 && mode != MXP_GATED && mode != MXP_ACT) SRB_FAIL("mx4_experts_pair: mode %d is not float, gated or activated", mode);
+  PairMx4Args a = {};
+  a.w = (const uint8_t*)w; a.w_scales = (const uint8_t*)w_scales; a.out = out; a.out_scales = (uint8_t*)out_scales; a.rows = slots;
+  a.features = features; a.w_rows = mode == MXP_GATED ? 2 * features : features; a.k_tiles = mx4_tiles(width); a.activation = activation;
+  a.act_param = act_param; a.error_word = error_word; a.plan = plan; a.experts = experts;
+  const long long rows = 256ll * max_tiles;
+  const int out_tiles = mx4_tiles(features);
+  a.x_lo_row = (int)rows; a.xs_lo_tile = 2 * max_tiles * a.k_tiles;
+  const int covered = mode == MXP_F32 ? features : 128 * out_tiles, per_tile = mode == MXP_GATED ? MXP_HALF : MXP_N;
+  a.tiles_f = (covered + per_tile - 1) / per_tile;
+  a.ldo = mode == MXP_F32 ? features : 128 * out_tiles;
+  a.out_part = (size_t)rows * a.ldo; a.os_part = (size_t)2 * max_tiles * out_tiles * MX4_TILE_BYTES;
+  if (2 * rows > 0x7fffffff || (long long)max_tiles * a.tiles_f > 0x3fffffff) SRB_FAIL("mx4_experts_pair: %d tiles are too many", max_tiles);
+  if (mode == MXP_F32 && (((uintptr_t)out & 15) || features % 4)) SRB_FAIL("mx4_experts_pair: rows of the result must start on 16-byte borders");
+  CUtensorMap maps[5];
+  if (make_bytes_map(&maps[0], x, 2 * rows, a.k_tiles * 128, MXP_ROWS) != SRB_OK ||
+      make_scales_map(&maps[1], x_scales, 4ll * max_tiles * a.k_tiles, 1) != SRB_OK)
+    return SRB_ERR_INVALID;
+  maps[2] = maps[3] = maps[4] = maps[0];
+  if (mode == MXP_F32 && make_map(&maps[4], CU_TENSOR_MAP_DATA_TYPE_FLOAT32, out, slots, features, features * 4ll, 32, 16, CU_TENSOR_MAP_SWIZZLE_64B) != SRB_OK)
+    return SRB_ERR_INVALID;
+  cudaStream_t s = (cudaStream_t)stream;
+  const int tiles = max_tiles * a.tiles_f;
+  if (mode == MXP_F32) return launch_pair<false, MXP_F32, true>(maps, a, tiles, s);
+  if (mode == MXP_GATED) return launch_pair<false, MXP_GATED, true>(maps, a, tiles, s);
+  return launch_pair<false, MXP_ACT, true>(maps, a, tiles, s);
+}

@@ -126,30 +126,19 @@ mx4_dequantize_kernel(const unsigned* __restrict__ codes, const unsigned* __rest
     if (k + i < width) dst[i] = srb_from_float<T>(v[i]);
 }
 
-// Rows of bfloat16 as the two eight-bit parts of mx4.cuh: parts [2, rows, 128 * column tiles] bytes, zero behind a row's last entry, and
-// their scales [2, row tiles, column tiles, 512] in the tiles of mx4.cuh (those of rows behind the last are not written: they are read,
-// but only for sums that nobody stores).
+// Eight entries of 128 of a row (lane of 16) as the two eight-bit parts of mx4.cuh, to `dst` and `dst + part`, and the row's scale words.
 template <bool WIDE>
-__global__ void __launch_bounds__(MX4_THREADS)
-mx4_split_kernel(const __nv_bfloat16* __restrict__ x, size_t pitch, int rows, int width, uint8_t* __restrict__ parts, uint8_t* __restrict__ scales) {
-  srb_launch_dependents();
-  srb_grid_dependency_wait();
-  const int k_tiles = mx4_tiles(width);
-  const int lane = threadIdx.x & 15;
-  const long long item = (long long)blockIdx.x * (MX4_THREADS / 16) + (threadIdx.x >> 4);
-  const int row = (int)(item / k_tiles), kt = (int)(item % k_tiles);
-  const bool live = row < rows;
-  const int k = kt * 128 + lane * 8;
+__device__ __forceinline__ void mx4_split_eight(const __nv_bfloat16* __restrict__ src, int left, bool live, int lane, uint8_t* dst, size_t part,
+                                                uint8_t* word, size_t scale_part) {
   float v[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) v[i] = 0.f;
   if (live) {
-    const __nv_bfloat16* src = x + (size_t)row * pitch + k;
-    if (WIDE && k + 8 <= width) mx4_unpack_bf16(*reinterpret_cast<const uint4*>(src), v);
+    if (WIDE && left >= 8) mx4_unpack_bf16(*reinterpret_cast<const uint4*>(src), v);
     else {
 #pragma unroll
       for (int i = 0; i < 8; ++i)
-        if (k + i < width) v[i] = srb_to_float(src[i]);
+        if (i < left) v[i] = srb_to_float(src[i]);
     }
   }
   unsigned most = 0u;
@@ -168,15 +157,51 @@ mx4_split_kernel(const __nv_bfloat16* __restrict__ x, size_t pitch, int rows, in
     low_word |= __shfl_xor_sync(0xffffffffu, low_word, offset);
   }
   if (!live) return;
-  const size_t part = (size_t)rows * k_tiles * 128, scale_part = (size_t)mx4_tiles(rows) * k_tiles * MX4_TILE_BYTES;
-  uint8_t* dst = parts + (size_t)row * k_tiles * 128 + k;
   *reinterpret_cast<uint2*>(dst) = make_uint2(h[0] | h[1] << 16, h[2] | h[3] << 16);
   *reinterpret_cast<uint2*>(dst + part) = make_uint2(l[0] | l[1] << 16, l[2] | l[3] << 16);
   if (lane == 0) {
-    uint8_t* word = scales + mx4_scale_word(row, kt, k_tiles);
     *reinterpret_cast<unsigned*>(word) = high_word;
     *reinterpret_cast<unsigned*>(word + scale_part) = low_word;
   }
+}
+
+// Rows of bfloat16 as parts [2, rows, 128 * column tiles] bytes, zero behind a row's last entry, and their scales [2, row tiles, column tiles, 512]
+// in the tiles of mx4.cuh (those of rows behind the last are not written: they are read, but only for sums that nobody stores).
+template <bool WIDE>
+__global__ void __launch_bounds__(MX4_THREADS)
+mx4_split_kernel(const __nv_bfloat16* __restrict__ x, size_t pitch, int rows, int width, uint8_t* __restrict__ parts, uint8_t* __restrict__ scales) {
+  srb_launch_dependents();
+  srb_grid_dependency_wait();
+  const int k_tiles = mx4_tiles(width), lane = threadIdx.x & 15;
+  const long long item = (long long)blockIdx.x * (MX4_THREADS / 16) + (threadIdx.x >> 4);
+  const int row = (int)(item / k_tiles), kt = (int)(item % k_tiles), k = kt * 128 + lane * 8;
+  mx4_split_eight<WIDE>(x + (size_t)row * pitch + k, width - k, row < rows, lane, parts + ((size_t)row * k_tiles * 128 + k),
+                        (size_t)rows * k_tiles * 128, scales + mx4_scale_word(row, kt, k_tiles),
+                        (size_t)mx4_tiles(rows) * k_tiles * MX4_TILE_BYTES);
+}
+
+// The same in the order of a plan's tiles (csrc/moe.cu) of 256 slots, with room for 256 rows a tile: parts [2, 256 tiles, ...].  16 lanes a
+// slot, 16 slots a block.
+template <bool WIDE>
+__global__ void __launch_bounds__(MX4_THREADS)
+mx4_split_slots_kernel(const __nv_bfloat16* __restrict__ x, int width, const int* __restrict__ plan, const int* __restrict__ slot_row, int experts,
+                       int max_tiles, uint8_t* __restrict__ parts, uint8_t* __restrict__ scales) {
+  srb_launch_dependents();
+  srb_grid_dependency_wait();
+  const int tile = blockIdx.y, in_tile = blockIdx.x * (MX4_THREADS / 16) + (threadIdx.x >> 4), lane = threadIdx.x & 15;
+  if (tile >= plan[0]) return;
+  const int expert = plan[1 + experts + 1 + 2 * tile], slot = plan[1 + experts + 1 + 2 * tile + 1] + in_tile;
+  const int end = plan[1 + expert + 1];
+  if (slot - (in_tile & 1) >= end) return;                   // neither half of the warp has a slot
+  const bool live = slot < end;
+  const int k_tiles = mx4_tiles(width), row = tile * 256 + in_tile;
+  const size_t part = (size_t)max_tiles * 256 * k_tiles * 128, scale_part = (size_t)max_tiles * 2 * k_tiles * MX4_TILE_BYTES;
+  const __nv_bfloat16* src = x + (size_t)(live ? slot_row[slot] : 0) * width + lane * 8;
+  uint8_t* dst = parts + ((size_t)row * k_tiles * 128 + lane * 8);
+#pragma unroll 4
+  for (int kt = 0; kt < k_tiles; ++kt)
+    mx4_split_eight<WIDE>(src + kt * 128, width - kt * 128 - lane * 8, live, lane, dst + kt * 128, part, scales + mx4_scale_word(row, kt, k_tiles),
+                          scale_part);
 }
 
 static int mx4_grid(int matrices, long long rows, int width, dim3* grid) {
@@ -234,5 +259,17 @@ extern "C" int srb_mx4_split(const void* x, long long pitch, int rows, int width
   SRB_CUDA_CALL(srb_launch(wide ? mx4_split_kernel<true> : mx4_split_kernel<false>, grid, dim3(MX4_THREADS), 0, (cudaStream_t)stream,
                            (const __nv_bfloat16*)x, (size_t)pitch, rows, width, (uint8_t*)parts, (uint8_t*)scales));
   SRB_LAUNCH_CHECK("mx4_split");
+  return SRB_OK;
+}
+
+extern "C" int srb_mx4_split_slots(const void* x, int width, const int* plan, const int* slot_row, int experts, int max_tiles, void* parts,
+                                   void* scales, void* stream) {
+  if (max_tiles <= 0 || width <= 0) return SRB_OK;
+  if (max_tiles > 65535) SRB_FAIL("mx4_split_slots: %d tiles are too many", max_tiles);
+  const bool wide = ((uintptr_t)x & 15) == 0 && width % 8 == 0;
+  SRB_CUDA_CALL(srb_launch(wide ? mx4_split_slots_kernel<true> : mx4_split_slots_kernel<false>, dim3(256 / (MX4_THREADS / 16), max_tiles),
+                           dim3(MX4_THREADS), 0, (cudaStream_t)stream, (const __nv_bfloat16*)x, width, plan, slot_row, experts, max_tiles,
+                           (uint8_t*)parts, (uint8_t*)scales));
+  SRB_LAUNCH_CHECK("mx4_split_slots");
   return SRB_OK;
 }

@@ -39,3 +39,45 @@ __device__ __forceinline__ void tmem_load_8(unsigned address, float (&v)[8]) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(r[i]);
 }
+
+// ---- pairs of CTAs (cta_group::2): M = 256, the even CTA's thread issues for both -----------------------------------------
+// kind mxf4: both operands in four bits, packed
+__device__ __forceinline__ unsigned mx_idesc_four(int m, int n) { return (1u << 7) | (1u << 10) | ((unsigned)(n >> 3) << 17) | (1u << 23) | ((unsigned)(m >> 4) << 24); }
+__device__ __forceinline__ void umma_mx4_pair(unsigned tmem_d, unsigned long long a_desc, unsigned long long b_desc, unsigned idesc, unsigned a_scales,
+                                              unsigned b_scales, unsigned accumulate) {
+  asm volatile(
+      "{\n.reg .pred p;\nsetp.ne.b32 p, %6, 0;\n"
+      "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n}\n"
+      ::"r"(tmem_d), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(a_scales), "r"(b_scales), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void umma_mx8_pair(unsigned tmem_d, unsigned long long a_desc, unsigned long long b_desc, unsigned idesc, unsigned a_scales,
+                                              unsigned b_scales, unsigned accumulate) {
+  asm volatile(
+      "{\n.reg .pred p;\nsetp.ne.b32 p, %6, 0;\n"
+      "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n}\n"
+      ::"r"(tmem_d), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(a_scales), "r"(b_scales), "r"(accumulate) : "memory");
+}
+// in both CTAs, each from its own shared memory
+__device__ __forceinline__ void tmem_copy_scales_pair(unsigned tmem, unsigned long long desc) {
+  asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
+}
+// A bounded wait on a barrier on which the other CTA's threads arrive too.
+__device__ __forceinline__ bool mbar_wait_warp_cluster(unsigned bar, unsigned parity, volatile int* abort_flag) {
+  const long long start = clock64();
+  bool done = false;
+  for (unsigned spins = 0; !done; ++spins) {
+    unsigned ok;
+    asm volatile(
+        "{\n.reg .pred p;\nmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}\n"
+        : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    done = ok != 0;
+    if (!done && (spins & 255u) == 255u) {
+      if (*abort_flag) break;
+      if (clock64() - start > SRB_SPIN_LIMIT) {
+        *abort_flag = 1;
+        break;
+      }
+    }
+  }
+  return __all_sync(0xffffffffu, done);
+}

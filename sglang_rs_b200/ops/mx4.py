@@ -18,6 +18,10 @@ from .trace import traced
 
 #: entries of a row that share a scale
 MX4_BLOCK = 32
+#: up to this many rows a product runs on the kernel that has the weights on the M side (csrc/gemm_mx4.cu), above it on pairs of CTAs
+MX4_FEW_ROWS = 64
+#: experts' products run on pairs of CTAs where a step has more choices per expert than this
+MX4_FEW_CHOICES = 16
 
 
 def _tiles(n: int) -> int:
@@ -175,14 +179,18 @@ def linear_mx4(x, weight: Mx4, error_word: torch.Tensor, *, bias: Optional[torch
         if bias.shape != (weight.rows,):
             raise KernelError("linear_mx4: one bias per feature is needed")
     _here("linear_mx4", x.codes if four else x, weight.codes, weight.scales, bias, error_word)
-    out = torch.empty((rows, weight.rows), dtype=out_dtype, device=weight.device)
+    many = rows > MX4_FEW_ROWS
+    # the kernel for many rows stores rows that start on 16-byte borders
+    pitch = -(-weight.rows // 8) * 8 if many else weight.rows
+    out = torch.empty((rows, pitch), dtype=out_dtype, device=weight.device)
     if out.numel():
-        lib = load_library("gemm_mx4")
+        lib = load_library("gemm_mx4_pair" if many else "gemm_mx4")
+        product = lib.srb_mx4_linear_pair if many else lib.srb_mx4_linear
         held, scales = (x.codes, x.scales) if four else _split(x)
-        _check(lib, lib.srb_mx4_linear(_ptr(held), _ptr(scales), int(four), _ptr(weight.codes), _ptr(weight.scales), _ptr(bias), _ptr(out),
-                                       ctypes.c_longlong(out.stride(0)), rows, weight.rows, width, int(out_dtype == torch.float32),
-                                       _ptr(error_word), _stream()))
-    return out
+        _check(lib, product(_ptr(held), _ptr(scales), int(four), _ptr(weight.codes), _ptr(weight.scales), _ptr(bias), _ptr(out),
+                            ctypes.c_longlong(out.stride(0)), rows, weight.rows, width, int(out_dtype == torch.float32),
+                            _ptr(error_word), _stream()))
+    return out if pitch == weight.rows else out[:, :weight.rows]
 
 
 @traced("routed_experts")
@@ -243,24 +251,39 @@ def chosen_experts_mx4(h: torch.Tensor, chosen: torch.Tensor, weights: torch.Ten
     if rows == 0 or top == 0:
         return torch.zeros((rows, width), dtype=torch.bfloat16, device=h.device)
     out = torch.empty((rows, width), dtype=torch.bfloat16, device=h.device)
-    device, entries, stream, tile = h.device, rows * top, _stream(), 64
+    device, entries, stream = h.device, rows * top, _stream()
+    # (the pairs' result rows start on 16-byte borders)
+    many = entries > MX4_FEW_CHOICES * experts and width % 4 == 0
+    tile = 256 if many else 64
     moe, lib = load_library("moe"), load_library("gemm_mx4")
     plan = torch.empty(moe.srb_moe_plan_ints_of(rows, top, experts, tile), dtype=torch.int32, device=device)
     slot_row = torch.empty(entries, dtype=torch.int32, device=device)
     entry_slot = torch.empty(entries, dtype=torch.int32, device=device)
-    act = torch.empty((2, entries, 128 * _tiles(inner)), dtype=torch.uint8, device=device)
-    act_scales = torch.empty((2, _tiles(entries), _tiles(inner), 512), dtype=torch.uint8, device=device)
     y = torch.empty((entries, width), dtype=torch.float32, device=device)
     _check(moe, moe.srb_moe_plan_of(_ptr(chosen), rows, top, experts, tile, _ptr(plan), _ptr(slot_row), _ptr(entry_slot), None, None,
                                     _ptr(error_word), stream))
     # a tile has a slot at least
     tiles = min(entries, moe.srb_moe_max_tiles_of(rows, top, experts, tile))
-    parts, scales = _split(h)
-    _check(lib, lib.srb_mx4_experts(_ptr(parts), _ptr(scales), rows, _ptr(slot_row), _ptr(w_gate_up.codes), _ptr(w_gate_up.scales), _ptr(act),
-                                    _ptr(act_scales), _ptr(plan), tiles, entries, experts, inner, width, GEMM_MODES["gated" if gated else "act"],
-                                    act_code, ctypes.c_float(activation_param), _ptr(error_word), stream))
-    _check(lib, lib.srb_mx4_experts(_ptr(act), _ptr(act_scales), entries, None, _ptr(w_down.codes), _ptr(w_down.scales), _ptr(y), None,
-                                    _ptr(plan), tiles, entries, experts, width, inner, GEMM_MODES["f32"], 0, ctypes.c_float(0.0),
-                                    _ptr(error_word), stream))
+    act_rows = 256 * tiles if many else entries
+    act = torch.empty((2, act_rows, 128 * _tiles(inner)), dtype=torch.uint8, device=device)
+    act_scales = torch.empty((2, _tiles(act_rows), _tiles(inner), 512), dtype=torch.uint8, device=device)
+    mode, param = GEMM_MODES["gated" if gated else "act"], ctypes.c_float(activation_param)
+    if many:
+        pair, split = load_library("gemm_mx4_pair"), load_library("mx4")
+        parts = torch.empty((2, act_rows, 128 * _tiles(width)), dtype=torch.uint8, device=device)
+        scales = torch.empty((2, 2 * tiles, _tiles(width), 512), dtype=torch.uint8, device=device)
+        _check(split, split.srb_mx4_split_slots(_ptr(h), width, _ptr(plan), _ptr(slot_row), experts, tiles, _ptr(parts), _ptr(scales), stream))
+        _check(pair, pair.srb_mx4_experts_pair(_ptr(parts), _ptr(scales), _ptr(w_gate_up.codes), _ptr(w_gate_up.scales), _ptr(act),
+                                               _ptr(act_scales), _ptr(plan), tiles, entries, experts, inner, width, mode, act_code, param,
+                                               _ptr(error_word), stream))
+        _check(pair, pair.srb_mx4_experts_pair(_ptr(act), _ptr(act_scales), _ptr(w_down.codes), _ptr(w_down.scales), _ptr(y), None, _ptr(plan),
+                                               tiles, entries, experts, width, inner, GEMM_MODES["f32"], 0, param, _ptr(error_word), stream))
+    else:
+        parts, scales = _split(h)
+        _check(lib, lib.srb_mx4_experts(_ptr(parts), _ptr(scales), rows, _ptr(slot_row), _ptr(w_gate_up.codes), _ptr(w_gate_up.scales), _ptr(act),
+                                        _ptr(act_scales), _ptr(plan), tiles, entries, experts, inner, width, mode, act_code, param,
+                                        _ptr(error_word), stream))
+        _check(lib, lib.srb_mx4_experts(_ptr(act), _ptr(act_scales), entries, None, _ptr(w_down.codes), _ptr(w_down.scales), _ptr(y), None,
+                                        _ptr(plan), tiles, entries, experts, width, inner, GEMM_MODES["f32"], 0, param, _ptr(error_word), stream))
     _check(lib, lib.srb_mx4_combine(_ptr(y), _ptr(entry_slot), _ptr(weights), rows, top, width, _ptr(out), stream))
     return out
