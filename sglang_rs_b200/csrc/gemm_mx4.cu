@@ -9,13 +9,12 @@
 // K is cut where the row tiles are fewer than two blocks an SM: the blocks of a cluster take a part each, leave their sums in shared memory
 // and add them in block order, so a result does not depend on timing.
 //
-// Warps 0-3 copy and then store, warp 4 issues the products.  Waits are bounded; one that runs out flags SRB_FLAG_WAIT_TIMEOUT.
+// Warps 0-3 copy (nothing waits for a copy but the products) and then store, warp 4 issues the products.  Waits are bounded; one that runs out flags SRB_FLAG_WAIT_TIMEOUT.
 //
 // Over experts (GROUPED) a block's rows are up to 64 slots of one expert (the plan of csrc/moe.cu).  The gated mode has 64 gate rows over the
 // 64 up rows of the same features, and leaves act(gate) * up as eight-bit parts again, rounded from 32 bits, for the next product.
 #include "common.cuh"
 #include "activations.cuh"
-#include "mma_helpers.cuh"
 #include "mx4.cuh"
 #include "mx4_umma.cuh"
 #include <algorithm>
@@ -142,36 +141,27 @@ mx4_few_kernel(const FewArgs a) {
     const int x_scale_row = x_scale_live ? x_row[x_token] : 0;
     const uint8_t* x_scales = a.x_scales + (second ? a.xs_part : 0);
     const size_t x_pitch = (size_t)a.k_tiles * (FOUR ? 64 : 128);
-    for (int i = 0; i < steps + STAGES - 1; ++i) {
-      if (i < steps) {
-        const int s = i % STAGES, kt = kt0 + i;
-        if (i >= STAGES) ok = ok && mbar_wait(smem_u32(&empty_bar[s]), (unsigned)(i / STAGES - 1) & 1u, &abort_flag);
-        if (ok) {
-          const unsigned w_to = smem_u32(smem) + s * stage_bytes, x_to = w_to + MXF_A_BYTES, scales_to = scales0 + s * 1024;
+    for (int i = 0; i < steps; ++i) {
+      const int s = i % STAGES, kt = kt0 + i;
+      if (i >= STAGES && !mbar_wait(smem_u32(&empty_bar[s]), (unsigned)(i / STAGES - 1) & 1u, &abort_flag)) break;
+      const unsigned w_to = smem_u32(smem) + s * stage_bytes, x_to = w_to + MXF_A_BYTES, scales_to = scales0 + s * 1024;
 #pragma unroll
-          for (int j = 0; j < 8; ++j)
-            cp_async_8(w_to + (sub + 16 * j) * 128 + place, w_at[j] + (size_t)kt * 64, (w_live >> j) & 1u ? 8 : 0);
-          cp_async_4(scales_to + lane * 16 + warp * 4, w_scales + mx4_scale_word(scale_row, kt, a.k_tiles), scale_live ? 4 : 0);
-          for (int n = sub; n < columns; n += 16) {
-            const bool low = !FOUR && n >= part_columns;
-            const int token = low ? n - part_columns : n;
-            const bool live = token < count;
-            const uint8_t* src = a.x + (low ? a.x_part : 0) + (size_t)x_row[live ? token : 0] * x_pitch;
-            if (FOUR) cp_async_8(x_to + n * 128 + place, src + kt * 64 + chunk * 8, live ? 8 : 0);
-            else cp_async_16_to(x_to + n * 128 + place, src + kt * 128 + chunk * 16, live ? 16 : 0);
-          }
-          if (t < columns)
-            cp_async_4(scales_to + 512 + lane * 16 + warp * 4, x_scales + mx4_scale_word(x_scale_row, kt, a.k_tiles), x_scale_live ? 4 : 0);
-        }
+      for (int j = 0; j < 8; ++j)
+        cp_async_8(w_to + (sub + 16 * j) * 128 + place, w_at[j] + (size_t)kt * 64, (w_live >> j) & 1u ? 8 : 0);
+      cp_async_4(scales_to + lane * 16 + warp * 4, w_scales + mx4_scale_word(scale_row, kt, a.k_tiles), scale_live ? 4 : 0);
+      for (int n = sub; n < columns; n += 16) {
+        const bool low = !FOUR && n >= part_columns;
+        const int token = low ? n - part_columns : n;
+        const bool live = token < count;
+        const uint8_t* src = a.x + (low ? a.x_part : 0) + (size_t)x_row[live ? token : 0] * x_pitch;
+        if (FOUR) cp_async_8(x_to + n * 128 + place, src + kt * 64 + chunk * 8, live ? 8 : 0);
+        else cp_async_16_to(x_to + n * 128 + place, src + kt * 128 + chunk * 16, live ? 16 : 0);
       }
-      cp_async_commit();
-      if (i >= STAGES - 1) {
-        cp_async_wait<STAGES - 1>();
-        fence_proxy_async_shared();
-        mbar_arrive(smem_u32(&full_bar[(i - (STAGES - 1)) % STAGES]));
-      }
+      if (t < columns)
+        cp_async_4(scales_to + 512 + lane * 16 + warp * 4, x_scales + mx4_scale_word(x_scale_row, kt, a.k_tiles), x_scale_live ? 4 : 0);
+      copies_arrive(smem_u32(&full_bar[s]));
     }
-    cp_async_wait<0>();
+    asm volatile("cp.async.wait_all;" ::: "memory");
   } else {
     // ---- products
     const unsigned idesc = mx_idesc(MX_E2M1, FOUR ? MX_E2M1 : MX_E4M3, 128, columns);
@@ -179,6 +169,7 @@ mx4_few_kernel(const FewArgs a) {
       const int s = i % STAGES;
       ok = mbar_wait_warp(smem_u32(&full_bar[s]), (unsigned)(i / STAGES) & 1u, &abort_flag);
       if (!ok) break;
+      fence_proxy_async_shared();
       tc_fence_after();
       const unsigned w_at = smem_u32(smem) + s * stage_bytes;
       const unsigned long long a_desc = smem_descriptor(w_at), b_desc = smem_descriptor(w_at + MXF_A_BYTES);

@@ -33,7 +33,6 @@ SRB_DEFINE_PDL_SWITCH()
 #define MXP_BOX_BYTES 2048       // a warp's piece of the output: 32 rows x 64 bytes, swizzled
 #define MXP_A_BYTES (MXP_ROWS * 128)
 #define MXP_B_BYTES (MXP_HALF * 128)
-#define MXP_COPIES_AHEAD 2       // steps of W that the copy warps have issued beyond the one that they hand over
 #define MXP_SUMS 384             // columns of tensor memory: scales lie behind
 #define MXP_BF16 0
 #define MXP_F32 1
@@ -153,7 +152,7 @@ mx4_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
   constexpr bool GATED = MODE == MXP_GATED, PARTS = MODE == MXP_GATED || MODE == MXP_ACT;
   extern __shared__ unsigned char smem_unaligned[];
   unsigned char* smem = reinterpret_cast<unsigned char*>(((uintptr_t)smem_unaligned + 1023) & ~(uintptr_t)1023);
-  __shared__ __align__(8) unsigned long long full_bar[STAGES], empty_bar[STAGES], acc_full[2], acc_empty[2];
+  __shared__ __align__(8) unsigned long long full_bar[STAGES], empty_bar[STAGES], copied_bar[STAGES], acc_full[2], acc_empty[2];
   __shared__ unsigned tmem_holder;
   __shared__ int abort_flag;
 
@@ -165,7 +164,8 @@ mx4_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
   if (threadIdx.x == 0) {
     abort_flag = 0;
     for (int s = 0; s < STAGES; ++s) {
-      mbar_init(smem_u32(&full_bar[s]), 1 + 2 * Shape::COPY_WARPS);
+      mbar_init(smem_u32(&full_bar[s]), FOUR ? 1 : 2);       // the even CTA's: its bytes by TMA, and the word that the odd CTA's copies are there
+      mbar_init(smem_u32(&copied_bar[s]), 128);
       mbar_init(smem_u32(&empty_bar[s]), 1);
     }
     for (int b = 0; b < 2; ++b) {
@@ -237,7 +237,9 @@ mx4_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
         for (int i = 0; i < steps && ok; ++i, ++round) {
           const int s = (int)(round % STAGES);
           ok = mbar_wait_warp_cluster(smem_u32(&full_bar[s]), (round / STAGES) & 1u, &abort_flag);
+          if (!FOUR && ok) ok = mbar_wait_warp(smem_u32(&copied_bar[s]), (round / STAGES) & 1u, &abort_flag);
           if (!ok) break;
+          if (!FOUR) fence_proxy_async_shared();
           tc_fence_after();
           const unsigned stage = smem_u32(smem) + s * Shape::STAGE_BYTES;
           const unsigned place = tmem + MXP_SUMS + (round % Shape::PLACES) * Shape::PLACE_COLUMNS;
@@ -272,20 +274,27 @@ mx4_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
           __syncwarp();
         }
       }
+    } else if (!FOUR) {
+      // ---- the odd CTA's copies: said to the even one when they are there
+      unsigned round = 0;
+      bool ok = true;
+      for (int tile = pair; tile < num_tiles && ok; tile += num_pairs)
+        for (int i = 0; i < steps && ok; ++i, ++round) {
+          const int s = (int)(round % STAGES);
+          ok = mbar_wait_warp(smem_u32(&copied_bar[s]), (round / STAGES) & 1u, &abort_flag);
+          if (!ok) break;
+          fence_proxy_async_shared();
+          if (lane == 0) arrive_at(smem_u32(&full_bar[s]), 0);
+          __syncwarp();
+        }
     }
   } else if (warp < 2 + Shape::COPY_WARPS) {
     // ---- codes of W, eight bytes to each 16, and the scales of all 192 rows: chunk t % 8 of rows t / 8 + 16 i, scales of row t (and 128 + t)
     const int t = threadIdx.x - 64, chunk = t & 7, sub = t >> 3;
     const unsigned to = (unsigned)(chunk ^ (sub & 7)) << 4;
     const size_t w_pitch = (size_t)a.k_tiles * 64;
-    unsigned round = 0, landed = 0;
+    unsigned round = 0;
     bool ok = true;
-    auto land = [&]() {
-      fence_proxy_async_shared();
-      __syncwarp();
-      if (lane == 0) arrive_at(smem_u32(&full_bar[landed % STAGES]), 0);
-      ++landed;
-    };
     for (int tile = pair; tile < num_tiles && ok; tile += num_pairs) {
       const PairMx4Tile tl = pair_mx4_tile<MODE, GROUPED>(a, tile);
       const uint8_t* w = a.w + (size_t)tl.matrix * a.w_rows * w_pitch;
@@ -318,16 +327,10 @@ mx4_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
         const unsigned word = stage + Shape::WS_AT + lane * 16 + ((t >> 5) << 2);
         cp_async_4(word, w_scales + first_word + (size_t)i * MX4_TILE_BYTES, first_live ? 4 : 0);
         if (t < 64) cp_async_4(word + 512, w_scales + second_word + (size_t)i * MX4_TILE_BYTES, second_live ? 4 : 0);
-        asm volatile("cp.async.commit_group;\n" ::: "memory");
-        if (round >= MXP_COPIES_AHEAD) {
-          asm volatile("cp.async.wait_group %0;\n" ::"n"(MXP_COPIES_AHEAD) : "memory");
-          land();
-        }
+        copies_arrive(smem_u32(&copied_bar[s]));
       }
     }
-    asm volatile("cp.async.wait_group 0;\n" ::: "memory");
-    if (ok)
-      while (landed < round) land();
+    asm volatile("cp.async.wait_all;" ::: "memory");
   } else {
     // ---- epilogue: warp w has lanes 32 * (w % 4) .. + 31 of its CTA's tensor memory, a row of X a lane, and a third of the columns
     const int quarter = warp & 3, third = (warp - 2 - Shape::COPY_WARPS) >> 2;
