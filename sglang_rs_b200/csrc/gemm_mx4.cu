@@ -3,8 +3,9 @@
 // The weight is the M side: a block owns 128 rows of W and up to 64 rows of X, the N side.  The tensor cores take the four-bit entries as
 // they are, so nothing is unpacked: turning 13 T entries a second (what the memory brings) into bfloat16 would take every instruction the SMs
 // issue.  Rows of X come as four-bit codes or as two eight-bit parts of a bfloat16 (mx4.cuh), which are columns of their own and meet in the
-// epilogue.  A product step of 128 entries: the codes, eight bytes to each 16 of a row in shared memory (cp.async puts them where the
-// instruction wants them), the rows of X, and both sides' scales, one word for each row.
+// epilogue.  A product step of 128 entries: the codes by TMA, which sets eight bytes to each 16 of a row in shared memory as the instruction
+// wants them (by cp.async of eight bytes, 50 MB of codes took 24 us instead of LATER), and by cp.async the rows of X and both sides' scales, one
+// word for each row.
 //
 // K is cut where the row tiles are fewer than two blocks an SM: the blocks of a cluster take a part each, leave their sums in shared memory
 // and add them in block order, so a result does not depend on timing.
@@ -35,7 +36,6 @@ struct FewArgs {
   const uint8_t* x;              // codes, or the first of two parts
   const uint8_t* x_scales;
   size_t x_part, xs_part;        // bytes from the first part to the second
-  const uint8_t* w;
   const uint8_t* w_scales;
   const float* bias;
   void* out;
@@ -53,7 +53,7 @@ struct FewArgs {
 };
 
 __device__ __forceinline__ void cp_async_8(unsigned dst, const void* src, int bytes) {
-  asm volatile("cp.async.ca.shared.global.L2::128B [%0], [%1], 8, %2;\n" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;\n" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
 __device__ __forceinline__ void cp_async_4(unsigned dst, const void* src, int bytes) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;\n" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
@@ -65,7 +65,7 @@ __device__ __forceinline__ void few_copy_threads_sync() { asm volatile("bar.sync
 
 template <bool FOUR, int MODE, bool GROUPED, int STAGES>
 __global__ void __launch_bounds__(MXF_THREADS)
-mx4_few_kernel(const FewArgs a) {
+mx4_few_kernel(const __grid_constant__ CUtensorMap map_w, const FewArgs a) {
   constexpr bool GATED = MODE == MXF_GATED, PARTS = MODE == MXF_GATED || MODE == MXF_ACT;
   constexpr int FEATURES = GATED ? 64 : 128;
   extern __shared__ unsigned char smem_unaligned[];
@@ -97,7 +97,7 @@ mx4_few_kernel(const FewArgs a) {
   if (t == 0) {
     abort_flag = 0;
     for (int s = 0; s < STAGES; ++s) {
-      mbar_init(smem_u32(&full_bar[s]), MXF_COPY_THREADS);
+      mbar_init(smem_u32(&full_bar[s]), MXF_COPY_THREADS + 1);      // and the word that W's bytes are awaited
       mbar_init(smem_u32(&empty_bar[s]), 1);
     }
     mbar_init(smem_u32(&done_bar), 1);
@@ -113,9 +113,7 @@ mx4_few_kernel(const FewArgs a) {
   bool ok = true;
 
   if (warp < 4) {
-    // ---- copies: a thread has chunk t % 8 of rows t / 8 + 16 i, and the scales of row t
-    const size_t w_pitch = (size_t)a.k_tiles * 64;
-    const uint8_t* w = a.w + (size_t)matrix * a.w_rows * w_pitch;
+    // ---- copies: a thread has chunk t % 8 of columns t / 8 + 16 i of X, and the scales of row t of W and of column t
     const uint8_t* w_scales = a.w_scales + (size_t)matrix * mx4_tiles(a.w_rows) * a.k_tiles * MX4_TILE_BYTES;
     const int chunk = t & 7, sub = t >> 3;
     const unsigned place = (unsigned)(chunk ^ (sub & 7)) << 4;
@@ -124,14 +122,6 @@ mx4_few_kernel(const FewArgs a) {
       live = feature < a.features;
       return !live ? 0 : GATED && r >= 64 ? a.features + feature : feature;
     };
-    const uint8_t* w_at[8];
-    unsigned w_live = 0u;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      bool live;
-      w_at[i] = w + (size_t)w_row(sub + 16 * i, live) * w_pitch + chunk * 8;
-      w_live |= (unsigned)live << i;
-    }
     bool scale_live;
     const int scale_row = w_row(t, scale_live);
     // the column of X whose scales this thread brings
@@ -145,9 +135,16 @@ mx4_few_kernel(const FewArgs a) {
       const int s = i % STAGES, kt = kt0 + i;
       if (i >= STAGES && !mbar_wait(smem_u32(&empty_bar[s]), (unsigned)(i / STAGES - 1) & 1u, &abort_flag)) break;
       const unsigned w_to = smem_u32(smem) + s * stage_bytes, x_to = w_to + MXF_A_BYTES, scales_to = scales0 + s * 1024;
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        cp_async_8(w_to + (sub + 16 * j) * 128 + place, w_at[j] + (size_t)kt * 64, (w_live >> j) & 1u ? 8 : 0);
+      if (warp == 0) {
+        __syncwarp();
+        if (elect_one()) {
+          const unsigned bar = smem_u32(&full_bar[s]);
+          mbar_expect_tx(bar, MXF_A_BYTES / 2);
+          tma_load_2d(w_to, &map_w, bar, kt * 128, matrix * a.w_rows + feature0);
+          if (GATED) tma_load_2d(w_to + MXF_A_BYTES / 2, &map_w, bar, kt * 128, matrix * a.w_rows + a.features + feature0);
+        }
+        __syncwarp();
+      }
       cp_async_4(scales_to + lane * 16 + warp * 4, w_scales + mx4_scale_word(scale_row, kt, a.k_tiles), scale_live ? 4 : 0);
       for (int n = sub; n < columns; n += 16) {
         const bool low = !FOUR && n >= part_columns;
@@ -162,6 +159,11 @@ mx4_few_kernel(const FewArgs a) {
       copies_arrive(smem_u32(&full_bar[s]));
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
+    if (abort_flag) {
+      // copies by TMA in flight when a wait ran out write into this block's memory: give them time to land
+      const long long start = clock64();
+      while (clock64() - start < 4000000ll) {}
+    }
   } else {
     // ---- products
     const unsigned idesc = mx_idesc(MX_E2M1, FOUR ? MX_E2M1 : MX_E4M3, 128, columns);
@@ -290,24 +292,29 @@ mx4_few_kernel(const FewArgs a) {
 }
 
 template <bool FOUR, int MODE, bool GROUPED, int STAGES>
-static int launch_few_staged(const FewArgs& a, int tiles_f, int tiles_t, cudaStream_t s) {
+static int launch_few_staged(const CUtensorMap& map_w, const FewArgs& a, int tiles_f, int tiles_t, cudaStream_t s) {
   const size_t smem = 1024 + (size_t)STAGES * (MXF_A_BYTES + a.columns * 128 + 1024);
   auto kernel = mx4_few_kernel<FOUR, MODE, GROUPED, STAGES>;
   SRB_CUDA_CALL(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-  SRB_CUDA_CALL(srb_launch_clustered(kernel, dim3(tiles_f * a.splits, tiles_t), dim3(MXF_THREADS), smem, s, dim3(a.splits), a));
+  SRB_CUDA_CALL(srb_launch_clustered(kernel, dim3(tiles_f * a.splits, tiles_t), dim3(MXF_THREADS), smem, s, dim3(a.splits), map_w, a));
   SRB_LAUNCH_CHECK("mx4_few");
   return SRB_OK;
 }
 
 // Two blocks an SM: stages for as much shared memory as that leaves.
 template <bool FOUR, int MODE, bool GROUPED>
-static int launch_few(FewArgs& a, int tokens, int tiles_f, int tiles_t, cudaStream_t s) {
+static int launch_few(const void* w, FewArgs& a, int tokens, int tiles_f, int tiles_t, cudaStream_t s) {
+  CUtensorMap map_w;
+  const long long w_rows = (long long)std::max(a.experts, 1) * a.w_rows;
+  if ((uintptr_t)w & 31) SRB_FAIL("mx4_few: codes must start on a 32-byte border");
+  if (w_rows > 0x7fffffff) SRB_FAIL("mx4_few: %lld rows of weights are too many", w_rows);
+  if (make_codes_map(&map_w, w, w_rows, a.k_tiles, MODE == MXF_GATED ? 64 : 128) != SRB_OK) return SRB_ERR_INVALID;
   tokens = std::min(tokens, MXF_TOKENS);
   a.columns = FOUR ? (tokens + 15) & ~15 : 2 * ((tokens + 7) & ~7);
   if (tiles_t > 65535) SRB_FAIL("mx4_few: %d tiles of rows are too many", tiles_t);
-  return a.columns <= 32 ? launch_few_staged<FOUR, MODE, GROUPED, 5>(a, tiles_f, tiles_t, s)
-         : a.columns <= 64 ? launch_few_staged<FOUR, MODE, GROUPED, 4>(a, tiles_f, tiles_t, s)
-                           : launch_few_staged<FOUR, MODE, GROUPED, 3>(a, tiles_f, tiles_t, s);
+  return a.columns <= 32 ? launch_few_staged<FOUR, MODE, GROUPED, 5>(map_w, a, tiles_f, tiles_t, s)
+         : a.columns <= 64 ? launch_few_staged<FOUR, MODE, GROUPED, 4>(map_w, a, tiles_f, tiles_t, s)
+                           : launch_few_staged<FOUR, MODE, GROUPED, 3>(map_w, a, tiles_f, tiles_t, s);
 }
 
 // K in parts until there are about two blocks an SM, at least two steps each.
@@ -323,15 +330,15 @@ extern "C" int srb_mx4_linear(const void* x, const void* x_scales, int four, con
   if (rows <= 0 || features <= 0) return SRB_OK;
   if (width <= 0) SRB_FAIL("mx4_linear: inner size %d must be positive", width);
   FewArgs a = {};
-  a.x = (const uint8_t*)x; a.x_scales = (const uint8_t*)x_scales; a.w = (const uint8_t*)w; a.w_scales = (const uint8_t*)w_scales; a.bias = bias;
+  a.x = (const uint8_t*)x; a.x_scales = (const uint8_t*)x_scales; a.w_scales = (const uint8_t*)w_scales; a.bias = bias;
   a.out = out; a.ldo = ldo; a.rows = rows; a.features = a.w_rows = features; a.k_tiles = mx4_tiles(width); a.error_word = error_word;
   a.x_part = (size_t)rows * a.k_tiles * 128; a.xs_part = (size_t)mx4_tiles(rows) * a.k_tiles * MX4_TILE_BYTES;
   const int tiles_f = mx4_tiles(features), tiles_t = (rows + MXF_TOKENS - 1) / MXF_TOKENS;
   a.splits = few_splits((long long)tiles_f * tiles_t, a.k_tiles);
   cudaStream_t s = (cudaStream_t)stream;
   if (four)
-    return out_float ? launch_few<true, MXF_F32, false>(a, rows, tiles_f, tiles_t, s) : launch_few<true, MXF_BF16, false>(a, rows, tiles_f, tiles_t, s);
-  return out_float ? launch_few<false, MXF_F32, false>(a, rows, tiles_f, tiles_t, s) : launch_few<false, MXF_BF16, false>(a, rows, tiles_f, tiles_t, s);
+    return out_float ? launch_few<true, MXF_F32, false>(w, a, rows, tiles_f, tiles_t, s) : launch_few<true, MXF_BF16, false>(w, a, rows, tiles_f, tiles_t, s);
+  return out_float ? launch_few<false, MXF_F32, false>(w, a, rows, tiles_f, tiles_t, s) : launch_few<false, MXF_BF16, false>(w, a, rows, tiles_f, tiles_t, s);
 }
 
 // The experts' products over the plan's tiles (of 64 slots).  x: parts [2, x_rows, 128 k_tiles] and their scales; rows by `slot_row`, or the
@@ -344,7 +351,7 @@ extern "C" int srb_mx4_experts(const void* x, const void* x_scales, int x_rows, 
   if (activation < 0 || activation >= SRB_ACT_COUNT) SRB_FAIL("mx4_experts: unknown activation %d", activation);
   if (mode != MXF_F32 && mode != MXF_GATED && mode != MXF_ACT) SRB_FAIL("mx4_experts: mode %d is not float, gated or activated", mode);
   FewArgs a = {};
-  a.x = (const uint8_t*)x; a.x_scales = (const uint8_t*)x_scales; a.w = (const uint8_t*)w; a.w_scales = (const uint8_t*)w_scales; a.out = out;
+  a.x = (const uint8_t*)x; a.x_scales = (const uint8_t*)x_scales; a.w_scales = (const uint8_t*)w_scales; a.out = out;
   a.out_scales = (uint8_t*)out_scales; a.rows = slots; a.features = features; a.w_rows = mode == MXF_GATED ? 2 * features : features;
   a.k_tiles = mx4_tiles(width); a.activation = activation; a.act_param = act_param; a.error_word = error_word;
   a.x_part = (size_t)x_rows * a.k_tiles * 128; a.xs_part = (size_t)mx4_tiles(x_rows) * a.k_tiles * MX4_TILE_BYTES;
@@ -353,12 +360,12 @@ extern "C" int srb_mx4_experts(const void* x, const void* x_scales, int x_rows, 
   const int out_tiles = mx4_tiles(features);
   if (mode == MXF_F32) {
     a.ldo = features;
-    return launch_few<false, MXF_F32, true>(a, slots, out_tiles, max_tiles, s);
+    return launch_few<false, MXF_F32, true>(w, a, slots, out_tiles, max_tiles, s);
   }
   a.ldo = (size_t)out_tiles * 128;
   a.out_part = (size_t)slots * a.ldo; a.os_part = (size_t)mx4_tiles(slots) * out_tiles * MX4_TILE_BYTES;
-  if (mode == MXF_GATED) return launch_few<false, MXF_GATED, true>(a, slots, 2 * out_tiles, max_tiles, s);
-  return launch_few<false, MXF_ACT, true>(a, slots, out_tiles, max_tiles, s);
+  if (mode == MXF_GATED) return launch_few<false, MXF_GATED, true>(w, a, slots, 2 * out_tiles, max_tiles, s);
+  return launch_few<false, MXF_ACT, true>(w, a, slots, out_tiles, max_tiles, s);
 }
 
 // out[row, :] = sum over the row's choices, in their order, of weight * y[slot, :], in 32 bits, rounded once.

@@ -4,23 +4,23 @@
 // Two kinds of rows.  FOUR: X in four bits too; both operands and their scales come by TMA as they lie, a step is 256 entries, four
 // products of kind mxf4 (64 entries each, four times bfloat16's rate).  Otherwise X is the two eight-bit parts of a bfloat16 (mx4.cuh): a
 // step is 128 entries, four products of kind mxf8f6f4 for each part into the same sums (each at twice bfloat16's rate); they want the codes of W
-// eight bytes to each 16, so four warps bring those, and the scales of W, by cp.async.  Nothing is unpacked in either.
+// eight bytes to each 16, as TMA sets them.  Nothing is unpacked in either.
 //
 // CTA r of a pair has 128 rows of X (the M side) and 96 rows of W (half of the N side) in shared memory, and in tensor memory two
 // buffers of 192 columns of sums for its rows of X, a row a lane, beside 128 columns of scales (256 columns of sums twice would leave none).  Scales
 // go from shared to tensor memory ahead of a step's products, in the same queue; steps use places in turn.
 //
 // Over experts (GROUPED) a tile is up to 256 slots of one expert (the plan of csrc/moe.cu); X and the parts that the gated mode leaves have room
-// for 256 rows a tile, so that a tile's scales are whole tiles.  Gated: the even CTA brings gate rows, the odd one the up rows of the same 96 features.
+// for 256 rows a tile, so that a tile's scales are whole tiles.  Gated: the even CTA brings gate rows, the odd one the up rows of the same 96 features;
+// their scales are no whole tiles, and four warps bring them by cp.async, a word a row.
 //
-// Warps: 0 TMA, 1 products (even CTA) and tensor memory, then four for W where X is parts, then twelve of the epilogue: a quarter of the lanes
+// Warps: 0 TMA, 1 products (even CTA) and tensor memory, then four for W's scales in the gated mode, then twelve of the epilogue: a quarter of the lanes
 // and a third of the columns each.  Waits are bounded; one that runs out flags SRB_FLAG_WAIT_TIMEOUT.
 #include "common.cuh"
 #include "activations.cuh"
 #include "mx4.cuh"
 #include "mx4_umma.cuh"
 #include <algorithm>
-#include <mutex>
 
 SRB_DEFINE_LAST_ERROR()
 SRB_DEFINE_PDL_SWITCH()
@@ -39,22 +39,21 @@ SRB_DEFINE_PDL_SWITCH()
 #define MXP_GATED 2
 #define MXP_ACT 5
 
-template <bool FOUR> struct PairShape {
+template <bool FOUR, bool GATED> struct PairShape {
   static constexpr int STAGES = FOUR ? 6 : 4;
   static constexpr int PARTS = FOUR ? 1 : 2;
   static constexpr int B_AT = PARTS * MXP_A_BYTES;
   static constexpr int XS_AT = B_AT + MXP_B_BYTES;           // scales of X: two column tiles, or a tile of each part
   static constexpr int WS_AT = XS_AT + 1024;                 // of W: two row tiles of each column tile, or 192 rows in order
   static constexpr int STAGE_BYTES = WS_AT + (FOUR ? 2048 : 1024);
-  static constexpr int TMA_BYTES = FOUR ? STAGE_BYTES : 2 * MXP_A_BYTES + 1024;    // a CTA's by TMA
-  static constexpr int COPY_WARPS = FOUR ? 0 : 4;
+  static constexpr int TMA_BYTES = FOUR ? STAGE_BYTES : 2 * MXP_A_BYTES + MXP_B_BYTES / 2 + (GATED ? 1024 : 2048);    // a CTA's by TMA
+  static constexpr int COPY_WARPS = GATED ? 4 : 0;
   static constexpr int THREADS = 32 * (2 + COPY_WARPS + MXP_EPILOGUE_WARPS);
   static constexpr int PLACE_COLUMNS = FOUR ? 24 : 16;       // of scales of a step
   static constexpr int PLACES = FOUR ? 5 : 4;
 };
 
 struct PairMx4Args {
-  const uint8_t* w;
   const uint8_t* w_scales;
   const float* bias;
   void* out;
@@ -71,9 +70,6 @@ struct PairMx4Args {
   int experts;
 };
 
-__device__ __forceinline__ void cp_async_8(unsigned dst, const void* src, int bytes) {
-  asm volatile("cp.async.ca.shared.global.L2::128B [%0], [%1], 8, %2;\n" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
 __device__ __forceinline__ void cp_async_4(unsigned dst, const void* src, int bytes) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;\n" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
@@ -144,10 +140,10 @@ __device__ __forceinline__ PairMx4Tile pair_mx4_tile(const PairMx4Args& a, int t
 }
 
 template <bool FOUR, int MODE, bool GROUPED>
-__global__ void __launch_bounds__(PairShape<FOUR>::THREADS, 1)
+__global__ void __launch_bounds__(PairShape<FOUR, MODE == MXP_GATED>::THREADS, 1)
 mx4_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_xs, const __grid_constant__ CUtensorMap map_w,
                 const __grid_constant__ CUtensorMap map_ws, const __grid_constant__ CUtensorMap map_out, const PairMx4Args a) {
-  using Shape = PairShape<FOUR>;
+  using Shape = PairShape<FOUR, MODE == MXP_GATED>;
   constexpr int STAGES = Shape::STAGES;
   constexpr bool GATED = MODE == MXP_GATED, PARTS = MODE == MXP_GATED || MODE == MXP_ACT;
   extern __shared__ unsigned char smem_unaligned[];
@@ -164,7 +160,7 @@ mx4_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
   if (threadIdx.x == 0) {
     abort_flag = 0;
     for (int s = 0; s < STAGES; ++s) {
-      mbar_init(smem_u32(&full_bar[s]), FOUR ? 1 : 2);       // the even CTA's: its bytes by TMA, and the word that the odd CTA's copies are there
+      mbar_init(smem_u32(&full_bar[s]), GATED ? 2 : 1);      // the even CTA's: its bytes by TMA, and the word that the odd CTA's copies are there
       mbar_init(smem_u32(&copied_bar[s]), 128);
       mbar_init(smem_u32(&empty_bar[s]), 1);
     }
@@ -191,7 +187,8 @@ mx4_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
     for (int tile = pair; tile < num_tiles && ok; tile += num_pairs) {
       const PairMx4Tile t = pair_mx4_tile<MODE, GROUPED>(a, tile);
       const int x_row = t.x_row0 + (int)rank * MXP_ROWS, xs_tile = (x_row >> 7) * a.k_tiles;
-      const int w_row = t.feature0 + (int)rank * MXP_HALF, ws_tile = (t.feature0 >> 7) * a.k_tiles;
+      const int w_row = t.matrix * a.w_rows + t.feature0 + (int)rank * (GATED ? a.features : MXP_HALF);
+      const int ws_tile = (t.matrix * mx4_tiles(a.w_rows) + (t.feature0 >> 7)) * a.k_tiles;
       for (int i = 0; i < steps && ok; ++i, ++round) {
         const int s = (int)(round % STAGES);
         ok = mbar_wait_warp(smem_u32(&empty_bar[s]), ((round / STAGES) & 1u) ^ 1u, &abort_flag);
@@ -208,7 +205,12 @@ mx4_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
           } else {
             pair_tma_load(stage + MXP_A_BYTES, &map_x, bar, i * 128, a.x_lo_row + x_row);
             pair_tma_load(stage + Shape::XS_AT, &map_xs, bar, 0, xs_tile + i);
+            pair_tma_load(stage + Shape::B_AT, &map_w, bar, i * 128, w_row);
             pair_tma_load(stage + Shape::XS_AT + 512, &map_xs, bar, 0, a.xs_lo_tile + xs_tile + i);
+            if (!GATED) {
+              pair_tma_load(stage + Shape::WS_AT, &map_ws, bar, 0, ws_tile + i);
+              pair_tma_load(stage + Shape::WS_AT + 512, &map_ws, bar, 0, ws_tile + a.k_tiles + i);
+            }
           }
         }
         ++issued;
@@ -233,13 +235,13 @@ mx4_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
         tc_fence_after();
         const unsigned acc = tmem + b * MXP_N;
         // a tile of W that starts in the middle of a tile of scales
-        const unsigned shift = FOUR ? (unsigned)(pair_mx4_tile<MODE, GROUPED>(a, tile).feature0 & 127) >> 5 : 0u;
+        const unsigned shift = !GATED ? (unsigned)(pair_mx4_tile<MODE, GROUPED>(a, tile).feature0 & 127) >> 5 : 0u;
         for (int i = 0; i < steps && ok; ++i, ++round) {
           const int s = (int)(round % STAGES);
           ok = mbar_wait_warp_cluster(smem_u32(&full_bar[s]), (round / STAGES) & 1u, &abort_flag);
-          if (!FOUR && ok) ok = mbar_wait_warp(smem_u32(&copied_bar[s]), (round / STAGES) & 1u, &abort_flag);
+          if (GATED && ok) ok = mbar_wait_warp(smem_u32(&copied_bar[s]), (round / STAGES) & 1u, &abort_flag);
           if (!ok) break;
-          if (!FOUR) fence_proxy_async_shared();
+          if (GATED) fence_proxy_async_shared();
           tc_fence_after();
           const unsigned stage = smem_u32(smem) + s * Shape::STAGE_BYTES;
           const unsigned place = tmem + MXP_SUMS + (round % Shape::PLACES) * Shape::PLACE_COLUMNS;
@@ -266,7 +268,7 @@ mx4_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
 #pragma unroll
               for (unsigned k = 0; k < 8; ++k)
                 umma_mx8_pair(acc, a_desc + (k >> 2) * (MXP_A_BYTES >> 4) + 2 * (k & 3), b_desc + 2 * (k & 3), mx_idesc_step(idesc, k & 3),
-                              place + 4 * (k >> 2), place + 8, (i > 0 || k > 0) ? 1u : 0u);
+                              place + 4 * (k >> 2), place + 8 + shift, (i > 0 || k > 0) ? 1u : 0u);
             }
             pair_commit(smem_u32(&empty_bar[s]));
             if (i == steps - 1) pair_commit(smem_u32(&acc_full[b]));
@@ -274,7 +276,7 @@ mx4_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
           __syncwarp();
         }
       }
-    } else if (!FOUR) {
+    } else if (GATED) {
       // ---- the odd CTA's copies: said to the even one when they are there
       unsigned round = 0;
       bool ok = true;
@@ -289,30 +291,19 @@ mx4_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
         }
     }
   } else if (warp < 2 + Shape::COPY_WARPS) {
-    // ---- codes of W, eight bytes to each 16, and the scales of all 192 rows: chunk t % 8 of rows t / 8 + 16 i, scales of row t (and 128 + t)
-    const int t = threadIdx.x - 64, chunk = t & 7, sub = t >> 3;
-    const unsigned to = (unsigned)(chunk ^ (sub & 7)) << 4;
-    const size_t w_pitch = (size_t)a.k_tiles * 64;
+    // ---- the scales of all 192 rows of W, gate and up: of row t, and 128 + t
+    const int t = threadIdx.x - 64;
     unsigned round = 0;
     bool ok = true;
     for (int tile = pair; tile < num_tiles && ok; tile += num_pairs) {
       const PairMx4Tile tl = pair_mx4_tile<MODE, GROUPED>(a, tile);
-      const uint8_t* w = a.w + (size_t)tl.matrix * a.w_rows * w_pitch;
       const uint8_t* w_scales = a.w_scales + (size_t)tl.matrix * mx4_tiles(a.w_rows) * a.k_tiles * MX4_TILE_BYTES;
       // row n of the N side
       auto w_row = [&](int n, bool& live) {
-        const int feature = tl.feature0 + (GATED && n >= MXP_HALF ? n - MXP_HALF : n);
+        const int feature = tl.feature0 + (n >= MXP_HALF ? n - MXP_HALF : n);
         live = feature < a.features;
-        return !live ? 0 : GATED && n >= MXP_HALF ? a.features + feature : feature;
+        return !live ? 0 : n >= MXP_HALF ? a.features + feature : feature;
       };
-      const uint8_t* w_at[6];
-      unsigned live = 0u;
-#pragma unroll
-      for (int i = 0; i < 6; ++i) {
-        bool here;
-        w_at[i] = w + (size_t)w_row((int)rank * MXP_HALF + sub + 16 * i, here) * w_pitch + chunk * 8;
-        live |= (unsigned)here << i;
-      }
       bool first_live, second_live;
       const size_t first_word = mx4_scale_word(w_row(t, first_live), 0, a.k_tiles);
       const size_t second_word = mx4_scale_word(w_row(128 + (t & 63), second_live), 0, a.k_tiles);
@@ -321,9 +312,6 @@ mx4_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
         ok = mbar_wait_warp(smem_u32(&empty_bar[s]), ((round / STAGES) & 1u) ^ 1u, &abort_flag);
         if (!ok) break;
         const unsigned stage = smem_u32(smem) + s * Shape::STAGE_BYTES;
-#pragma unroll
-        for (int j = 0; j < 6; ++j)
-          cp_async_8(stage + Shape::B_AT + (sub + 16 * j) * 128 + to, w_at[j] + (size_t)i * 64, (live >> j) & 1u ? 8 : 0);
         const unsigned word = stage + Shape::WS_AT + lane * 16 + ((t >> 5) << 2);
         cp_async_4(word, w_scales + first_word + (size_t)i * MX4_TILE_BYTES, first_live ? 4 : 0);
         if (t < 64) cp_async_4(word + 512, w_scales + second_word + (size_t)i * MX4_TILE_BYTES, second_live ? 4 : 0);
@@ -455,46 +443,9 @@ mx4_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
 }
 
 // ------------------------------------------------------------------------------- host side
-typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
-                                  const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
-                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-static EncodeTiledFn encode_tiled() {
-  static EncodeTiledFn fn = nullptr;
-  static std::once_flag once;
-  std::call_once(once, [] {
-    void* entry = nullptr;
-    cudaDriverEntryPointQueryResult result;
-    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &entry, 12000, cudaEnableDefault, &result) == cudaSuccess &&
-        result == cudaDriverEntryPointSuccess)
-      fn = reinterpret_cast<EncodeTiledFn>(entry);
-  });
-  return fn;
-}
-
-// A matrix [rows, columns] of elements of `type`, `pitch` bytes apart, cut into boxes.
-static int make_map(CUtensorMap* map, CUtensorMapDataType type, const void* base, long long rows, long long columns, long long pitch,
-                    int box_rows, int box_columns, CUtensorMapSwizzle swizzle) {
-  EncodeTiledFn fn = encode_tiled();
-  if (!fn) SRB_FAIL("gemm_mx4_pair: the driver does not offer cuTensorMapEncodeTiled");
-  const cuuint64_t dims[2] = {(cuuint64_t)columns, (cuuint64_t)rows};
-  const cuuint64_t strides[1] = {(cuuint64_t)pitch};
-  const cuuint32_t box[2] = {(cuuint32_t)box_columns, (cuuint32_t)box_rows};
-  const cuuint32_t element[2] = {1, 1};
-  const CUresult status = fn(map, type, 2, const_cast<void*>(base), dims, strides, box, element, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
-                             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (status != CUDA_SUCCESS) SRB_FAIL("gemm_mx4_pair: cuTensorMapEncodeTiled failed with %d", (int)status);
-  return SRB_OK;
-}
-static int make_bytes_map(CUtensorMap* map, const void* base, long long rows, long long bytes, int box_rows) {
-  return make_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, base, rows, bytes, bytes, box_rows, 128, CU_TENSOR_MAP_SWIZZLE_128B);
-}
-static int make_scales_map(CUtensorMap* map, const void* base, long long tiles, int at_once) {
-  return make_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, base, tiles, 128, MX4_TILE_BYTES, at_once, 128, CU_TENSOR_MAP_SWIZZLE_NONE);
-}
-
 template <bool FOUR, int MODE, bool GROUPED>
 static int launch_pair(const CUtensorMap (&maps)[5], const PairMx4Args& a, int max_tiles, cudaStream_t s) {
-  using Shape = PairShape<FOUR>;
+  using Shape = PairShape<FOUR, MODE == MXP_GATED>;
   const int pairs = std::max(1, std::min(srb_sm_count() / 2, max_tiles));
   const size_t smem = (size_t)Shape::STAGES * Shape::STAGE_BYTES + MXP_EPILOGUE_WARPS * MXP_BOX_BYTES + 1024;
   auto kernel = mx4_pair_kernel<FOUR, MODE, GROUPED>;
@@ -509,9 +460,10 @@ extern "C" int srb_mx4_linear_pair(const void* x, const void* x_scales, int four
                                    void* out, long long ldo, int rows, int features, int width, int out_float, int* error_word, void* stream) {
   if (rows <= 0 || features <= 0) return SRB_OK;
   if (width <= 0) SRB_FAIL("mx4_linear_pair: inner size %d must be positive", width);
+  if ((uintptr_t)w & 31) SRB_FAIL("mx4_linear_pair: codes must start on a 32-byte border");
   if (((uintptr_t)out & 15) || ldo * (out_float ? 4 : 2) % 16) SRB_FAIL("mx4_linear_pair: rows of the result must start on 16-byte borders");
   PairMx4Args a = {};
-  a.w = (const uint8_t*)w; a.w_scales = (const uint8_t*)w_scales; a.bias = bias; a.out = out; a.ldo = ldo; a.rows = rows;
+  a.w_scales = (const uint8_t*)w_scales; a.bias = bias; a.out = out; a.ldo = ldo; a.rows = rows;
   a.features = a.w_rows = features; a.k_tiles = mx4_tiles(width); a.error_word = error_word;
   a.x_lo_row = rows; a.xs_lo_tile = mx4_tiles(rows) * a.k_tiles;
   a.tiles_t = (rows + MXP_TILE - 1) / MXP_TILE; a.tiles_f = (features + MXP_N - 1) / MXP_N;
@@ -520,8 +472,8 @@ extern "C" int srb_mx4_linear_pair(const void* x, const void* x_scales, int four
   CUtensorMap maps[5];
   if (make_bytes_map(&maps[0], x, four ? rows : 2ll * rows, a.k_tiles * (four ? 64 : 128), MXP_ROWS) != SRB_OK ||
       make_scales_map(&maps[1], x_scales, (four ? 1 : 2) * row_tiles * a.k_tiles, four ? 2 : 1) != SRB_OK ||
-      make_bytes_map(&maps[2], w, features, a.k_tiles * 64, MXP_HALF) != SRB_OK ||
-      make_scales_map(&maps[3], w_scales, (long long)mx4_tiles(features) * a.k_tiles, 2) != SRB_OK ||
+      (four ? make_bytes_map(&maps[2], w, features, a.k_tiles * 64, MXP_HALF) : make_codes_map(&maps[2], w, features, a.k_tiles, MXP_HALF)) != SRB_OK ||
+      make_scales_map(&maps[3], w_scales, (long long)mx4_tiles(features) * a.k_tiles, four ? 2 : 1) != SRB_OK ||
       make_map(&maps[4], out_float ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, out, rows, features, ldo * (out_float ? 4 : 2),
                32, out_float ? 16 : 32, CU_TENSOR_MAP_SWIZZLE_64B) != SRB_OK)
     return SRB_ERR_INVALID;
@@ -537,10 +489,11 @@ extern "C" int srb_mx4_experts_pair(const void* x, const void* x_scales, const v
                                     float act_param, int* error_word, void* stream) {
   if (max_tiles <= 0 || features <= 0) return SRB_OK;
   if (width <= 0) SRB_FAIL("mx4_experts_pair: inner size %d must be positive", width);
+  if ((uintptr_t)w & 31) SRB_FAIL("mx4_experts_pair: codes must start on a 32-byte border");
   if (activation < 0 || activation >= SRB_ACT_COUNT) SRB_FAIL("mx4_experts_pair: unknown activation %d", activation);
   if (mode != MXP_F32 && mode != MXP_GATED && mode != MXP_ACT) SRB_FAIL("mx4_experts_pair: mode %d is not float, gated or activated", mode);
   PairMx4Args a = {};
-  a.w = (const uint8_t*)w; a.w_scales = (const uint8_t*)w_scales; a.out = out; a.out_scales = (uint8_t*)out_scales; a.rows = slots;
+  a.w_scales = (const uint8_t*)w_scales; a.out = out; a.out_scales = (uint8_t*)out_scales; a.rows = slots;
   a.features = features; a.w_rows = mode == MXP_GATED ? 2 * features : features; a.k_tiles = mx4_tiles(width); a.activation = activation;
   a.act_param = act_param; a.error_word = error_word; a.plan = plan; a.experts = experts;
   const long long rows = 256ll * max_tiles;
@@ -550,13 +503,15 @@ extern "C" int srb_mx4_experts_pair(const void* x, const void* x_scales, const v
   a.tiles_f = (covered + per_tile - 1) / per_tile;
   a.ldo = mode == MXP_F32 ? features : 128 * out_tiles;
   a.out_part = (size_t)rows * a.ldo; a.os_part = (size_t)2 * max_tiles * out_tiles * MX4_TILE_BYTES;
-  if (2 * rows > 0x7fffffff || (long long)max_tiles * a.tiles_f > 0x3fffffff) SRB_FAIL("mx4_experts_pair: %d tiles are too many", max_tiles);
+  if (2 * rows > 0x7fffffff || (long long)experts * a.w_rows > 0x7fffffff || (long long)experts * mx4_tiles(a.w_rows) * a.k_tiles > 0x7fffffff || (long long)max_tiles * a.tiles_f > 0x3fffffff) SRB_FAIL("mx4_experts_pair: %d tiles are too many", max_tiles);
   if (mode == MXP_F32 && (((uintptr_t)out & 15) || features % 4)) SRB_FAIL("mx4_experts_pair: rows of the result must start on 16-byte borders");
   CUtensorMap maps[5];
   if (make_bytes_map(&maps[0], x, 2 * rows, a.k_tiles * 128, MXP_ROWS) != SRB_OK ||
-      make_scales_map(&maps[1], x_scales, 4ll * max_tiles * a.k_tiles, 1) != SRB_OK)
+      make_scales_map(&maps[1], x_scales, 4ll * max_tiles * a.k_tiles, 1) != SRB_OK ||
+      make_codes_map(&maps[2], w, (long long)experts * a.w_rows, a.k_tiles, MXP_HALF) != SRB_OK ||
+      make_scales_map(&maps[3], w_scales, (long long)experts * mx4_tiles(a.w_rows) * a.k_tiles, 1) != SRB_OK)
     return SRB_ERR_INVALID;
-  maps[2] = maps[3] = maps[4] = maps[0];
+  maps[4] = maps[0];
   if (mode == MXP_F32 && make_map(&maps[4], CU_TENSOR_MAP_DATA_TYPE_FLOAT32, out, slots, features, features * 4ll, 32, 16, CU_TENSOR_MAP_SWIZZLE_64B) != SRB_OK)
     return SRB_ERR_INVALID;
   cudaStream_t s = (cudaStream_t)stream;

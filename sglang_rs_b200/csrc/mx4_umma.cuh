@@ -5,7 +5,9 @@
 // codes and eight that are not read.  Scales lie in tensor memory: row r's in lane r % 32 (of every quarter of the lanes) and
 // column r / 32, a byte for each of four consecutive blocks of 32 entries; the instruction descriptor says which bytes a step takes.
 #pragma once
+#include "common.cuh"
 #include "tcgen05_helpers.cuh"
+#include <mutex>
 
 #define MX_E4M3 0u
 #define MX_E2M1 5u       // among the types of kind mxf8f6f4
@@ -45,6 +47,49 @@ __device__ __forceinline__ void tmem_load_8(unsigned address, float (&v)[8]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
   for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(r[i]);
+}
+
+// ---- maps for TMA ----------------------------------------------------------------------------------------------------
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                  const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+static EncodeTiledFn encode_tiled() {
+  static EncodeTiledFn fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* entry = nullptr;
+    cudaDriverEntryPointQueryResult result;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &entry, 12000, cudaEnableDefault, &result) == cudaSuccess &&
+        result == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<EncodeTiledFn>(entry);
+  });
+  return fn;
+}
+
+// A matrix [rows, columns] of elements of `type`, `pitch` bytes apart, cut into boxes.
+static int make_map(CUtensorMap* map, CUtensorMapDataType type, const void* base, long long rows, long long columns, long long pitch,
+                    int box_rows, int box_columns, CUtensorMapSwizzle swizzle) {
+  EncodeTiledFn fn = encode_tiled();
+  if (!fn) SRB_FAIL("four-bit products: the driver does not offer cuTensorMapEncodeTiled");
+  const cuuint64_t dims[2] = {(cuuint64_t)columns, (cuuint64_t)rows};
+  const cuuint64_t strides[1] = {(cuuint64_t)pitch};
+  const cuuint32_t box[2] = {(cuuint32_t)box_columns, (cuuint32_t)box_rows};
+  const cuuint32_t element[2] = {1, 1};
+  const CUresult status = fn(map, type, 2, const_cast<void*>(base), dims, strides, box, element, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+                             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (status != CUDA_SUCCESS) SRB_FAIL("four-bit products: cuTensorMapEncodeTiled failed with %d", (int)status);
+  return SRB_OK;
+}
+static int make_bytes_map(CUtensorMap* map, const void* base, long long rows, long long bytes, int box_rows) {
+  return make_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, base, rows, bytes, bytes, box_rows, 128, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+// Codes that stand 16 to 16 bytes in shared memory, as kind mxf8f6f4 takes them (a box of 128 entries is 128 bytes a row there; the barrier
+// counts the 64 bytes of codes).  Base on a 32-byte border, `k_tiles` * 64 bytes a row.
+static int make_codes_map(CUtensorMap* map, const void* base, long long rows, int k_tiles, int box_rows) {
+  return make_map(map, CU_TENSOR_MAP_DATA_TYPE_16U4_ALIGN16B, base, rows, k_tiles * 128ll, k_tiles * 64ll, box_rows, 128, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+static int make_scales_map(CUtensorMap* map, const void* base, long long tiles, int at_once) {
+  return make_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, base, tiles, 128, 512, at_once, 128, CU_TENSOR_MAP_SWIZZLE_NONE);
 }
 
 // ---- pairs of CTAs (cta_group::2): M = 256, the even CTA's thread issues for both -----------------------------------------

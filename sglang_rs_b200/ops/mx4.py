@@ -74,7 +74,7 @@ def _need_mx4(q: Mx4, name: str, stacked: Optional[bool]) -> None:
         raise KernelError(f"{name} must be {'a stack of matrices' if stacked else 'one matrix'}, found {q.shape}")
     lead = q.codes.shape[:-2]
     if (q.codes.dim() not in (2, 3) or q.width <= 0 or q.codes.shape[-1] != 64 * _tiles(q.width)
-            or q.scales.shape != (*lead, _tiles(q.rows), _tiles(q.width), 512) or (q.codes.data_ptr() | q.scales.data_ptr()) % 16):
+            or q.scales.shape != (*lead, _tiles(q.rows), _tiles(q.width), 512) or q.codes.data_ptr() % 32 or q.scales.data_ptr() % 16):
         raise KernelError(f"{name}: codes {tuple(q.codes.shape)} and scales {tuple(q.scales.shape)} do not hold rows of {q.width}")
 
 
