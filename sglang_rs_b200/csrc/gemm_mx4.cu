@@ -2,18 +2,23 @@
 //
 // The weight is the M side: a block owns 128 rows of W and up to 64 rows of X, the N side.  The tensor cores take the four-bit entries as
 // they are, so nothing is unpacked: turning 13 T entries a second (what the memory brings) into bfloat16 would take every instruction the SMs
-// issue.  Rows of X come as four-bit codes or as two eight-bit parts of a bfloat16 (mx4.cuh), which are columns of their own and meet in the
-// epilogue.  A product step of 128 entries: the codes by TMA, which sets eight bytes to each 16 of a row in shared memory as the instruction
-// wants them (by cp.async of eight bytes, 50 MB of codes took 24 us instead of LATER), and by cp.async the rows of X and both sides' scales, one
-// word for each row.
+// issue.  Rows of X come as four-bit codes or as the two eight-bit parts of a bfloat16 (mx4.cuh), each multiplied into the same sums.
 //
-// K is cut where the row tiles are fewer than two blocks an SM: the blocks of a cluster take a part each, leave their sums in shared memory
-// and add them in block order, so a result does not depend on timing.
+// A step is 128 entries of K.  All of it comes by TMA: the codes, set eight bytes to each 16 as kind mxf8f6f4 wants them, the rows of X, and
+// both sides' scales in the tiles that mx4.cuh lays them out in, which the issuing thread copies to tensor memory ahead of the step's products.
+// (With cp.async for the scales and for X a step took 700 cycles however many were in flight: the fence that ordinary writes need ahead of the
+// products stands in the products' way.)
 //
-// Warps 0-3 copy (nothing waits for a copy but the products) and then store, warp 4 issues the products.  Waits are bounded; one that runs out flags SRB_FLAG_WAIT_TIMEOUT.
+// Two blocks an SM.  K is cut where the row tiles are fewer than that: the blocks of a cluster take a part each, leave their sums in shared
+// memory and add them in block order, so a result does not depend on timing.  Otherwise a block walks tiles, copying for the next one while
+// the last one's sums, in one of two buffers, are stored.
 //
-// Over experts (GROUPED) a block's rows are up to 64 slots of one expert (the plan of csrc/moe.cu).  The gated mode has 64 gate rows over the
-// 64 up rows of the same features, and leaves act(gate) * up as eight-bit parts again, rounded from 32 bits, for the next product.
+// Over experts (GROUPED) a block's rows are up to 32 slots of one expert (the plan of csrc/moe.cu), X and the parts that the first product
+// leaves having room for 64 rows a tile: scales of a product may begin at an even column of tensor memory alone (an odd one faults), that is at a
+// multiple of 64 rows.  The gated mode multiplies the gate rows and the up rows of 128 features into sums of their own, a feature
+// a lane in both, and leaves act(gate) * up as eight-bit parts, rounded once from 32 bits, a warp's 32 features a block.
+//
+// Warps: 0 copies, 1 products and tensor memory, 2-5 epilogue.  Waits are bounded; one that runs out flags SRB_FLAG_WAIT_TIMEOUT.
 #include "common.cuh"
 #include "activations.cuh"
 #include "mx4.cuh"
@@ -23,304 +28,330 @@
 SRB_DEFINE_LAST_ERROR()
 SRB_DEFINE_PDL_SWITCH()
 
-#define MXF_TOKENS 64            // rows of X of a block
-#define MXF_COPY_THREADS 128
-#define MXF_THREADS 160
-#define MXF_A_BYTES 16384        // 128 rows x 128 entries, 16 to 16 bytes
+#define MXF_TOKENS 64            // rows of X of a tile, at most
+#define MXF_SLOTS 32             // ... over experts, at most
+#define MXF_ROOM 64              // ... and rows that a tile has room for
+#define MXF_THREADS 192
+#define MXF_EPILOGUE_THREADS 128
+#define MXF_W_BYTES 16384        // 128 rows x 128 entries, 16 to 16 bytes
+#define MXF_MAX_SPLITS 8         // blocks of a cluster
+#define MXF_PLACES 4             // of a step's scales in tensor memory
 #define MXF_BF16 0     // out bfloat16 = x w^T + bias
 #define MXF_F32 1      // out float
 #define MXF_GATED 2    // out two eight-bit parts of act(x gate^T) * (x up^T), the up rows `features` behind the gate rows
 #define MXF_ACT 5      // ... of act(x w^T)
 
 struct FewArgs {
-  const uint8_t* x;              // codes, or the first of two parts
-  const uint8_t* x_scales;
-  size_t x_part, xs_part;        // bytes from the first part to the second
-  const uint8_t* w_scales;
   const float* bias;
   void* out;
   uint8_t* out_scales;           // of parts
   size_t ldo;                    // elements; bytes of parts
   size_t out_part, os_part;
   int rows, features, w_rows, k_tiles, splits;
-  int columns;                   // room for columns of the N side
+  int columns;                   // of the N side: rows of X of a tile, up to a multiple of 16
+  int x_lo_row, xs_lo_tile;      // where the second part's rows and tiles of scales begin
+  int ws_tiles, up_tile;         // row tiles of scales of a matrix; the one where the up rows begin
+  int tiles_f, tiles_t;
   int activation;
   float act_param;
   int* error_word;
   const int* plan;               // GROUPED
-  const int* slot_row;           // rows of x by slot, or null: the slots themselves
-  int experts;
+  int experts, tile_slots;
 };
 
-__device__ __forceinline__ void cp_async_8(unsigned dst, const void* src, int bytes) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;\n" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+template <bool FOUR, bool GATED>
+struct FewShape {
+  static constexpr int PARTS = FOUR ? 1 : 2, SIDES = GATED ? 2 : 1;
+  static constexpr int PLACE_COLUMNS = 4 * (SIDES + PARTS);
+  static constexpr int SCALE_BYTES = 512 * (SIDES + PARTS);
+  static __host__ __device__ constexpr int stage_bytes(int columns) { return SIDES * MXF_W_BYTES + PARTS * columns * 128; }
+  // what the barrier counts: codes without the gaps
+  static __host__ __device__ constexpr int tx_bytes(int columns) { return SIDES * MXF_W_BYTES / 2 + (FOUR ? columns * 64 : 2 * columns * 128) + SCALE_BYTES; }
+};
+
+__device__ __forceinline__ float4 few_load_peer(const float* mine, unsigned rank) {
+  unsigned remote;
+  float4 v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(smem_u32(mine)), "r"(rank));
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(remote) : "memory");
+  return v;
 }
-__device__ __forceinline__ void cp_async_4(unsigned dst, const void* src, int bytes) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;\n" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+
+// What a tile is, the same in every role.
+struct FewTile {
+  int matrix, feature0;
+  int x_row0;                    // the first row of X (with room for MXF_ROOM a tile, over experts)
+  int out_row0, count;
+};
+template <bool GROUPED>
+__device__ __forceinline__ FewTile few_tile(const FewArgs& a, int item) {
+  FewTile t;
+  if (GROUPED) {
+    const int* first_slot = a.plan + 1;
+    const int* tiles = first_slot + a.experts + 1;
+    const int index = item / a.tiles_f;
+    t.matrix = tiles[2 * index];
+    t.out_row0 = tiles[2 * index + 1];
+    t.count = min(a.tile_slots, first_slot[t.matrix + 1] - t.out_row0);
+    t.x_row0 = index * MXF_ROOM;
+    t.feature0 = item % a.tiles_f * 128;
+  } else {
+    t.matrix = 0;
+    t.x_row0 = t.out_row0 = item / a.tiles_f * MXF_TOKENS;
+    t.count = min(MXF_TOKENS, a.rows - t.out_row0);
+    t.feature0 = item % a.tiles_f * 128;
+  }
+  return t;
 }
-__device__ __forceinline__ void cp_async_16_to(unsigned dst, const void* src, int bytes) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void few_copy_threads_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
 
 template <bool FOUR, int MODE, bool GROUPED, int STAGES>
-__global__ void __launch_bounds__(MXF_THREADS)
-mx4_few_kernel(const __grid_constant__ CUtensorMap map_w, const FewArgs a) {
+__global__ void __launch_bounds__(MXF_THREADS, 2)
+mx4_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_ws, const __grid_constant__ CUtensorMap map_x,
+               const __grid_constant__ CUtensorMap map_xs, const FewArgs a) {
   constexpr bool GATED = MODE == MXF_GATED, PARTS = MODE == MXF_GATED || MODE == MXF_ACT;
-  constexpr int FEATURES = GATED ? 64 : 128;
+  using Shape = FewShape<FOUR, GATED>;
   extern __shared__ unsigned char smem_unaligned[];
   unsigned char* smem = reinterpret_cast<unsigned char*>(((uintptr_t)smem_unaligned + 1023) & ~(uintptr_t)1023);
-  __shared__ __align__(8) unsigned long long full_bar[STAGES], empty_bar[STAGES], done_bar;
+  __shared__ __align__(8) unsigned long long full_bar[STAGES], empty_bar[STAGES], acc_full[2], acc_empty[2];
   __shared__ unsigned tmem_holder;
   __shared__ int abort_flag;
-  __shared__ int x_row[MXF_TOKENS];
 
-  const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
-  srb_launch_dependents();
-  int matrix = 0, token0 = blockIdx.y * MXF_TOKENS, count = min(MXF_TOKENS, a.rows - token0);
-  if (GROUPED) {
-    srb_grid_dependency_wait();
-    if ((int)blockIdx.y >= a.plan[0]) return;
-    const int* tiles = a.plan + 1 + a.experts + 1;
-    matrix = tiles[2 * blockIdx.y];
-    token0 = tiles[2 * blockIdx.y + 1];
-    count = min(MXF_TOKENS, a.plan[1 + matrix + 1] - token0);
-  }
-  const int part_columns = FOUR ? (count + 15) & ~15 : (count + 7) & ~7;
-  const int columns = FOUR ? part_columns : 2 * part_columns;
-  const int rank = blockIdx.x % a.splits, feature0 = blockIdx.x / a.splits * FEATURES;
-  const int kt0 = (int)((long long)rank * a.k_tiles / a.splits), kt1 = (int)((long long)(rank + 1) * a.k_tiles / a.splits);
-  const int steps = kt1 - kt0;
-  const int stage_bytes = MXF_A_BYTES + a.columns * 128;
-  const unsigned scales0 = smem_u32(smem) + STAGES * stage_bytes;        // per stage 512 bytes of W's and 512 of X's
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = blockIdx.x % a.splits;
+  const int kt0 = (int)((long long)rank * a.k_tiles / a.splits), steps = (int)((long long)(rank + 1) * a.k_tiles / a.splits) - kt0;
+  const int first_item = blockIdx.x / a.splits, item_step = gridDim.x / a.splits;
+  const int stage_bytes = Shape::stage_bytes(a.columns);
+  const unsigned stages = smem_u32(smem), scales = stages + STAGES * stage_bytes;
 
-  if (t == 0) {
+  if (threadIdx.x == 0) {
     abort_flag = 0;
     for (int s = 0; s < STAGES; ++s) {
-      mbar_init(smem_u32(&full_bar[s]), MXF_COPY_THREADS + 1);      // and the word that W's bytes are awaited
+      mbar_init(smem_u32(&full_bar[s]), 1);
       mbar_init(smem_u32(&empty_bar[s]), 1);
     }
-    mbar_init(smem_u32(&done_bar), 1);
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(smem_u32(&acc_full[b]), 1);
+      mbar_init(smem_u32(&acc_empty[b]), MXF_EPILOGUE_THREADS / 32);
+    }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 4) tmem_alloc(smem_u32(&tmem_holder), 256);
-  if (!GROUPED) srb_grid_dependency_wait();
-  if (t < MXF_TOKENS) x_row[t] = t < count ? (GROUPED && a.slot_row ? a.slot_row[token0 + t] : token0 + t) : 0;
+  if (warp == 1) tmem_alloc(smem_u32(&tmem_holder), 256);
+  srb_launch_dependents();
+  srb_grid_dependency_wait();
+  const int items = (GROUPED ? a.plan[0] : a.tiles_t) * a.tiles_f;
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const unsigned tmem = tmem_holder;
-  bool ok = true;
+  // sums: a buffer is `columns` for each side; scales lie behind 128 columns
+  const int buffer_columns = Shape::SIDES * a.columns;
 
-  if (warp < 4) {
-    // ---- copies: a thread has chunk t % 8 of columns t / 8 + 16 i of X, and the scales of row t of W and of column t
-    const uint8_t* w_scales = a.w_scales + (size_t)matrix * mx4_tiles(a.w_rows) * a.k_tiles * MX4_TILE_BYTES;
-    const int chunk = t & 7, sub = t >> 3;
-    const unsigned place = (unsigned)(chunk ^ (sub & 7)) << 4;
-    auto w_row = [&](int r, bool& live) {
-      const int feature = feature0 + (GATED ? r & 63 : r);
-      live = feature < a.features;
-      return !live ? 0 : GATED && r >= 64 ? a.features + feature : feature;
-    };
-    bool scale_live;
-    const int scale_row = w_row(t, scale_live);
-    // the column of X whose scales this thread brings
-    const bool second = !FOUR && t >= part_columns;
-    const int x_token = second ? t - part_columns : t;
-    const bool x_scale_live = t < columns && x_token < count;
-    const int x_scale_row = x_scale_live ? x_row[x_token] : 0;
-    const uint8_t* x_scales = a.x_scales + (second ? a.xs_part : 0);
-    const size_t x_pitch = (size_t)a.k_tiles * (FOUR ? 64 : 128);
-    for (int i = 0; i < steps; ++i) {
-      const int s = i % STAGES, kt = kt0 + i;
-      if (i >= STAGES && !mbar_wait(smem_u32(&empty_bar[s]), (unsigned)(i / STAGES - 1) & 1u, &abort_flag)) break;
-      const unsigned w_to = smem_u32(smem) + s * stage_bytes, x_to = w_to + MXF_A_BYTES, scales_to = scales0 + s * 1024;
-      if (warp == 0) {
-        __syncwarp();
+  if (warp == 0) {
+    unsigned round = 0;
+    bool ok = true;
+    for (int item = first_item; item < items && ok; item += item_step) {
+      const FewTile t = few_tile<GROUPED>(a, item);
+      const int w_row = t.matrix * a.w_rows + t.feature0;
+      const int ws_tile = (t.matrix * a.ws_tiles + (t.feature0 >> 7)) * a.k_tiles, xs_tile = (t.x_row0 >> 7) * a.k_tiles;
+      for (int i = 0; i < steps; ++i, ++round) {
+        const int s = (int)(round % STAGES), kt = kt0 + i;
+        ok = mbar_wait_warp(smem_u32(&empty_bar[s]), ((round / STAGES) & 1u) ^ 1u, &abort_flag);
+        if (!ok) break;
+        const unsigned bar = smem_u32(&full_bar[s]), to = stages + s * stage_bytes, scales_to = scales + s * Shape::SCALE_BYTES;
         if (elect_one()) {
-          const unsigned bar = smem_u32(&full_bar[s]);
-          mbar_expect_tx(bar, MXF_A_BYTES / 2);
-          tma_load_2d(w_to, &map_w, bar, kt * 128, matrix * a.w_rows + feature0);
-          if (GATED) tma_load_2d(w_to + MXF_A_BYTES / 2, &map_w, bar, kt * 128, matrix * a.w_rows + a.features + feature0);
+          mbar_expect_tx(bar, Shape::tx_bytes(a.columns));
+          tma_load_2d(to, &map_w, bar, kt * 128, w_row);
+          tma_load_2d(scales_to, &map_ws, bar, 0, ws_tile + kt);
+          if (GATED) {
+            tma_load_2d(to + MXF_W_BYTES, &map_w, bar, kt * 128, w_row + a.features);
+            tma_load_2d(scales_to + 512, &map_ws, bar, 0, ws_tile + a.up_tile * a.k_tiles + kt);
+          }
+          const unsigned x_to = to + Shape::SIDES * MXF_W_BYTES, xs_to = scales_to + 512 * Shape::SIDES;
+          tma_load_2d(x_to, &map_x, bar, kt * 128, t.x_row0);
+          tma_load_2d(xs_to, &map_xs, bar, 0, xs_tile + kt);
+          if (!FOUR) {
+            tma_load_2d(x_to + a.columns * 128, &map_x, bar, kt * 128, a.x_lo_row + t.x_row0);
+            tma_load_2d(xs_to + 512, &map_xs, bar, 0, a.xs_lo_tile + xs_tile + kt);
+          }
         }
         __syncwarp();
       }
-      cp_async_4(scales_to + lane * 16 + warp * 4, w_scales + mx4_scale_word(scale_row, kt, a.k_tiles), scale_live ? 4 : 0);
-      for (int n = sub; n < columns; n += 16) {
-        const bool low = !FOUR && n >= part_columns;
-        const int token = low ? n - part_columns : n;
-        const bool live = token < count;
-        const uint8_t* src = a.x + (low ? a.x_part : 0) + (size_t)x_row[live ? token : 0] * x_pitch;
-        if (FOUR) cp_async_8(x_to + n * 128 + place, src + kt * 64 + chunk * 8, live ? 8 : 0);
-        else cp_async_16_to(x_to + n * 128 + place, src + kt * 128 + chunk * 16, live ? 16 : 0);
-      }
-      if (t < columns)
-        cp_async_4(scales_to + 512 + lane * 16 + warp * 4, x_scales + mx4_scale_word(x_scale_row, kt, a.k_tiles), x_scale_live ? 4 : 0);
-      copies_arrive(smem_u32(&full_bar[s]));
     }
-    asm volatile("cp.async.wait_all;" ::: "memory");
-    if (abort_flag) {
-      // copies by TMA in flight when a wait ran out write into this block's memory: give them time to land
+    if (abort_flag && round > 0) {
+      // copies in flight when a wait ran out write into this block's memory: give them time to land
       const long long start = clock64();
       while (clock64() - start < 4000000ll) {}
     }
-  } else {
-    // ---- products
-    const unsigned idesc = mx_idesc(MX_E2M1, FOUR ? MX_E2M1 : MX_E4M3, 128, columns);
-    for (int i = 0; i < steps && ok; ++i) {
-      const int s = i % STAGES;
-      ok = mbar_wait_warp(smem_u32(&full_bar[s]), (unsigned)(i / STAGES) & 1u, &abort_flag);
+  } else if (warp == 1) {
+    const unsigned idesc = mx_idesc(MX_E2M1, FOUR ? MX_E2M1 : MX_E4M3, 128, a.columns);
+    unsigned round = 0;
+    int local = 0;
+    bool ok = true;
+    for (int item = first_item; item < items && ok; item += item_step, ++local) {
+      const int b = local & 1;
+      // rows of X that start in the middle of a tile of scales
+      const unsigned x_shift = (unsigned)(few_tile<GROUPED>(a, item).x_row0 & 127) >> 5;
+      ok = mbar_wait_warp(smem_u32(&acc_empty[b]), (((unsigned)local >> 1) & 1u) ^ 1u, &abort_flag);
       if (!ok) break;
-      fence_proxy_async_shared();
       tc_fence_after();
-      const unsigned w_at = smem_u32(smem) + s * stage_bytes;
-      const unsigned long long a_desc = smem_descriptor(w_at), b_desc = smem_descriptor(w_at + MXF_A_BYTES);
-      const unsigned sa = tmem + 128 + 8 * s, sb = sa + 4;
-      if (elect_one()) {
-        tmem_copy_scales(sa, scales_descriptor(scales0 + s * 1024));
-        tmem_copy_scales(sb, scales_descriptor(scales0 + s * 1024 + 512));
+      const unsigned acc = tmem + b * buffer_columns;
+      for (int i = 0; i < steps; ++i, ++round) {
+        const int s = (int)(round % STAGES);
+        ok = mbar_wait_warp(smem_u32(&full_bar[s]), (round / STAGES) & 1u, &abort_flag);
+        if (!ok) break;
+        tc_fence_after();
+        const unsigned at = stages + s * stage_bytes, place = tmem + 128 + (round % MXF_PLACES) * Shape::PLACE_COLUMNS;
+        const unsigned long long w_desc = smem_descriptor(at), x_desc = smem_descriptor(at + Shape::SIDES * MXF_W_BYTES);
+        const unsigned long long x_lo = (unsigned long long)(a.columns * 128 >> 4);
+        if (elect_one()) {
+          const unsigned long long from = scales_descriptor(scales + s * Shape::SCALE_BYTES);
 #pragma unroll
-        for (unsigned k = 0; k < 4; ++k)
-          umma_mx8(tmem, a_desc + 2 * k, b_desc + 2 * k, mx_idesc_step(idesc, k), sa, sb, (i > 0 || k > 0) ? 1u : 0u);
-        umma_commit(smem_u32(&empty_bar[s]));
-        if (i == steps - 1) umma_commit(smem_u32(&done_bar));
-      }
-      __syncwarp();
-    }
-  }
-
-  // ---- epilogue: warp w has lanes 32 w .. + 31 of tensor memory, a row of W a lane, and all columns
-  float* shared = reinterpret_cast<float*>(smem);            // the stages are done with
-  if (warp < 4) {
-    mbar_wait_warp(smem_u32(&done_bar), 0u, &abort_flag);
-    few_copy_threads_sync();
-    ok = *reinterpret_cast<volatile int*>(&abort_flag) == 0;  // the same in every warp
-    tc_fence_after();
-  }
-  const unsigned lane_address = tmem + ((unsigned)(warp * 32) << 16);
-  auto eight = [&](int token, float (&v)[8]) {
-    tmem_load_8(lane_address + token, v);
-    if (!FOUR) {
-      float low[8];
-      tmem_load_8(lane_address + part_columns + token, low);
+          for (int j = 0; j < Shape::SCALE_BYTES / 512; ++j) tmem_copy_scales(place + 4 * j, from + j * (512 >> 4));
+          const unsigned xs = place + 4 * Shape::SIDES + x_shift;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] += low[j];
-    }
-  };
-  auto store = [&](int token, int feature, float v) {
-    if (a.bias) v += a.bias[feature];
-    const size_t at = (size_t)(token0 + token) * a.ldo + feature;
-    if (MODE == MXF_F32) reinterpret_cast<float*>(a.out)[at] = v;
-    else reinterpret_cast<__nv_bfloat16*>(a.out)[at] = __float2bfloat16_rn(v);
-  };
-  if (PARTS) {
-    if (warp < 4 && ok) {
-      if (GATED) {
-        if (warp >= 2) {
-          for (int token = 0; token < count; token += 8) {
-            float v[8];
-            eight(token, v);
+          for (int part = 0; part < Shape::PARTS; ++part)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) shared[(token + j) * 64 + (t & 63)] = v[j];
-          }
+            for (unsigned k = 0; k < 4; ++k) {
+              const unsigned accumulate = (i > 0 || part > 0 || k > 0) ? 1u : 0u;
+              umma_mx8(acc, w_desc + 2 * k, x_desc + part * x_lo + 2 * k, mx_idesc_step(idesc, k), place, xs + 4 * part, accumulate);
+              if (GATED)
+                umma_mx8(acc + a.columns, w_desc + (MXF_W_BYTES >> 4) + 2 * k, x_desc + part * x_lo + 2 * k, mx_idesc_step(idesc, k),
+                         place + 4, xs + 4 * part, accumulate);
+            }
+          umma_commit(smem_u32(&empty_bar[s]));
+          if (i == steps - 1) umma_commit(smem_u32(&acc_full[b]));
         }
-        few_copy_threads_sync();
+        __syncwarp();
       }
-      if (!GATED || warp < 2) {
-        const int feature = feature0 + t;
-        for (int token = 0; token < count; token += 8) {
-          float v[8];
-          eight(token, v);
+    }
+  } else {
+    // ---- epilogue: warp w has lanes 32 (w % 4) .. + 31 of tensor memory, a feature a lane, and all columns
+    const int quarter = warp & 3, in_tile = quarter * 32 + lane;
+    const unsigned lane_address = tmem + ((unsigned)(quarter * 32) << 16);
+    int local = 0;
+    for (int item = first_item; item < items; item += item_step, ++local) {
+      const int b = local & 1;
+      const FewTile t = few_tile<GROUPED>(a, item);
+      const int feature = t.feature0 + in_tile;
+      if (!mbar_wait_warp(smem_u32(&acc_full[b]), ((unsigned)local >> 1) & 1u, &abort_flag)) break;
+      tc_fence_after();
+      const unsigned sums = lane_address + b * buffer_columns;
+      const float bias = !PARTS && a.splits == 1 && a.bias && feature < a.features ? a.bias[feature] : 0.f;
+      for (int token = 0; token < t.count; token += 8) {
+        float v[8];
+        tmem_load_8(sums + token, v);
+        if (PARTS) {
+          float up[8];
+          if (GATED) tmem_load_8(sums + a.columns + token, up);
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
-            if (token + j >= count) break;
-            float r = srb_gated<true>(a.activation, v[j], GATED ? shared[(token + j) * 64 + t] : 1.0f, a.act_param);
-            if (feature >= a.features) r = 0.f;              // behind the rows of W: the part that pads the parts' rows
+            if (token + j >= t.count) break;
+            float r = srb_gated<true>(a.activation, v[j], GATED ? up[j] : 1.0f, a.act_param);
+            if (feature >= a.features) r = 0.f;              // the part that pads the parts' rows
             const unsigned high = mx8_scale_high(__reduce_max_sync(0xffffffffu, __float_as_uint(r) & 0x7fffffffu)), low = mx8_scale_low(high);
             unsigned high_byte, low_byte;
             mx8_split(r, 0.f, high, low, high_byte, low_byte);
-            uint8_t* dst = reinterpret_cast<uint8_t*>(a.out) + (size_t)(token0 + token + j) * a.ldo + feature;
+            const int row = t.x_row0 + token + j;
+            uint8_t* dst = reinterpret_cast<uint8_t*>(a.out) + (size_t)row * a.ldo + feature;
             dst[0] = (uint8_t)high_byte;
             dst[a.out_part] = (uint8_t)low_byte;
             if (lane == 0) {
-              uint8_t* scale = a.out_scales + mx4_scale_word(token0 + token + j, feature >> 7, (int)(a.ldo / 128)) + ((feature >> 5) & 3);
+              uint8_t* scale = a.out_scales + mx4_scale_word(row, feature >> 7, (int)(a.ldo / 128)) + quarter;
               scale[0] = (uint8_t)high;
               scale[a.os_part] = (uint8_t)low;
             }
           }
+        } else if (a.splits == 1) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (token + j < t.count && feature < a.features) {
+              const size_t at = (size_t)(t.out_row0 + token + j) * a.ldo + feature;
+              if (MODE == MXF_F32) reinterpret_cast<float*>(a.out)[at] = v[j] + bias;
+              else reinterpret_cast<__nv_bfloat16*>(a.out)[at] = __float2bfloat16_rn(v[j] + bias);
+            }
+        } else {
+          // (the products are done with the stages: the block has one tile)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) reinterpret_cast<float*>(smem)[(token + j) * 128 + in_tile] = v[j];
         }
       }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&acc_empty[b]));
     }
-  } else if (a.splits == 1) {
-    if (warp < 4 && ok) {
-      const int feature = feature0 + t;
-      for (int token = 0; token < count; token += 8) {
-        float v[8];
-        eight(token, v);
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (token + j < count && feature < a.features) store(token + j, feature, v[j]);
-      }
-    }
-  } else {
-    if (warp < 4 && ok) {
-      for (int token = 0; token < count; token += 8) {
-        float v[8];
-        eight(token, v);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) shared[(token + j) * 128 + t] = v[j];
-      }
-    }
+  }
+  if (a.splits > 1) {
+    __syncwarp();
     srb_cluster_sync();
-    if (warp < 4 && ok) {
-      const int feature = feature0 + t;
-      for (int token = rank; token < count; token += a.splits) {
-        float sum = 0.f;
-        for (int r = 0; r < a.splits; ++r) sum += srb_load_peer_shared(shared + token * 128 + t, r);
-        if (feature < a.features) store(token, feature, sum);
+    const FewTile t = few_tile<GROUPED>(a, first_item);
+    if (warp >= 2 && abort_flag == 0) {
+      // four features of a row a thread, from all blocks at once
+      for (int i = rank + a.splits * ((int)threadIdx.x - 64); i < t.count * 32; i += a.splits * MXF_EPILOGUE_THREADS) {
+        float4 part[MXF_MAX_SPLITS];
+#pragma unroll
+        for (int r = 0; r < MXF_MAX_SPLITS; ++r)
+          if (r < a.splits) part[r] = few_load_peer(reinterpret_cast<float*>(smem) + 4 * i, r);
+        float4 sum = part[0];
+#pragma unroll
+        for (int r = 1; r < MXF_MAX_SPLITS; ++r)
+          if (r < a.splits) sum = make_float4(sum.x + part[r].x, sum.y + part[r].y, sum.z + part[r].z, sum.w + part[r].w);
+        const float v[4] = {sum.x, sum.y, sum.z, sum.w};
+        const int feature = t.feature0 + 4 * (i & 31);
+        const size_t at = (size_t)(t.out_row0 + (i >> 5)) * a.ldo + feature;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (feature + j < a.features) {
+            const float r = v[j] + (a.bias ? a.bias[feature + j] : 0.f);
+            if (MODE == MXF_F32) reinterpret_cast<float*>(a.out)[at + j] = r;
+            else reinterpret_cast<__nv_bfloat16*>(a.out)[at + j] = __float2bfloat16_rn(r);
+          }
       }
     }
+    __syncwarp();
     srb_cluster_sync();                                      // nobody leaves while its sums may still be read
   }
   tc_fence_before();
   __syncthreads();
-  if (t == 0 && abort_flag) atomicOr(a.error_word, SRB_FLAG_WAIT_TIMEOUT);
-  if (warp == 4) {
+  if (threadIdx.x == 0 && abort_flag) atomicOr(a.error_word, SRB_FLAG_WAIT_TIMEOUT);
+  if (warp == 1) {
     tc_fence_after();
     tmem_dealloc(tmem, 256);
   }
 }
 
 template <bool FOUR, int MODE, bool GROUPED, int STAGES>
-static int launch_few_staged(const CUtensorMap& map_w, const FewArgs& a, int tiles_f, int tiles_t, cudaStream_t s) {
-  const size_t smem = 1024 + (size_t)STAGES * (MXF_A_BYTES + a.columns * 128 + 1024);
+static int launch_few_staged(const CUtensorMap (&maps)[4], const FewArgs& a, int blocks, cudaStream_t s) {
+  using Shape = FewShape<FOUR, MODE == MXF_GATED>;
+  const size_t smem = 1024 + (size_t)STAGES * (Shape::stage_bytes(a.columns) + Shape::SCALE_BYTES);
   auto kernel = mx4_few_kernel<FOUR, MODE, GROUPED, STAGES>;
   SRB_CUDA_CALL(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-  SRB_CUDA_CALL(srb_launch_clustered(kernel, dim3(tiles_f * a.splits, tiles_t), dim3(MXF_THREADS), smem, s, dim3(a.splits), map_w, a));
+  SRB_CUDA_CALL(srb_launch_clustered(kernel, dim3(blocks), dim3(MXF_THREADS), smem, s, dim3(a.splits), maps[0], maps[1], maps[2], maps[3], a));
   SRB_LAUNCH_CHECK("mx4_few");
   return SRB_OK;
 }
 
-// Two blocks an SM: stages for as much shared memory as that leaves.
+// x_rows, x_scale_tiles: of all parts.  Stages for as much shared memory as two blocks an SM leave.
 template <bool FOUR, int MODE, bool GROUPED>
-static int launch_few(const void* w, FewArgs& a, int tokens, int tiles_f, int tiles_t, cudaStream_t s) {
-  CUtensorMap map_w;
-  const long long w_rows = (long long)std::max(a.experts, 1) * a.w_rows;
-  if ((uintptr_t)w & 31) SRB_FAIL("mx4_few: codes must start on a 32-byte border");
-  if (w_rows > 0x7fffffff) SRB_FAIL("mx4_few: %lld rows of weights are too many", w_rows);
-  if (make_codes_map(&map_w, w, w_rows, a.k_tiles, MODE == MXF_GATED ? 64 : 128) != SRB_OK) return SRB_ERR_INVALID;
-  tokens = std::min(tokens, MXF_TOKENS);
-  a.columns = FOUR ? (tokens + 15) & ~15 : 2 * ((tokens + 7) & ~7);
-  if (tiles_t > 65535) SRB_FAIL("mx4_few: %d tiles of rows are too many", tiles_t);
-  return a.columns <= 32 ? launch_few_staged<FOUR, MODE, GROUPED, 5>(map_w, a, tiles_f, tiles_t, s)
-         : a.columns <= 64 ? launch_few_staged<FOUR, MODE, GROUPED, 4>(map_w, a, tiles_f, tiles_t, s)
-                           : launch_few_staged<FOUR, MODE, GROUPED, 3>(map_w, a, tiles_f, tiles_t, s);
-}
-
-// K in parts until there are about two blocks an SM, at least two steps each.
-static int few_splits(long long tiles, int k_tiles) {
-  const long long wanted = 2ll * srb_sm_count() / std::max(tiles, 1ll);
-  return (int)std::max(1ll, std::min(std::min(wanted, 8ll), (long long)k_tiles / 2));
+static int launch_few(const void* x, const void* x_scales, long long x_rows, long long x_scale_tiles, const void* w, const void* w_scales, FewArgs& a,
+                      cudaStream_t s) {
+  const long long matrices = std::max(a.experts, 1), w_rows = matrices * a.w_rows, ws_tiles = matrices * a.ws_tiles * a.k_tiles;
+  const long long items = (long long)a.tiles_t * a.tiles_f;
+  if (((uintptr_t)w | (uintptr_t)x) & 31) SRB_FAIL("mx4_few: codes and rows must start on a 32-byte border");
+  if (w_rows > 0x7fffffff || ws_tiles > 0x7fffffff || x_rows > 0x7fffffff || x_scale_tiles > 0x7fffffff || items > 0x3fffffff)
+    SRB_FAIL("mx4_few: %lld rows of weights and %lld of inputs are too many", w_rows, x_rows);
+  CUtensorMap maps[4];
+  if (make_codes_map(&maps[0], w, w_rows, a.k_tiles, 128) != SRB_OK || make_scales_map(&maps[1], w_scales, ws_tiles, 1) != SRB_OK ||
+      (FOUR ? make_codes_map(&maps[2], x, x_rows, a.k_tiles, a.columns) : make_bytes_map(&maps[2], x, x_rows, a.k_tiles * 128ll, a.columns)) != SRB_OK ||
+      make_scales_map(&maps[3], x_scales, x_scale_tiles, 1) != SRB_OK)
+    return SRB_ERR_INVALID;
+  // K in parts until there are about two blocks an SM, at least two steps each
+  const long long room = 2ll * srb_sm_count();
+  a.splits = GROUPED ? 1 : (int)std::max(1ll, std::min(std::min<long long>(room / items, MXF_MAX_SPLITS), (long long)a.k_tiles / 2));
+  const int blocks = (int)(a.splits > 1 ? items * a.splits : std::min(items, room));
+  if (MODE == MXF_GATED) return a.columns <= 16 ? launch_few_staged<FOUR, MODE, GROUPED, 3>(maps, a, blocks, s) : launch_few_staged<FOUR, MODE, GROUPED, 2>(maps, a, blocks, s);
+  return a.columns * (FOUR ? 1 : 2) <= 32 ? launch_few_staged<FOUR, MODE, GROUPED, 5>(maps, a, blocks, s)
+         : a.columns * (FOUR ? 1 : 2) <= 64 ? launch_few_staged<FOUR, MODE, GROUPED, 4>(maps, a, blocks, s)
+                                            : launch_few_staged<FOUR, MODE, GROUPED, 3>(maps, a, blocks, s);
 }
 
 // x: codes [rows, 64 k_tiles] with their scales (`four`), or parts [2, rows, 128 k_tiles] with theirs; w: codes [features, 64 k_tiles]; out
@@ -330,42 +361,48 @@ extern "C" int srb_mx4_linear(const void* x, const void* x_scales, int four, con
   if (rows <= 0 || features <= 0) return SRB_OK;
   if (width <= 0) SRB_FAIL("mx4_linear: inner size %d must be positive", width);
   FewArgs a = {};
-  a.x = (const uint8_t*)x; a.x_scales = (const uint8_t*)x_scales; a.w_scales = (const uint8_t*)w_scales; a.bias = bias;
-  a.out = out; a.ldo = ldo; a.rows = rows; a.features = a.w_rows = features; a.k_tiles = mx4_tiles(width); a.error_word = error_word;
-  a.x_part = (size_t)rows * a.k_tiles * 128; a.xs_part = (size_t)mx4_tiles(rows) * a.k_tiles * MX4_TILE_BYTES;
-  const int tiles_f = mx4_tiles(features), tiles_t = (rows + MXF_TOKENS - 1) / MXF_TOKENS;
-  a.splits = few_splits((long long)tiles_f * tiles_t, a.k_tiles);
+  a.bias = bias; a.out = out; a.ldo = ldo; a.rows = rows; a.features = a.w_rows = features; a.k_tiles = mx4_tiles(width); a.error_word = error_word;
+  a.x_lo_row = rows; a.xs_lo_tile = mx4_tiles(rows) * a.k_tiles; a.ws_tiles = a.tiles_f = mx4_tiles(features);
+  a.tiles_t = (rows + MXF_TOKENS - 1) / MXF_TOKENS;
+  a.columns = (std::min(rows, MXF_TOKENS) + 15) & ~15;
+  const long long parts = four ? 1 : 2, x_rows = parts * rows, xs_tiles = parts * a.xs_lo_tile;
   cudaStream_t s = (cudaStream_t)stream;
   if (four)
-    return out_float ? launch_few<true, MXF_F32, false>(w, a, rows, tiles_f, tiles_t, s) : launch_few<true, MXF_BF16, false>(w, a, rows, tiles_f, tiles_t, s);
-  return out_float ? launch_few<false, MXF_F32, false>(w, a, rows, tiles_f, tiles_t, s) : launch_few<false, MXF_BF16, false>(w, a, rows, tiles_f, tiles_t, s);
+    return out_float ? launch_few<true, MXF_F32, false>(x, x_scales, x_rows, xs_tiles, w, w_scales, a, s)
+                     : launch_few<true, MXF_BF16, false>(x, x_scales, x_rows, xs_tiles, w, w_scales, a, s);
+  return out_float ? launch_few<false, MXF_F32, false>(x, x_scales, x_rows, xs_tiles, w, w_scales, a, s)
+                   : launch_few<false, MXF_BF16, false>(x, x_scales, x_rows, xs_tiles, w, w_scales, a, s);
 }
 
-// The experts' products over the plan's tiles (of 64 slots).  x: parts [2, x_rows, 128 k_tiles] and their scales; rows by `slot_row`, or the
-// slots themselves (null).  Mode gated / act: out parts [2, slots, 128 ceil(features / 128)], out_scales theirs; float: out [slots, features].
-extern "C" int srb_mx4_experts(const void* x, const void* x_scales, int x_rows, const int* slot_row, const void* w, const void* w_scales,
-                               void* out, void* out_scales, const int* plan, int max_tiles, int slots, int experts, int features, int width,
-                               int mode, int activation, float act_param, int* error_word, void* stream) {
+// The experts' products over the plan's tiles of `tile_slots` (32 at most) slots.  x: parts [2, 64 max_tiles, 128 k_tiles] and their scales, 64 rows a
+// tile.  Mode gated / act: out parts [2, 64 max_tiles, 128 ceil(features / 128)], out_scales theirs; float: out [slots, features].  The
+// gated mode: `up_scale_row` is the row of w_scales' tiles where the up rows begin, a multiple of 128; `scale_rows` the rows that they hold a matrix.
+extern "C" int srb_mx4_experts(const void* x, const void* x_scales, const void* w, const void* w_scales, int scale_rows, int up_scale_row, void* out,
+                               void* out_scales, const int* plan, int tile_slots, int max_tiles, int experts, int features, int width, int mode,
+                               int activation, float act_param, int* error_word, void* stream) {
   if (max_tiles <= 0 || features <= 0) return SRB_OK;
   if (width <= 0) SRB_FAIL("mx4_experts: inner size %d must be positive", width);
+  if (tile_slots != 16 && tile_slots != MXF_SLOTS) SRB_FAIL("mx4_experts: tiles of %d slots are not 16 or %d", tile_slots, MXF_SLOTS);
   if (activation < 0 || activation >= SRB_ACT_COUNT) SRB_FAIL("mx4_experts: unknown activation %d", activation);
   if (mode != MXF_F32 && mode != MXF_GATED && mode != MXF_ACT) SRB_FAIL("mx4_experts: mode %d is not float, gated or activated", mode);
+  if (mode == MXF_GATED && up_scale_row % 128) SRB_FAIL("mx4_experts: scales of up rows begin at row %d, no multiple of 128", up_scale_row);
   FewArgs a = {};
-  a.x = (const uint8_t*)x; a.x_scales = (const uint8_t*)x_scales; a.w_scales = (const uint8_t*)w_scales; a.out = out;
-  a.out_scales = (uint8_t*)out_scales; a.rows = slots; a.features = features; a.w_rows = mode == MXF_GATED ? 2 * features : features;
+  a.out = out; a.out_scales = (uint8_t*)out_scales; a.features = features; a.w_rows = mode == MXF_GATED ? 2 * features : features;
   a.k_tiles = mx4_tiles(width); a.activation = activation; a.act_param = act_param; a.error_word = error_word;
-  a.x_part = (size_t)x_rows * a.k_tiles * 128; a.xs_part = (size_t)mx4_tiles(x_rows) * a.k_tiles * MX4_TILE_BYTES;
-  a.plan = plan; a.slot_row = slot_row; a.experts = experts; a.splits = 1;
+  a.ws_tiles = mx4_tiles(scale_rows); a.up_tile = up_scale_row >> 7;
+  a.plan = plan; a.experts = experts; a.tile_slots = a.columns = tile_slots;
+  a.tiles_f = mx4_tiles(features); a.tiles_t = max_tiles;
+  const long long rows = (long long)MXF_ROOM * max_tiles, tiles = (rows + 127) / 128;
+  a.x_lo_row = (int)rows; a.xs_lo_tile = (int)tiles * a.k_tiles;
   cudaStream_t s = (cudaStream_t)stream;
-  const int out_tiles = mx4_tiles(features);
   if (mode == MXF_F32) {
     a.ldo = features;
-    return launch_few<false, MXF_F32, true>(w, a, slots, out_tiles, max_tiles, s);
+    return launch_few<false, MXF_F32, true>(x, x_scales, 2 * rows, 2 * tiles * a.k_tiles, w, w_scales, a, s);
   }
-  a.ldo = (size_t)out_tiles * 128;
-  a.out_part = (size_t)slots * a.ldo; a.os_part = (size_t)mx4_tiles(slots) * out_tiles * MX4_TILE_BYTES;
-  if (mode == MXF_GATED) return launch_few<false, MXF_GATED, true>(w, a, slots, 2 * out_tiles, max_tiles, s);
-  return launch_few<false, MXF_ACT, true>(w, a, slots, out_tiles, max_tiles, s);
+  a.ldo = (size_t)a.tiles_f * 128;
+  a.out_part = (size_t)rows * a.ldo; a.os_part = (size_t)tiles * a.tiles_f * MX4_TILE_BYTES;
+  if (mode == MXF_GATED) return launch_few<false, MXF_GATED, true>(x, x_scales, 2 * rows, 2 * tiles * a.k_tiles, w, w_scales, a, s);
+  return launch_few<false, MXF_ACT, true>(x, x_scales, 2 * rows, 2 * tiles * a.k_tiles, w, w_scales, a, s);
 }
 
 // out[row, :] = sum over the row's choices, in their order, of weight * y[slot, :], in 32 bits, rounded once.

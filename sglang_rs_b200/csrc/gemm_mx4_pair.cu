@@ -11,11 +11,11 @@
 // go from shared to tensor memory ahead of a step's products, in the same queue; steps use places in turn.
 //
 // Over experts (GROUPED) a tile is up to 256 slots of one expert (the plan of csrc/moe.cu); X and the parts that the gated mode leaves have room
-// for 256 rows a tile, so that a tile's scales are whole tiles.  Gated: the even CTA brings gate rows, the odd one the up rows of the same 96 features;
-// their scales are no whole tiles, and four warps bring them by cp.async, a word a row.
+// for 256 rows a tile, so that a tile's scales are whole tiles.  Gated: the even CTA brings gate rows, the odd one the up rows of the same 96 features,
+// whose scales come regrouped (srb_mx4_gated_scales: 96 and 96 rows are no whole tiles; a word a row by cp.async instead kept the tensor cores
+// waiting, 296 us instead of LATER for the gate/up of 12,288 slots, 64 experts of 2,048 x 1,408).
 //
-// Warps: 0 TMA, 1 products (even CTA) and tensor memory, then four for W's scales in the gated mode, then twelve of the epilogue: a quarter of the lanes
-// and a third of the columns each.  Waits are bounded; one that runs out flags SRB_FLAG_WAIT_TIMEOUT.
+// Warps: 0 TMA, 1 products (even CTA) and tensor memory, 2-13 epilogue: a quarter of the lanes and a third of the columns each.  Waits are bounded; one that runs out flags SRB_FLAG_WAIT_TIMEOUT.
 #include "common.cuh"
 #include "activations.cuh"
 #include "mx4.cuh"
@@ -39,22 +39,20 @@ SRB_DEFINE_PDL_SWITCH()
 #define MXP_GATED 2
 #define MXP_ACT 5
 
-template <bool FOUR, bool GATED> struct PairShape {
+template <bool FOUR> struct PairShape {
   static constexpr int STAGES = FOUR ? 6 : 4;
   static constexpr int PARTS = FOUR ? 1 : 2;
   static constexpr int B_AT = PARTS * MXP_A_BYTES;
   static constexpr int XS_AT = B_AT + MXP_B_BYTES;           // scales of X: two column tiles, or a tile of each part
   static constexpr int WS_AT = XS_AT + 1024;                 // of W: two row tiles of each column tile, or 192 rows in order
   static constexpr int STAGE_BYTES = WS_AT + (FOUR ? 2048 : 1024);
-  static constexpr int TMA_BYTES = FOUR ? STAGE_BYTES : 2 * MXP_A_BYTES + MXP_B_BYTES / 2 + (GATED ? 1024 : 2048);    // a CTA's by TMA
-  static constexpr int COPY_WARPS = GATED ? 4 : 0;
-  static constexpr int THREADS = 32 * (2 + COPY_WARPS + MXP_EPILOGUE_WARPS);
+  static constexpr int TMA_BYTES = FOUR ? STAGE_BYTES : 2 * MXP_A_BYTES + MXP_B_BYTES / 2 + 2048;    // what the barrier counts: codes without the gaps
+  static constexpr int THREADS = 32 * (2 + MXP_EPILOGUE_WARPS);
   static constexpr int PLACE_COLUMNS = FOUR ? 24 : 16;       // of scales of a step
   static constexpr int PLACES = FOUR ? 5 : 4;
 };
 
 struct PairMx4Args {
-  const uint8_t* w_scales;
   const float* bias;
   void* out;
   uint8_t* out_scales;           // of parts
@@ -62,6 +60,7 @@ struct PairMx4Args {
   size_t out_part, os_part;
   int rows, features, w_rows, k_tiles;
   int x_lo_row, xs_lo_tile;      // where the second part's rows and tiles of scales begin
+  int ws_tiles;                  // row tiles of scales of a matrix
   int tiles_t, tiles_f;
   int activation;
   float act_param;
@@ -70,9 +69,6 @@ struct PairMx4Args {
   int experts;
 };
 
-__device__ __forceinline__ void cp_async_4(unsigned dst, const void* src, int bytes) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;\n" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
 __device__ __forceinline__ void pair_tmem_alloc(unsigned holder) {
   asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(holder), "r"(512) : "memory");
   asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
@@ -140,15 +136,15 @@ __device__ __forceinline__ PairMx4Tile pair_mx4_tile(const PairMx4Args& a, int t
 }
 
 template <bool FOUR, int MODE, bool GROUPED>
-__global__ void __launch_bounds__(PairShape<FOUR, MODE == MXP_GATED>::THREADS, 1)
+__global__ void __launch_bounds__(PairShape<FOUR>::THREADS, 1)
 mx4_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_xs, const __grid_constant__ CUtensorMap map_w,
                 const __grid_constant__ CUtensorMap map_ws, const __grid_constant__ CUtensorMap map_out, const PairMx4Args a) {
-  using Shape = PairShape<FOUR, MODE == MXP_GATED>;
+  using Shape = PairShape<FOUR>;
   constexpr int STAGES = Shape::STAGES;
   constexpr bool GATED = MODE == MXP_GATED, PARTS = MODE == MXP_GATED || MODE == MXP_ACT;
   extern __shared__ unsigned char smem_unaligned[];
   unsigned char* smem = reinterpret_cast<unsigned char*>(((uintptr_t)smem_unaligned + 1023) & ~(uintptr_t)1023);
-  __shared__ __align__(8) unsigned long long full_bar[STAGES], empty_bar[STAGES], copied_bar[STAGES], acc_full[2], acc_empty[2];
+  __shared__ __align__(8) unsigned long long full_bar[STAGES], empty_bar[STAGES], acc_full[2], acc_empty[2];
   __shared__ unsigned tmem_holder;
   __shared__ int abort_flag;
 
@@ -160,8 +156,7 @@ mx4_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
   if (threadIdx.x == 0) {
     abort_flag = 0;
     for (int s = 0; s < STAGES; ++s) {
-      mbar_init(smem_u32(&full_bar[s]), GATED ? 2 : 1);      // the even CTA's: its bytes by TMA, and the word that the odd CTA's copies are there
-      mbar_init(smem_u32(&copied_bar[s]), 128);
+      mbar_init(smem_u32(&full_bar[s]), 1);
       mbar_init(smem_u32(&empty_bar[s]), 1);
     }
     for (int b = 0; b < 2; ++b) {
@@ -188,7 +183,8 @@ mx4_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
       const PairMx4Tile t = pair_mx4_tile<MODE, GROUPED>(a, tile);
       const int x_row = t.x_row0 + (int)rank * MXP_ROWS, xs_tile = (x_row >> 7) * a.k_tiles;
       const int w_row = t.matrix * a.w_rows + t.feature0 + (int)rank * (GATED ? a.features : MXP_HALF);
-      const int ws_tile = (t.matrix * mx4_tiles(a.w_rows) + (t.feature0 >> 7)) * a.k_tiles;
+      // (the gated mode's scales are in groups of 96 gate and 96 up rows, two tiles each)
+      const int ws_tile = (t.matrix * a.ws_tiles + (GATED ? t.feature0 / MXP_HALF * 2 : t.feature0 >> 7)) * a.k_tiles;
       for (int i = 0; i < steps && ok; ++i, ++round) {
         const int s = (int)(round % STAGES);
         ok = mbar_wait_warp(smem_u32(&empty_bar[s]), ((round / STAGES) & 1u) ^ 1u, &abort_flag);
@@ -207,10 +203,8 @@ mx4_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
             pair_tma_load(stage + Shape::XS_AT, &map_xs, bar, 0, xs_tile + i);
             pair_tma_load(stage + Shape::B_AT, &map_w, bar, i * 128, w_row);
             pair_tma_load(stage + Shape::XS_AT + 512, &map_xs, bar, 0, a.xs_lo_tile + xs_tile + i);
-            if (!GATED) {
-              pair_tma_load(stage + Shape::WS_AT, &map_ws, bar, 0, ws_tile + i);
-              pair_tma_load(stage + Shape::WS_AT + 512, &map_ws, bar, 0, ws_tile + a.k_tiles + i);
-            }
+            pair_tma_load(stage + Shape::WS_AT, &map_ws, bar, 0, ws_tile + i);
+            pair_tma_load(stage + Shape::WS_AT + 512, &map_ws, bar, 0, ws_tile + a.k_tiles + i);
           }
         }
         ++issued;
@@ -239,9 +233,7 @@ mx4_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
         for (int i = 0; i < steps && ok; ++i, ++round) {
           const int s = (int)(round % STAGES);
           ok = mbar_wait_warp_cluster(smem_u32(&full_bar[s]), (round / STAGES) & 1u, &abort_flag);
-          if (GATED && ok) ok = mbar_wait_warp(smem_u32(&copied_bar[s]), (round / STAGES) & 1u, &abort_flag);
           if (!ok) break;
-          if (GATED) fence_proxy_async_shared();
           tc_fence_after();
           const unsigned stage = smem_u32(smem) + s * Shape::STAGE_BYTES;
           const unsigned place = tmem + MXP_SUMS + (round % Shape::PLACES) * Shape::PLACE_COLUMNS;
@@ -276,54 +268,12 @@ mx4_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
           __syncwarp();
         }
       }
-    } else if (GATED) {
-      // ---- the odd CTA's copies: said to the even one when they are there
-      unsigned round = 0;
-      bool ok = true;
-      for (int tile = pair; tile < num_tiles && ok; tile += num_pairs)
-        for (int i = 0; i < steps && ok; ++i, ++round) {
-          const int s = (int)(round % STAGES);
-          ok = mbar_wait_warp(smem_u32(&copied_bar[s]), (round / STAGES) & 1u, &abort_flag);
-          if (!ok) break;
-          fence_proxy_async_shared();
-          if (lane == 0) arrive_at(smem_u32(&full_bar[s]), 0);
-          __syncwarp();
-        }
     }
-  } else if (warp < 2 + Shape::COPY_WARPS) {
-    // ---- the scales of all 192 rows of W, gate and up: of row t, and 128 + t
-    const int t = threadIdx.x - 64;
-    unsigned round = 0;
-    bool ok = true;
-    for (int tile = pair; tile < num_tiles && ok; tile += num_pairs) {
-      const PairMx4Tile tl = pair_mx4_tile<MODE, GROUPED>(a, tile);
-      const uint8_t* w_scales = a.w_scales + (size_t)tl.matrix * mx4_tiles(a.w_rows) * a.k_tiles * MX4_TILE_BYTES;
-      // row n of the N side
-      auto w_row = [&](int n, bool& live) {
-        const int feature = tl.feature0 + (n >= MXP_HALF ? n - MXP_HALF : n);
-        live = feature < a.features;
-        return !live ? 0 : n >= MXP_HALF ? a.features + feature : feature;
-      };
-      bool first_live, second_live;
-      const size_t first_word = mx4_scale_word(w_row(t, first_live), 0, a.k_tiles);
-      const size_t second_word = mx4_scale_word(w_row(128 + (t & 63), second_live), 0, a.k_tiles);
-      for (int i = 0; i < steps; ++i, ++round) {
-        const int s = (int)(round % STAGES);
-        ok = mbar_wait_warp(smem_u32(&empty_bar[s]), ((round / STAGES) & 1u) ^ 1u, &abort_flag);
-        if (!ok) break;
-        const unsigned stage = smem_u32(smem) + s * Shape::STAGE_BYTES;
-        const unsigned word = stage + Shape::WS_AT + lane * 16 + ((t >> 5) << 2);
-        cp_async_4(word, w_scales + first_word + (size_t)i * MX4_TILE_BYTES, first_live ? 4 : 0);
-        if (t < 64) cp_async_4(word + 512, w_scales + second_word + (size_t)i * MX4_TILE_BYTES, second_live ? 4 : 0);
-        copies_arrive(smem_u32(&copied_bar[s]));
-      }
-    }
-    asm volatile("cp.async.wait_all;" ::: "memory");
   } else {
     // ---- epilogue: warp w has lanes 32 * (w % 4) .. + 31 of its CTA's tensor memory, a row of X a lane, and a third of the columns
-    const int quarter = warp & 3, third = (warp - 2 - Shape::COPY_WARPS) >> 2;
+    const int quarter = warp & 3, third = (warp - 2) >> 2;
     const unsigned lane_address = tmem + ((unsigned)(quarter * 32) << 16);
-    const unsigned box = smem_u32(smem) + STAGES * Shape::STAGE_BYTES + (warp - 2 - Shape::COPY_WARPS) * MXP_BOX_BYTES;
+    const unsigned box = smem_u32(smem) + STAGES * Shape::STAGE_BYTES + (warp - 2) * MXP_BOX_BYTES;
     int local = 0;
     for (int tile = pair; tile < num_tiles; tile += num_pairs, ++local) {
       const int b = local & 1;
@@ -445,7 +395,7 @@ mx4_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
 // ------------------------------------------------------------------------------- host side
 template <bool FOUR, int MODE, bool GROUPED>
 static int launch_pair(const CUtensorMap (&maps)[5], const PairMx4Args& a, int max_tiles, cudaStream_t s) {
-  using Shape = PairShape<FOUR, MODE == MXP_GATED>;
+  using Shape = PairShape<FOUR>;
   const int pairs = std::max(1, std::min(srb_sm_count() / 2, max_tiles));
   const size_t smem = (size_t)Shape::STAGES * Shape::STAGE_BYTES + MXP_EPILOGUE_WARPS * MXP_BOX_BYTES + 1024;
   auto kernel = mx4_pair_kernel<FOUR, MODE, GROUPED>;
@@ -463,10 +413,11 @@ extern "C" int srb_mx4_linear_pair(const void* x, const void* x_scales, int four
   if ((uintptr_t)w & 31) SRB_FAIL("mx4_linear_pair: codes must start on a 32-byte border");
   if (((uintptr_t)out & 15) || ldo * (out_float ? 4 : 2) % 16) SRB_FAIL("mx4_linear_pair: rows of the result must start on 16-byte borders");
   PairMx4Args a = {};
-  a.w_scales = (const uint8_t*)w_scales; a.bias = bias; a.out = out; a.ldo = ldo; a.rows = rows;
+  a.bias = bias; a.out = out; a.ldo = ldo; a.rows = rows;
   a.features = a.w_rows = features; a.k_tiles = mx4_tiles(width); a.error_word = error_word;
   a.x_lo_row = rows; a.xs_lo_tile = mx4_tiles(rows) * a.k_tiles;
   a.tiles_t = (rows + MXP_TILE - 1) / MXP_TILE; a.tiles_f = (features + MXP_N - 1) / MXP_N;
+  a.ws_tiles = mx4_tiles(features);
   const long long row_tiles = mx4_tiles(rows), tiles = (long long)a.tiles_t * a.tiles_f;
   if (tiles > 0x3fffffff || 2ll * row_tiles * 128 > 0x7fffffff) SRB_FAIL("mx4_linear_pair: %d rows x %d features are too many", rows, features);
   CUtensorMap maps[5];
@@ -483,7 +434,8 @@ extern "C" int srb_mx4_linear_pair(const void* x, const void* x_scales, int four
 }
 
 // The experts' products over the plan's tiles of 256 slots.  x: parts [2, 256 max_tiles, 128 k_tiles] and their scales, 256 rows a tile.  Mode gated /
-// act: out parts [2, 256 max_tiles, 128 ceil(features / 128)], out_scales theirs; float: out [slots, features], rows on 16-byte borders.
+// act: out parts [2, 256 max_tiles, 128 ceil(features / 128)], out_scales theirs; float: out [slots, features], rows on 16-byte borders.  The gated
+// mode's w_scales are those of srb_mx4_gated_scales, groups of 96 in the room of 256.
 extern "C" int srb_mx4_experts_pair(const void* x, const void* x_scales, const void* w, const void* w_scales, void* out, void* out_scales,
                                     const int* plan, int max_tiles, int slots, int experts, int features, int width, int mode, int activation,
                                     float act_param, int* error_word, void* stream) {
@@ -493,7 +445,7 @@ extern "C" int srb_mx4_experts_pair(const void* x, const void* x_scales, const v
   if (activation < 0 || activation >= SRB_ACT_COUNT) SRB_FAIL("mx4_experts_pair: unknown activation %d", activation);
   if (mode != MXP_F32 && mode != MXP_GATED && mode != MXP_ACT) SRB_FAIL("mx4_experts_pair: mode %d is not float, gated or activated", mode);
   PairMx4Args a = {};
-  a.w_scales = (const uint8_t*)w_scales; a.out = out; a.out_scales = (uint8_t*)out_scales; a.rows = slots;
+  a.out = out; a.out_scales = (uint8_t*)out_scales; a.rows = slots;
   a.features = features; a.w_rows = mode == MXP_GATED ? 2 * features : features; a.k_tiles = mx4_tiles(width); a.activation = activation;
   a.act_param = act_param; a.error_word = error_word; a.plan = plan; a.experts = experts;
   const long long rows = 256ll * max_tiles;
@@ -501,15 +453,16 @@ extern "C" int srb_mx4_experts_pair(const void* x, const void* x_scales, const v
   a.x_lo_row = (int)rows; a.xs_lo_tile = 2 * max_tiles * a.k_tiles;
   const int covered = mode == MXP_F32 ? features : 128 * out_tiles, per_tile = mode == MXP_GATED ? MXP_HALF : MXP_N;
   a.tiles_f = (covered + per_tile - 1) / per_tile;
+  a.ws_tiles = mode == MXP_GATED ? 2 * a.tiles_f : mx4_tiles(features);
   a.ldo = mode == MXP_F32 ? features : 128 * out_tiles;
   a.out_part = (size_t)rows * a.ldo; a.os_part = (size_t)2 * max_tiles * out_tiles * MX4_TILE_BYTES;
-  if (2 * rows > 0x7fffffff || (long long)experts * a.w_rows > 0x7fffffff || (long long)experts * mx4_tiles(a.w_rows) * a.k_tiles > 0x7fffffff || (long long)max_tiles * a.tiles_f > 0x3fffffff) SRB_FAIL("mx4_experts_pair: %d tiles are too many", max_tiles);
+  if (2 * rows > 0x7fffffff || (long long)experts * a.w_rows > 0x7fffffff || (long long)experts * a.ws_tiles * a.k_tiles > 0x7fffffff || (long long)max_tiles * a.tiles_f > 0x3fffffff) SRB_FAIL("mx4_experts_pair: %d tiles are too many", max_tiles);
   if (mode == MXP_F32 && (((uintptr_t)out & 15) || features % 4)) SRB_FAIL("mx4_experts_pair: rows of the result must start on 16-byte borders");
   CUtensorMap maps[5];
   if (make_bytes_map(&maps[0], x, 2 * rows, a.k_tiles * 128, MXP_ROWS) != SRB_OK ||
       make_scales_map(&maps[1], x_scales, 4ll * max_tiles * a.k_tiles, 1) != SRB_OK ||
       make_codes_map(&maps[2], w, (long long)experts * a.w_rows, a.k_tiles, MXP_HALF) != SRB_OK ||
-      make_scales_map(&maps[3], w_scales, (long long)experts * mx4_tiles(a.w_rows) * a.k_tiles, 1) != SRB_OK)
+      make_scales_map(&maps[3], w_scales, (long long)experts * a.ws_tiles * a.k_tiles, 1) != SRB_OK)
     return SRB_ERR_INVALID;
   maps[4] = maps[0];
   if (mode == MXP_F32 && make_map(&maps[4], CU_TENSOR_MAP_DATA_TYPE_FLOAT32, out, slots, features, features * 4ll, 32, 16, CU_TENSOR_MAP_SWIZZLE_64B) != SRB_OK)

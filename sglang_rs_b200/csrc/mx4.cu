@@ -180,28 +180,51 @@ mx4_split_kernel(const __nv_bfloat16* __restrict__ x, size_t pitch, int rows, in
                         (size_t)mx4_tiles(rows) * k_tiles * MX4_TILE_BYTES);
 }
 
-// The same in the order of a plan's tiles (csrc/moe.cu) of 256 slots, with room for 256 rows a tile: parts [2, 256 tiles, ...].  16 lanes a
-// slot, 16 slots a block.
+// The same in the order of a plan's tiles (csrc/moe.cu), with `room` rows a tile: parts [2, room * tiles, ...].  16 lanes a slot, 16 slots
+// a block.
 template <bool WIDE>
 __global__ void __launch_bounds__(MX4_THREADS)
 mx4_split_slots_kernel(const __nv_bfloat16* __restrict__ x, int width, const int* __restrict__ plan, const int* __restrict__ slot_row, int experts,
-                       int max_tiles, uint8_t* __restrict__ parts, uint8_t* __restrict__ scales) {
+                       int tile_slots, int room, int max_tiles, uint8_t* __restrict__ parts, uint8_t* __restrict__ scales) {
   srb_launch_dependents();
   srb_grid_dependency_wait();
   const int tile = blockIdx.y, in_tile = blockIdx.x * (MX4_THREADS / 16) + (threadIdx.x >> 4), lane = threadIdx.x & 15;
   if (tile >= plan[0]) return;
   const int expert = plan[1 + experts + 1 + 2 * tile], slot = plan[1 + experts + 1 + 2 * tile + 1] + in_tile;
-  const int end = plan[1 + expert + 1];
+  const int end = min(plan[1 + expert + 1], slot - in_tile + tile_slots);
   if (slot - (in_tile & 1) >= end) return;                   // neither half of the warp has a slot
   const bool live = slot < end;
-  const int k_tiles = mx4_tiles(width), row = tile * 256 + in_tile;
-  const size_t part = (size_t)max_tiles * 256 * k_tiles * 128, scale_part = (size_t)max_tiles * 2 * k_tiles * MX4_TILE_BYTES;
+  const int k_tiles = mx4_tiles(width), row = tile * room + in_tile;
+  const size_t part = (size_t)max_tiles * room * k_tiles * 128, scale_part = (size_t)mx4_tiles(max_tiles * room) * k_tiles * MX4_TILE_BYTES;
   const __nv_bfloat16* src = x + (size_t)(live ? slot_row[slot] : 0) * width + lane * 8;
   uint8_t* dst = parts + ((size_t)row * k_tiles * 128 + lane * 8);
 #pragma unroll 4
   for (int kt = 0; kt < k_tiles; ++kt)
     mx4_split_eight<WIDE>(src + kt * 128, width - kt * 128 - lane * 8, live, lane, dst + kt * 128, part, scales + mx4_scale_word(row, kt, k_tiles),
                           scale_part);
+}
+
+// Scales of stacked gate and up rows (2 * inner rows a matrix) in groups: `group` gate rows, the `group` up rows of the same features, room for
+// `room` rows (a multiple of 128) a group.  A product tile's scales are whole tiles then, wherever the up rows begin.  Matrices without a slot in
+// the plan are left out.  A thread has the 16 bytes of four rows, 32 apart.
+__global__ void __launch_bounds__(MX4_THREADS)
+mx4_gated_scales_kernel(const unsigned* __restrict__ scales, int inner, int group, int room, int groups, int k_tiles, const int* __restrict__ plan,
+                        uint4* __restrict__ out) {
+  srb_launch_dependents();
+  srb_grid_dependency_wait();
+  const int matrix = blockIdx.y;
+  if (plan[1 + matrix] == plan[1 + matrix + 1]) return;
+  const int tiles = groups * (room / 128), item = blockIdx.x * MX4_THREADS + threadIdx.x;
+  if (item >= tiles * k_tiles * 32) return;
+  const int kt = item / 32 % k_tiles, tile = item / 32 / k_tiles;
+  const size_t from = (size_t)matrix * mx4_tiles(2 * inner) * k_tiles * MX4_TILE_BYTES;
+  unsigned w[4];
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const int row = tile * 128 + q * 32 + (item & 31), n = row % room, feature = row / room * group + (n < group ? n : n - group);
+    w[q] = n < 2 * group && feature < inner ? scales[(from + mx4_scale_word(n < group ? feature : inner + feature, kt, k_tiles)) / 4] : 0x7f7f7f7fu;
+  }
+  out[((size_t)(matrix * tiles + tile) * k_tiles + kt) * (MX4_TILE_BYTES / 16) + (item & 31)] = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
 static int mx4_grid(int matrices, long long rows, int width, dim3* grid) {
@@ -262,14 +285,27 @@ extern "C" int srb_mx4_split(const void* x, long long pitch, int rows, int width
   return SRB_OK;
 }
 
-extern "C" int srb_mx4_split_slots(const void* x, int width, const int* plan, const int* slot_row, int experts, int max_tiles, void* parts,
-                                   void* scales, void* stream) {
+extern "C" int srb_mx4_split_slots(const void* x, int width, const int* plan, const int* slot_row, int experts, int tile_slots,
+                                   int room, int max_tiles, void* parts, void* scales, void* stream) {
   if (max_tiles <= 0 || width <= 0) return SRB_OK;
-  if (max_tiles > 65535) SRB_FAIL("mx4_split_slots: %d tiles are too many", max_tiles);
+  if (max_tiles > 65535 || (long long)max_tiles * room > 0x3fffffff) SRB_FAIL("mx4_split_slots: %d tiles are too many", max_tiles);
+  if (tile_slots > room || room % 16) SRB_FAIL("mx4_split_slots: %d slots in the room of %d", tile_slots, room);
   const bool wide = ((uintptr_t)x & 15) == 0 && width % 8 == 0;
-  SRB_CUDA_CALL(srb_launch(wide ? mx4_split_slots_kernel<true> : mx4_split_slots_kernel<false>, dim3(256 / (MX4_THREADS / 16), max_tiles),
-                           dim3(MX4_THREADS), 0, (cudaStream_t)stream, (const __nv_bfloat16*)x, width, plan, slot_row, experts, max_tiles,
-                           (uint8_t*)parts, (uint8_t*)scales));
+  SRB_CUDA_CALL(srb_launch(wide ? mx4_split_slots_kernel<true> : mx4_split_slots_kernel<false>, dim3((tile_slots + 15) / 16, max_tiles),
+                           dim3(MX4_THREADS), 0, (cudaStream_t)stream, (const __nv_bfloat16*)x, width, plan, slot_row, experts, tile_slots, room,
+                           max_tiles, (uint8_t*)parts, (uint8_t*)scales));
   SRB_LAUNCH_CHECK("mx4_split_slots");
+  return SRB_OK;
+}
+
+extern "C" int srb_mx4_gated_scales(const void* scales, int matrices, int inner, int width, int group, int room, int groups, const int* plan,
+                                    void* out, void* stream) {
+  if (matrices <= 0 || inner <= 0 || width <= 0) return SRB_OK;
+  const long long items = (long long)groups * (room / 128) * mx4_tiles(width) * 32;
+  if (group <= 0 || room % 128 || room < 2 * group || matrices > 65535 || items > 0x3fffffff)
+    SRB_FAIL("mx4_gated_scales: %d matrices, groups of %d in the room of %d", matrices, group, room);
+  SRB_CUDA_CALL(srb_launch(mx4_gated_scales_kernel, dim3((unsigned)((items + MX4_THREADS - 1) / MX4_THREADS), matrices), dim3(MX4_THREADS), 0,
+                           (cudaStream_t)stream, (const unsigned*)scales, inner, group, room, groups, mx4_tiles(width), plan, (uint4*)out));
+  SRB_LAUNCH_CHECK("mx4_gated_scales");
   return SRB_OK;
 }

@@ -12,13 +12,6 @@
 #define MX_E4M3 0u
 #define MX_E2M1 5u       // among the types of kind mxf8f6f4
 
-// Arrives on the barrier once this thread's cp.async copies so far have landed; the arrival is one of the barrier's count.  The copies are
-// ordinary writes to the tensor cores: whoever waits on the barrier puts fence.proxy.async ahead of the products.  (A fence by the copying
-// threads waits for all of their copies in flight: 30 us for 50 MB of codes at 4 steps of five in flight, a step each 0.9 us.)
-__device__ __forceinline__ void copies_arrive(unsigned bar) {
-  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
-}
-
 // kind mxf8f6f4: scales of 2^n, both operands K-major, M = 128.  The scale byte `k` of a word is ORed in by mx_idesc_step.
 __device__ __forceinline__ unsigned mx_idesc(unsigned a_type, unsigned b_type, int m, int n) {
   return (a_type << 7) | (b_type << 10) | ((unsigned)(n >> 3) << 17) | (1u << 23) | ((unsigned)(m >> 4) << 24);

@@ -254,8 +254,9 @@ def chosen_experts_mx4(h: torch.Tensor, chosen: torch.Tensor, weights: torch.Ten
     device, entries, stream = h.device, rows * top, _stream()
     # (the pairs' result rows start on 16-byte borders)
     many = entries > MX4_FEW_CHOICES * experts and width % 4 == 0
-    tile = 256 if many else 64
-    moe, lib = load_library("moe"), load_library("gemm_mx4")
+    # slots of a tile, and the rows of its inputs that there is room for
+    tile, room = (256, 256) if many else (32 if entries > 4 * experts else 16, 64)
+    moe, lib, split = load_library("moe"), load_library("gemm_mx4"), load_library("mx4")
     plan = torch.empty(moe.srb_moe_plan_ints_of(rows, top, experts, tile), dtype=torch.int32, device=device)
     slot_row = torch.empty(entries, dtype=torch.int32, device=device)
     entry_slot = torch.empty(entries, dtype=torch.int32, device=device)
@@ -264,26 +265,36 @@ def chosen_experts_mx4(h: torch.Tensor, chosen: torch.Tensor, weights: torch.Ten
                                     _ptr(error_word), stream))
     # a tile has a slot at least
     tiles = min(entries, moe.srb_moe_max_tiles_of(rows, top, experts, tile))
-    act_rows = 256 * tiles if many else entries
-    act = torch.empty((2, act_rows, 128 * _tiles(inner)), dtype=torch.uint8, device=device)
-    act_scales = torch.empty((2, _tiles(act_rows), _tiles(inner), 512), dtype=torch.uint8, device=device)
+
+    def held(entries_of_a_row):
+        """Room for both parts of every tile's rows, and for their scales."""
+        return (torch.empty((2, room * tiles, 128 * _tiles(entries_of_a_row)), dtype=torch.uint8, device=device),
+                torch.empty((2, _tiles(room * tiles), _tiles(entries_of_a_row), 512), dtype=torch.uint8, device=device))
+    (parts, scales), (act, act_scales) = held(width), held(inner)
+    _check(split, split.srb_mx4_split_slots(_ptr(h), width, _ptr(plan), _ptr(slot_row), experts, tile, room, tiles, _ptr(parts), _ptr(scales),
+                                            stream))
+    up_scales, scale_rows, up_row = w_gate_up.scales, w_gate_up.rows, inner
+    if gated and (many or inner % 128):
+        # a tile's gate and up rows side by side: 96 of each for the pairs; otherwise all of them, the up rows on the border of a tile
+        group = 96 if many else 128 * _tiles(inner)
+        group_room, groups = (256, -(-128 * _tiles(inner) // 96)) if many else (2 * group, 1)
+        scale_rows, up_row = groups * group_room, group
+        up_scales = torch.empty((experts, scale_rows // 128, _tiles(width), 512), dtype=torch.uint8, device=device)
+        _check(split, split.srb_mx4_gated_scales(_ptr(w_gate_up.scales), experts, inner, width, group, group_room, groups, _ptr(plan),
+                                                 _ptr(up_scales), stream))
     mode, param = GEMM_MODES["gated" if gated else "act"], ctypes.c_float(activation_param)
     if many:
-        pair, split = load_library("gemm_mx4_pair"), load_library("mx4")
-        parts = torch.empty((2, act_rows, 128 * _tiles(width)), dtype=torch.uint8, device=device)
-        scales = torch.empty((2, 2 * tiles, _tiles(width), 512), dtype=torch.uint8, device=device)
-        _check(split, split.srb_mx4_split_slots(_ptr(h), width, _ptr(plan), _ptr(slot_row), experts, tiles, _ptr(parts), _ptr(scales), stream))
-        _check(pair, pair.srb_mx4_experts_pair(_ptr(parts), _ptr(scales), _ptr(w_gate_up.codes), _ptr(w_gate_up.scales), _ptr(act),
+        pair = load_library("gemm_mx4_pair")
+        _check(pair, pair.srb_mx4_experts_pair(_ptr(parts), _ptr(scales), _ptr(w_gate_up.codes), _ptr(up_scales), _ptr(act),
                                                _ptr(act_scales), _ptr(plan), tiles, entries, experts, inner, width, mode, act_code, param,
                                                _ptr(error_word), stream))
         _check(pair, pair.srb_mx4_experts_pair(_ptr(act), _ptr(act_scales), _ptr(w_down.codes), _ptr(w_down.scales), _ptr(y), None, _ptr(plan),
                                                tiles, entries, experts, width, inner, GEMM_MODES["f32"], 0, param, _ptr(error_word), stream))
     else:
-        parts, scales = _split(h)
-        _check(lib, lib.srb_mx4_experts(_ptr(parts), _ptr(scales), rows, _ptr(slot_row), _ptr(w_gate_up.codes), _ptr(w_gate_up.scales), _ptr(act),
-                                        _ptr(act_scales), _ptr(plan), tiles, entries, experts, inner, width, mode, act_code, param,
+        _check(lib, lib.srb_mx4_experts(_ptr(parts), _ptr(scales), _ptr(w_gate_up.codes), _ptr(up_scales), scale_rows, up_row if gated else 0,
+                                        _ptr(act), _ptr(act_scales), _ptr(plan), tile, tiles, experts, inner, width, mode, act_code, param,
                                         _ptr(error_word), stream))
-        _check(lib, lib.srb_mx4_experts(_ptr(act), _ptr(act_scales), entries, None, _ptr(w_down.codes), _ptr(w_down.scales), _ptr(y), None,
-                                        _ptr(plan), tiles, entries, experts, width, inner, GEMM_MODES["f32"], 0, param, _ptr(error_word), stream))
+        _check(lib, lib.srb_mx4_experts(_ptr(act), _ptr(act_scales), _ptr(w_down.codes), _ptr(w_down.scales), width, 0, _ptr(y), None,
+                                        _ptr(plan), tile, tiles, experts, width, inner, GEMM_MODES["f32"], 0, param, _ptr(error_word), stream))
     _check(lib, lib.srb_mx4_combine(_ptr(y), _ptr(entry_slot), _ptr(weights), rows, top, width, _ptr(out), stream))
     return out
