@@ -59,3 +59,57 @@ __device__ __forceinline__ void mx8_split(float a, float b, unsigned high, unsig
   high_bytes = h;
   low_bytes = l;
 }
+
+// ---- a float as eight parts of four bits ------------------------------------------------------------------------------
+// Few rows go in as eight rows of four-bit entries each: the entries of a block over 2^(E - 1), E = floor(log2(largest magnitude)), are below 4
+// and rounded to the format's values, at most 0.5 off; what is left goes in over a scale 2^3 less, below 4 again, and so on.  The first
+// scale is 2^-106 at least, so that the last is the format's least.  An entry is held to 2^-23 of its block's largest or to 2^-129.
+#define MX4_PARTS 8
+__device__ __forceinline__ unsigned mx4_first_scale(unsigned largest_bits) {
+  return largest_bits >= 0x7f800000u ? 255u : max((largest_bits >> 23), 22u) - 1u;
+}
+__device__ __forceinline__ unsigned mx4_part_scale(unsigned first, int part) { return first == 255u ? 255u : first - 3u * part; }
+__device__ __forceinline__ float mx4_over_first_scale(float v, unsigned first) {
+  return first == 255u ? 0.f : v * __uint_as_float((254u - first) << 23);
+}
+// Eight entries to four bits each, nearest with ties to even, magnitudes above 6 to 6; the first entry in the low bits.
+__device__ __forceinline__ unsigned mx4_pack_eight(const float (&v)[8]) {
+  unsigned out;
+  asm("{\n.reg .b8 a, b, c, d;\n"
+      "cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\ncvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n"
+      "cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\ncvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n"
+      "mov.b32 %0, {a, b, c, d};\n}\n"
+      : "=r"(out) : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]));
+  return out;
+}
+// Two codes (a byte) to their values.
+__device__ __forceinline__ void mx4_two_values(unsigned byte, float& a, float& b) {
+  asm("{\n.reg .b8 c, d, e, f;\n.reg .b32 h;\n.reg .b16 x, y;\nmov.b32 {c, d, e, f}, %2;\ncvt.rn.f16x2.e2m1x2 h, c;\n"
+      "mov.b32 {x, y}, h;\ncvt.f32.f16 %0, x;\ncvt.f32.f16 %1, y;\n}\n" : "=f"(a), "=f"(b) : "r"(byte));
+}
+// The next part of eight entries: their codes; the entries become what is left, over the next part's scale.
+__device__ __forceinline__ unsigned mx4_next_part(float (&v)[8]) {
+  const unsigned codes = mx4_pack_eight(v);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float a, b;
+    mx4_two_values((codes >> (8 * i)) & 255u, a, b);
+    v[2 * i] = (v[2 * i] - a) * 8.f;
+    v[2 * i + 1] = (v[2 * i + 1] - b) * 8.f;
+  }
+  return codes;
+}
+// One entry: the codes of all its parts, the first in the low bits.
+__device__ __forceinline__ unsigned mx4_all_parts(float v) {
+  unsigned all = 0u;
+#pragma unroll
+  for (int part = 0; part < MX4_PARTS; ++part) {
+    unsigned code;
+    asm("{\n.reg .b8 a;\ncvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\nmov.b32 %0, {a, a, a, a};\n}\n" : "=r"(code) : "f"(v), "f"(0.f));
+    float a, b;
+    mx4_two_values(code, a, b);
+    all |= (code & 15u) << (4 * part);
+    v = (v - a) * 8.f;
+  }
+  return all;
+}

@@ -3,7 +3,8 @@
 // Operands lie in shared memory in rows of 128 bytes with the 128-byte swizzle, as for the plain products; a step takes 32 bytes of a row: 64
 // four-bit entries (kind mxf4), or 32 entries of eight bits (kind mxf8f6f4), where four-bit entries stand 16 to 16 bytes, eight bytes of
 // codes and eight that are not read.  Scales lie in tensor memory: row r's in lane r % 32 (of every quarter of the lanes) and
-// column r / 32, a byte for each of four consecutive blocks of 32 entries; the instruction descriptor says which bytes a step takes.
+// column r / 32, a byte for each of four consecutive blocks of 32 entries; the instruction descriptor says which bytes a step takes, and the
+// address may be an even column alone (an odd one faults).
 #pragma once
 #include "common.cuh"
 #include "tcgen05_helpers.cuh"
@@ -18,11 +19,13 @@ __device__ __forceinline__ unsigned mx_idesc(unsigned a_type, unsigned b_type, i
 }
 __device__ __forceinline__ unsigned mx_idesc_step(unsigned idesc, unsigned byte) { return idesc | (byte << 4) | (byte << 29); }
 
-__device__ __forceinline__ void umma_mx8(unsigned tmem_d, unsigned long long a_desc, unsigned long long b_desc, unsigned idesc, unsigned a_scales,
+// kind mxf4: both operands in four bits, packed
+__device__ __forceinline__ unsigned mx_idesc_four(int m, int n) { return (1u << 7) | (1u << 10) | ((unsigned)(n >> 3) << 17) | (1u << 23) | ((unsigned)(m >> 4) << 24); }
+__device__ __forceinline__ void umma_mx4(unsigned tmem_d, unsigned long long a_desc, unsigned long long b_desc, unsigned idesc, unsigned a_scales,
                                          unsigned b_scales, unsigned accumulate) {
   asm volatile(
       "{\n.reg .pred p;\nsetp.ne.b32 p, %6, 0;\n"
-      "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n}\n"
+      "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n}\n"
       ::"r"(tmem_d), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(a_scales), "r"(b_scales), "r"(accumulate) : "memory");
 }
 // 512 bytes of shared memory, 32 rows of 16, to four columns of all lanes (every quarter gets the 32 rows)
@@ -86,8 +89,6 @@ static int make_scales_map(CUtensorMap* map, const void* base, long long tiles, 
 }
 
 // ---- pairs of CTAs (cta_group::2): M = 256, the even CTA's thread issues for both -----------------------------------------
-// kind mxf4: both operands in four bits, packed
-__device__ __forceinline__ unsigned mx_idesc_four(int m, int n) { return (1u << 7) | (1u << 10) | ((unsigned)(n >> 3) << 17) | (1u << 23) | ((unsigned)(m >> 4) << 24); }
 __device__ __forceinline__ void umma_mx4_pair(unsigned tmem_d, unsigned long long a_desc, unsigned long long b_desc, unsigned idesc, unsigned a_scales,
                                               unsigned b_scales, unsigned accumulate) {
   asm volatile(

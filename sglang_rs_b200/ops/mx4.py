@@ -142,6 +142,16 @@ def dequantize_mx4(q: Mx4, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     return out
 
 
+def _parts(x: torch.Tensor):
+    """bfloat16 rows as eight rows of four bits each, and their scales (csrc/mx4.cuh)."""
+    rows, width = x.shape
+    codes = torch.empty((8 * rows, 64 * _tiles(width)), dtype=torch.uint8, device=x.device)
+    scales = torch.empty((_tiles(8 * rows), _tiles(width), 512), dtype=torch.uint8, device=x.device)
+    lib = load_library("mx4")
+    _check(lib, lib.srb_mx4_parts(_ptr(x), ctypes.c_longlong(x.stride(0)), rows, width, _ptr(codes), _ptr(scales), _stream()))
+    return codes, scales
+
+
 def _split(x: torch.Tensor):
     """bfloat16 rows as the two eight-bit parts (and their scales) that multiply four-bit entries (csrc/mx4.cuh)."""
     rows, width = x.shape
@@ -186,8 +196,8 @@ def linear_mx4(x, weight: Mx4, error_word: torch.Tensor, *, bias: Optional[torch
     if out.numel():
         lib = load_library("gemm_mx4_pair" if many else "gemm_mx4")
         product = lib.srb_mx4_linear_pair if many else lib.srb_mx4_linear
-        held, scales = (x.codes, x.scales) if four else _split(x)
-        _check(lib, product(_ptr(held), _ptr(scales), int(four), _ptr(weight.codes), _ptr(weight.scales), _ptr(bias), _ptr(out),
+        held, scales = (x.codes, x.scales) if four else _split(x) if many else _parts(x)
+        _check(lib, product(_ptr(held), _ptr(scales), int(four if many else not four), _ptr(weight.codes), _ptr(weight.scales), _ptr(bias), _ptr(out),
                             ctypes.c_longlong(out.stride(0)), rows, weight.rows, width, int(out_dtype == torch.float32),
                             _ptr(error_word), _stream()))
     return out if pitch == weight.rows else out[:, :weight.rows]
@@ -254,8 +264,7 @@ def chosen_experts_mx4(h: torch.Tensor, chosen: torch.Tensor, weights: torch.Ten
     device, entries, stream = h.device, rows * top, _stream()
     # (the pairs' result rows start on 16-byte borders)
     many = entries > MX4_FEW_CHOICES * experts and width % 4 == 0
-    # slots of a tile, and the rows of its inputs that there is room for
-    tile, room = (256, 256) if many else (32 if entries > 4 * experts else 16, 64)
+    tile = 256 if many else 8
     moe, lib, split = load_library("moe"), load_library("gemm_mx4"), load_library("mx4")
     plan = torch.empty(moe.srb_moe_plan_ints_of(rows, top, experts, tile), dtype=torch.int32, device=device)
     slot_row = torch.empty(entries, dtype=torch.int32, device=device)
@@ -266,13 +275,14 @@ def chosen_experts_mx4(h: torch.Tensor, chosen: torch.Tensor, weights: torch.Ten
     # a tile has a slot at least
     tiles = min(entries, moe.srb_moe_max_tiles_of(rows, top, experts, tile))
 
-    def held(entries_of_a_row):
-        """Room for both parts of every tile's rows, and for their scales."""
-        return (torch.empty((2, room * tiles, 128 * _tiles(entries_of_a_row)), dtype=torch.uint8, device=device),
-                torch.empty((2, _tiles(room * tiles), _tiles(entries_of_a_row), 512), dtype=torch.uint8, device=device))
+    def held(size):
+        """Room for every tile's rows of ``size`` entries, and for their scales: two eight-bit parts of 256 rows, or eight four-bit ones of 8."""
+        if many:
+            return (torch.empty((2, 256 * tiles, 128 * _tiles(size)), dtype=torch.uint8, device=device),
+                    torch.empty((2, 2 * tiles, _tiles(size), 512), dtype=torch.uint8, device=device))
+        return (torch.empty((64 * tiles, 64 * _tiles(size)), dtype=torch.uint8, device=device),
+                torch.empty((_tiles(64 * tiles), _tiles(size), 512), dtype=torch.uint8, device=device))
     (parts, scales), (act, act_scales) = held(width), held(inner)
-    _check(split, split.srb_mx4_split_slots(_ptr(h), width, _ptr(plan), _ptr(slot_row), experts, tile, room, tiles, _ptr(parts), _ptr(scales),
-                                            stream))
     up_scales, scale_rows, up_row = w_gate_up.scales, w_gate_up.rows, inner
     if gated and (many or inner % 128):
         # a tile's gate and up rows side by side: 96 of each for the pairs; otherwise all of them, the up rows on the border of a tile
@@ -282,6 +292,9 @@ def chosen_experts_mx4(h: torch.Tensor, chosen: torch.Tensor, weights: torch.Ten
         up_scales = torch.empty((experts, scale_rows // 128, _tiles(width), 512), dtype=torch.uint8, device=device)
         _check(split, split.srb_mx4_gated_scales(_ptr(w_gate_up.scales), experts, inner, width, group, group_room, groups, _ptr(plan),
                                                  _ptr(up_scales), stream))
+    # (last ahead of the products: those for few rows read what is older than it before it is done)
+    in_slots = split.srb_mx4_split_slots if many else split.srb_mx4_parts_slots
+    _check(split, in_slots(_ptr(h), width, _ptr(plan), _ptr(slot_row), experts, tiles, _ptr(parts), _ptr(scales), stream))
     mode, param = GEMM_MODES["gated" if gated else "act"], ctypes.c_float(activation_param)
     if many:
         pair = load_library("gemm_mx4_pair")
@@ -292,9 +305,9 @@ def chosen_experts_mx4(h: torch.Tensor, chosen: torch.Tensor, weights: torch.Ten
                                                tiles, entries, experts, width, inner, GEMM_MODES["f32"], 0, param, _ptr(error_word), stream))
     else:
         _check(lib, lib.srb_mx4_experts(_ptr(parts), _ptr(scales), _ptr(w_gate_up.codes), _ptr(up_scales), scale_rows, up_row if gated else 0,
-                                        _ptr(act), _ptr(act_scales), _ptr(plan), tile, tiles, experts, inner, width, mode, act_code, param,
+                                        _ptr(act), _ptr(act_scales), _ptr(plan), tiles, experts, inner, width, mode, act_code, param,
                                         _ptr(error_word), stream))
         _check(lib, lib.srb_mx4_experts(_ptr(act), _ptr(act_scales), _ptr(w_down.codes), _ptr(w_down.scales), width, 0, _ptr(y), None,
-                                        _ptr(plan), tile, tiles, experts, width, inner, GEMM_MODES["f32"], 0, param, _ptr(error_word), stream))
+                                        _ptr(plan), tiles, experts, width, inner, GEMM_MODES["f32"], 0, param, _ptr(error_word), stream))
     _check(lib, lib.srb_mx4_combine(_ptr(y), _ptr(entry_slot), _ptr(weights), rows, top, width, _ptr(out), stream))
     return out

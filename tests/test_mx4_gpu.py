@@ -115,12 +115,13 @@ def test_nothing_to_quantize():
 # ------------------------------------------------------------------------------------------- products
 def room_of(x, w, y, out_dtype):
     """How far a product may be off: sums of ceil(width / 32) + 8 terms in 32 bits, each off by at most 2^-23 of the magnitudes; rows held as
-    two parts to 2^-22 of a block's largest entry; one rounding of the result."""
+    parts to 2^-22 of a block's largest entry or, since the format's least scale is 2^-127 and its least step 0.5, to half of 2^-128; one
+    rounding of the result."""
     width = x.shape[1]
     around = x.abs() @ w.abs().T
     padded = torch.nn.functional.pad(x.abs(), (0, -width % 32)).view(x.shape[0], -1, 32).amax(-1)
     blocks = torch.nn.functional.pad(w.abs(), (0, -width % 32)).view(w.shape[0], -1, 32).sum(-1)
-    room = (-(-width // 32) + 8) * 2.0 ** -23 * around + 2.0 ** -22 * (padded @ blocks.T)
+    room = (-(-width // 32) + 8) * 2.0 ** -23 * around + 2.0 ** -22 * (padded @ blocks.T) + 2.0 ** -129 * w.abs().sum(1)
     return room + torch.finfo(out_dtype).eps / 2 * (y.abs() + room) + torch.finfo(out_dtype).smallest_normal
 
 
