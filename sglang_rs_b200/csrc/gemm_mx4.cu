@@ -22,6 +22,7 @@
 #include "common.cuh"
 #include "activations.cuh"
 #include "mx4.cuh"
+#include "mx4_rows.cuh"
 #include "mx4_umma.cuh"
 #include <algorithm>
 
@@ -356,7 +357,6 @@ static int launch_few_staged(const CUtensorMap (&maps)[4], const FewArgs& a, int
   auto kernel = mx4_few_kernel<PARTS, MODE, GROUPED, STAGES>;
   SRB_CUDA_CALL(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   SRB_CUDA_CALL(srb_launch_clustered(kernel, dim3(blocks), dim3(MXF_THREADS), smem, s, dim3(a.splits), maps[0], maps[1], maps[2], maps[3], a));
-  SRB_LAUNCH_CHECK("mx4_few");
   return SRB_OK;
 }
 
@@ -381,101 +381,92 @@ static int launch_few(const void* x, const void* x_scales, long long x_rows, con
   return a.columns <= 64 ? launch_few_staged<PARTS, MODE, GROUPED, 4>(maps, a, blocks, s) : launch_few_staged<PARTS, MODE, GROUPED, 3>(maps, a, blocks, s);
 }
 
-// x: codes [rows, 64 k_tiles] with their scales, or (`parts`) those of srb_mx4_parts [8 rows, 64 k_tiles]; w: codes [features, 64 k_tiles];
-// out [rows, ldo].
-extern "C" int srb_mx4_linear(const void* x, const void* x_scales, int parts, const void* w, const void* w_scales, const float* bias,
-                              void* out, long long ldo, int rows, int features, int width, int out_float, int* error_word, void* stream) {
+// ---- entries: `scratch` has srb_mx4_linear_scratch bytes (none are needed for rows in four bits) ----------------------------
+extern "C" long long srb_mx4_linear_scratch(int rows, int width) {
+  Mx4Scratch scratch = {};
+  scratch.take((size_t)rows * MX4_PARTS * mx4_pitch(width));
+  scratch.take((size_t)mx4_tiles(rows * MX4_PARTS) * mx4_tiles(width) * MX4_TILE_BYTES);
+  return (long long)scratch.used;
+}
+
+// x: bfloat16 [rows, width], `ldx` elements apart, or (x_scales given) codes and their scales; w: codes and scales of features rows; out [rows, ldo].
+extern "C" int srb_mx4_linear(const void* x, long long ldx, const void* x_scales, const void* w, const void* w_scales, const float* bias, void* out,
+                              long long ldo, int rows, int features, int width, int out_float, void* scratch_memory, int* error_word, void* stream) {
   if (rows <= 0 || features <= 0) return SRB_OK;
   if (width <= 0) SRB_FAIL("mx4_linear: inner size %d must be positive", width);
+  if (rows > 1 << 20) SRB_FAIL("mx4_linear: %d rows are not few", rows);
   FewArgs a = {};
   a.bias = bias; a.out = out; a.ldo = ldo; a.rows = rows; a.features = a.w_rows = features; a.k_tiles = mx4_tiles(width); a.error_word = error_word;
   a.ws_tiles = a.tiles_f = mx4_tiles(features);
+  const bool parts = x_scales == nullptr;
   a.tokens = std::min(rows, parts ? MXF_PART_TOKENS : MXF_TOKENS);
   a.columns = (a.tokens * (parts ? MX4_PARTS : 1) + 15) & ~15;
   a.tiles_t = (rows + a.tokens - 1) / a.tokens;
   cudaStream_t s = (cudaStream_t)stream;
   if (!parts)
     return out_float ? launch_few<false, MXF_F32, false>(x, x_scales, rows, w, w_scales, a, s) : launch_few<false, MXF_BF16, false>(x, x_scales, rows, w, w_scales, a, s);
-  return out_float ? launch_few<true, MXF_F32, false>(x, x_scales, 8ll * rows, w, w_scales, a, s) : launch_few<true, MXF_BF16, false>(x, x_scales, 8ll * rows, w, w_scales, a, s);
+  Mx4Scratch scratch = {(uint8_t*)scratch_memory, 0};
+  uint8_t* codes = scratch.take((size_t)rows * MX4_PARTS * mx4_pitch(width));
+  uint8_t* scales = scratch.take((size_t)mx4_tiles(rows * MX4_PARTS) * a.k_tiles * MX4_TILE_BYTES);
+  if (const int status = mx4_launch_parts(x, ldx, rows, width, codes, scales, s)) return status;
+  return out_float ? launch_few<true, MXF_F32, false>(codes, scales, 8ll * rows, w, w_scales, a, s)
+                   : launch_few<true, MXF_BF16, false>(codes, scales, 8ll * rows, w, w_scales, a, s);
 }
 
-// The experts' products over the plan's tiles of 8 slots.  x: parts [64 max_tiles, 64 k_tiles] and their scales, 64 rows a tile.  Mode gated / act:
-// out parts [64 max_tiles, 64 ceil(features / 128)], out_scales theirs; float: out [slots, features].  The gated mode: `up_scale_row` is
-// the row of w_scales' tiles where the up rows begin, a multiple of 128; `scale_rows` the rows that they hold a matrix.
-extern "C" int srb_mx4_experts(const void* x, const void* x_scales, const void* w, const void* w_scales, int scale_rows, int up_scale_row, void* out,
-                               void* out_scales, const int* plan, int max_tiles, int experts, int features, int width, int mode, int activation,
-                               float act_param, int* error_word, void* stream) {
-  if (max_tiles <= 0 || features <= 0) return SRB_OK;
-  if (width <= 0) SRB_FAIL("mx4_experts: inner size %d must be positive", width);
-  if (activation < 0 || activation >= SRB_ACT_COUNT) SRB_FAIL("mx4_experts: unknown activation %d", activation);
-  if (mode != MXF_F32 && mode != MXF_GATED && mode != MXF_ACT) SRB_FAIL("mx4_experts: mode %d is not float, gated or activated", mode);
-  if (mode == MXF_GATED && up_scale_row % 128) SRB_FAIL("mx4_experts: scales of up rows begin at row %d, no multiple of 128", up_scale_row);
+// Scratch of a call on the experts, in the order in which it is taken: rows of the slots, what is between the products, the results, and
+// gate/up scales with the up rows on the border of a tile, where they do not begin there.
+struct FewExpertsScratch {
+  uint8_t *x, *x_scales, *act, *act_scales, *y, *up_scales;
+  size_t bytes;
+  FewExpertsScratch(void* memory, int entries, int max_tiles, int experts, int width, int inner, int gated) {
+    Mx4Scratch s = {(uint8_t*)memory, 0};
+    const size_t rows = (size_t)MXF_SLOTS * MX4_PARTS * max_tiles, row_tiles = (rows + 127) / 128;
+    x = s.take(rows * mx4_pitch(width));
+    x_scales = s.take(row_tiles * mx4_tiles(width) * MX4_TILE_BYTES);
+    act = s.take(rows * mx4_pitch(inner));
+    act_scales = s.take(row_tiles * mx4_tiles(inner) * MX4_TILE_BYTES);
+    y = s.take((size_t)entries * width * 4);
+    up_scales = gated && inner % 128 ? s.take(mx4_gated_scales_bytes(experts, width, 256 * mx4_tiles(inner), 1)) : nullptr;
+    bytes = s.used;
+  }
+};
+extern "C" long long srb_mx4_experts_scratch(int entries, int max_tiles, int experts, int width, int inner, int gated) {
+  return (long long)FewExpertsScratch(nullptr, entries, max_tiles, experts, width, inner, gated).bytes;
+}
+extern "C" int srb_mx4_experts_tile() { return MXF_SLOTS; }
+
+// `plan` (tiles of srb_mx4_experts_tile slots, at most max_tiles), slot_row and entry_slot are those of csrc/moe.cu.
+extern "C" int srb_mx4_experts(const void* h, const int* plan, const int* slot_row, const int* entry_slot, const float* weights, const void* up,
+                               const void* up_scales, const void* down, const void* down_scales, void* out, int rows, int top, int max_tiles,
+                               int experts, int width, int inner, int gated, int activation, float act_param, void* scratch_memory,
+                               int* error_word, void* stream) {
+  if (rows <= 0 || top <= 0) return SRB_OK;
+  const Mx4ExpertsCall c = {h, plan, slot_row, entry_slot, weights, up, up_scales, down, down_scales, out, rows, top, max_tiles, experts, width, inner, gated,
+                            activation, act_param, error_word, (cudaStream_t)stream};
+  if (const int status = mx4_check_experts(c)) return status;
+  const FewExpertsScratch scratch(scratch_memory, rows * top, max_tiles, experts, width, inner, gated);
+  const long long x_rows = (long long)MXF_SLOTS * MX4_PARTS * max_tiles;
   FewArgs a = {};
-  a.out = out; a.out_scales = (uint8_t*)out_scales; a.features = features; a.w_rows = mode == MXF_GATED ? 2 * features : features;
-  a.k_tiles = mx4_tiles(width); a.activation = activation; a.act_param = act_param; a.error_word = error_word;
-  a.ws_tiles = mx4_tiles(scale_rows); a.up_tile = up_scale_row >> 7;
-  a.plan = plan; a.experts = experts; a.tokens = MXF_SLOTS; a.columns = MXF_SLOTS * MX4_PARTS;
-  a.tiles_f = mx4_tiles(features); a.tiles_t = max_tiles;
-  a.ldo = mode == MXF_F32 ? features : (size_t)a.tiles_f * 64;
-  const long long x_rows = (long long)a.columns * max_tiles;
-  cudaStream_t s = (cudaStream_t)stream;
-  if (mode == MXF_F32) return launch_few<true, MXF_F32, true>(x, x_scales, x_rows, w, w_scales, a, s);
-  if (mode == MXF_GATED) return launch_few<true, MXF_GATED, true>(x, x_scales, x_rows, w, w_scales, a, s);
-  return launch_few<true, MXF_ACT, true>(x, x_scales, x_rows, w, w_scales, a, s);
-}
-
-// out[row, :] = sum over the row's choices, in their order, of weight * y[slot, :], in 32 bits, rounded once.  Bound by the bytes of y: four
-// columns a thread, the loads of four choices in flight.
-template <bool WIDE>
-__global__ void __launch_bounds__(128)
-mx4_combine_kernel(const float* __restrict__ y, const int* __restrict__ entry_slot, const float* __restrict__ weights, int top, int width,
-                   __nv_bfloat16* __restrict__ out) {
-  srb_launch_dependents();
-  srb_grid_dependency_wait();
-  const int row = blockIdx.x, i = (blockIdx.y * 128 + threadIdx.x) * 4;
-  if (i >= width) return;
-  const int* slots = entry_slot + (size_t)row * top;
-  const float* w = weights + (size_t)row * top;
-  float sum[4] = {};
-  for (int first = 0; first < top; first += 4) {
-    float v[4][4], by[4];
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const int slot = first + k < top ? slots[first + k] : -1;
-      by[k] = slot >= 0 ? w[first + k] : 0.f;
-      const float* src = y + (size_t)max(slot, 0) * width + i;
-      if (slot < 0) {
-        v[k][0] = v[k][1] = v[k][2] = v[k][3] = 0.f;
-      } else if (WIDE) {
-        const float4 q = *reinterpret_cast<const float4*>(src);
-        v[k][0] = q.x; v[k][1] = q.y; v[k][2] = q.z; v[k][3] = q.w;
-      } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) v[k][j] = i + j < width ? src[j] : 0.f;
-      }
-    }
-#pragma unroll
-    for (int k = 0; k < 4; ++k)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) sum[j] = fmaf(by[k], v[k][j], sum[j]);
+  a.activation = activation; a.act_param = act_param; a.error_word = error_word; a.plan = plan; a.experts = experts; a.tiles_t = max_tiles;
+  a.tokens = MXF_SLOTS; a.columns = MXF_SLOTS * MX4_PARTS;
+  // gate/up: into parts
+  FewArgs first = a;
+  first.out = scratch.act; first.out_scales = scratch.act_scales; first.features = inner; first.w_rows = gated ? 2 * inner : inner;
+  first.k_tiles = mx4_tiles(width); first.tiles_f = mx4_tiles(inner); first.ldo = mx4_pitch(inner);
+  first.ws_tiles = mx4_tiles(first.w_rows); first.up_tile = inner / 128;
+  if (scratch.up_scales) {
+    const int group = 128 * mx4_tiles(inner);
+    if (const int status = mx4_launch_gated_scales(up_scales, experts, inner, width, group, 2 * group, 1, plan, scratch.up_scales, c.stream)) return status;
+    up_scales = scratch.up_scales;
+    first.ws_tiles = 2 * mx4_tiles(inner); first.up_tile = mx4_tiles(inner);
   }
-  __nv_bfloat16* dst = out + (size_t)row * width + i;
-  if (WIDE) {
-    const __nv_bfloat162 a = __floats2bfloat162_rn(sum[0], sum[1]), b = __floats2bfloat162_rn(sum[2], sum[3]);
-    *reinterpret_cast<uint2*>(dst) = make_uint2(*reinterpret_cast<const unsigned*>(&a), *reinterpret_cast<const unsigned*>(&b));
-  } else {
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (i + j < width) dst[j] = __float2bfloat16_rn(sum[j]);
-  }
-}
-extern "C" int srb_mx4_combine(const float* y, const int* entry_slot, const float* weights, int rows, int top, int width, void* out, void* stream) {
-  if (rows <= 0 || width <= 0) return SRB_OK;
-  const bool wide = width % 4 == 0 && (((uintptr_t)y & 15) | ((uintptr_t)out & 7)) == 0;
-  const int pieces = (width + 511) / 512;
-  if (pieces > 65535) SRB_FAIL("mx4_combine: rows of %d are too wide", width);
-  SRB_CUDA_CALL(srb_launch(wide ? mx4_combine_kernel<true> : mx4_combine_kernel<false>, dim3(rows, pieces), dim3(128), 0, (cudaStream_t)stream, y,
-                           entry_slot, weights, top, width, (__nv_bfloat16*)out));
-  SRB_LAUNCH_CHECK("mx4_combine");
-  return SRB_OK;
+  // (last ahead of the products, which read what is older than it before it is done)
+  if (const int status = mx4_launch_parts_slots(h, width, plan, slot_row, experts, max_tiles, scratch.x, scratch.x_scales, c.stream)) return status;
+  if (const int status = gated ? launch_few<true, MXF_GATED, true>(scratch.x, scratch.x_scales, x_rows, up, up_scales, first, c.stream)
+                               : launch_few<true, MXF_ACT, true>(scratch.x, scratch.x_scales, x_rows, up, up_scales, first, c.stream)) return status;
+  FewArgs second = a;
+  second.out = scratch.y; second.features = second.w_rows = width; second.k_tiles = mx4_tiles(inner); second.ws_tiles = second.tiles_f = mx4_tiles(width);
+  second.ldo = width;
+  if (const int status = launch_few<true, MXF_F32, true>(scratch.act, scratch.act_scales, x_rows, down, down_scales, second, c.stream)) return status;
+  return mx4_launch_combine((const float*)scratch.y, entry_slot, weights, rows, top, width, out, c.stream);
 }

@@ -19,6 +19,7 @@
 #include "common.cuh"
 #include "activations.cuh"
 #include "mx4.cuh"
+#include "mx4_rows.cuh"
 #include "mx4_umma.cuh"
 #include <algorithm>
 
@@ -401,75 +402,125 @@ static int launch_pair(const CUtensorMap (&maps)[5], const PairMx4Args& a, int m
   auto kernel = mx4_pair_kernel<FOUR, MODE, GROUPED>;
   SRB_CUDA_CALL(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   SRB_CUDA_CALL(srb_launch_clustered(kernel, dim3(2 * pairs), dim3(Shape::THREADS), smem, s, dim3(2), maps[0], maps[1], maps[2], maps[3], maps[4], a));
-  SRB_LAUNCH_CHECK("mx4_pair");
   return SRB_OK;
 }
 
-// As srb_mx4_linear of gemm_mx4.cu, for many rows; out's rows are `ldo` elements apart, a multiple of 16 bytes.
-extern "C" int srb_mx4_linear_pair(const void* x, const void* x_scales, int four, const void* w, const void* w_scales, const float* bias,
-                                   void* out, long long ldo, int rows, int features, int width, int out_float, int* error_word, void* stream) {
+// ---- entries, as those of gemm_mx4.cu --------------------------------------------------------------------------------
+extern "C" long long srb_mx4_linear_pair_scratch(int rows, int width) {
+  Mx4Scratch scratch = {};
+  scratch.take(2 * (size_t)rows * mx4_tiles(width) * 128);
+  scratch.take(2 * (size_t)mx4_tiles(rows) * mx4_tiles(width) * MX4_TILE_BYTES);
+  return (long long)scratch.used;
+}
+
+// out's rows are `ldo` elements apart, a multiple of 16 bytes.
+extern "C" int srb_mx4_linear_pair(const void* x, long long ldx, const void* x_scales, const void* w, const void* w_scales, const float* bias, void* out,
+                                   long long ldo, int rows, int features, int width, int out_float, void* scratch_memory, int* error_word, void* stream) {
   if (rows <= 0 || features <= 0) return SRB_OK;
   if (width <= 0) SRB_FAIL("mx4_linear_pair: inner size %d must be positive", width);
-  if ((uintptr_t)w & 31) SRB_FAIL("mx4_linear_pair: codes must start on a 32-byte border");
+  if (((uintptr_t)w & 31) || (x_scales && ((uintptr_t)x & 31))) SRB_FAIL("mx4_linear_pair: codes must start on 32-byte borders");
   if (((uintptr_t)out & 15) || ldo * (out_float ? 4 : 2) % 16) SRB_FAIL("mx4_linear_pair: rows of the result must start on 16-byte borders");
   PairMx4Args a = {};
-  a.bias = bias; a.out = out; a.ldo = ldo; a.rows = rows;
-  a.features = a.w_rows = features; a.k_tiles = mx4_tiles(width); a.error_word = error_word;
-  a.x_lo_row = rows; a.xs_lo_tile = mx4_tiles(rows) * a.k_tiles;
-  a.tiles_t = (rows + MXP_TILE - 1) / MXP_TILE; a.tiles_f = (features + MXP_N - 1) / MXP_N;
-  a.ws_tiles = mx4_tiles(features);
-  const long long row_tiles = mx4_tiles(rows), tiles = (long long)a.tiles_t * a.tiles_f;
-  if (tiles > 0x3fffffff || 2ll * row_tiles * 128 > 0x7fffffff) SRB_FAIL("mx4_linear_pair: %d rows x %d features are too many", rows, features);
+  a.bias = bias; a.out = out; a.ldo = ldo; a.rows = rows; a.features = a.w_rows = features; a.k_tiles = mx4_tiles(width); a.error_word = error_word;
+  a.tiles_t = (rows + MXP_TILE - 1) / MXP_TILE; a.tiles_f = (features + MXP_N - 1) / MXP_N; a.ws_tiles = mx4_tiles(features);
+  const long long row_tiles = mx4_tiles(rows), tiles = (long long)a.tiles_t * a.tiles_f, scale_tiles = 2 * row_tiles * a.k_tiles;
+  if (tiles > 0x3fffffff || 2ll * row_tiles * 128 > 0x7fffffff || scale_tiles > 0x7fffffff || (long long)a.ws_tiles * a.k_tiles > 0x7fffffff)
+    SRB_FAIL("mx4_linear_pair: %d rows x %d features of %d are too many", rows, features, width);
+  a.x_lo_row = rows; a.xs_lo_tile = (int)(row_tiles * a.k_tiles);
+  cudaStream_t s = (cudaStream_t)stream;
+  const bool four = x_scales != nullptr;
+  if (!four) {
+    Mx4Scratch scratch = {(uint8_t*)scratch_memory, 0};
+    uint8_t* parts = scratch.take(2 * (size_t)rows * a.k_tiles * 128);
+    uint8_t* scales = scratch.take((size_t)scale_tiles * MX4_TILE_BYTES);
+    if (const int status = mx4_launch_split(x, ldx, rows, width, parts, scales, s)) return status;
+    x = parts; x_scales = scales;
+  }
   CUtensorMap maps[5];
   if (make_bytes_map(&maps[0], x, four ? rows : 2ll * rows, a.k_tiles * (four ? 64 : 128), MXP_ROWS) != SRB_OK ||
-      make_scales_map(&maps[1], x_scales, (four ? 1 : 2) * row_tiles * a.k_tiles, four ? 2 : 1) != SRB_OK ||
+      make_scales_map(&maps[1], x_scales, four ? scale_tiles / 2 : scale_tiles, four ? 2 : 1) != SRB_OK ||
       (four ? make_bytes_map(&maps[2], w, features, a.k_tiles * 64, MXP_HALF) : make_codes_map(&maps[2], w, features, a.k_tiles, MXP_HALF)) != SRB_OK ||
-      make_scales_map(&maps[3], w_scales, (long long)mx4_tiles(features) * a.k_tiles, four ? 2 : 1) != SRB_OK ||
+      make_scales_map(&maps[3], w_scales, (long long)a.ws_tiles * a.k_tiles, four ? 2 : 1) != SRB_OK ||
       make_map(&maps[4], out_float ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, out, rows, features, ldo * (out_float ? 4 : 2),
                32, out_float ? 16 : 32, CU_TENSOR_MAP_SWIZZLE_64B) != SRB_OK)
     return SRB_ERR_INVALID;
-  cudaStream_t s = (cudaStream_t)stream;
   if (four) return out_float ? launch_pair<true, MXP_F32, false>(maps, a, (int)tiles, s) : launch_pair<true, MXP_BF16, false>(maps, a, (int)tiles, s);
   return out_float ? launch_pair<false, MXP_F32, false>(maps, a, (int)tiles, s) : launch_pair<false, MXP_BF16, false>(maps, a, (int)tiles, s);
 }
 
-// The experts' products over the plan's tiles of 256 slots.  x: parts [2, 256 max_tiles, 128 k_tiles] and their scales, 256 rows a tile.  Mode gated /
-// act: out parts [2, 256 max_tiles, 128 ceil(features / 128)], out_scales theirs; float: out [slots, features], rows on 16-byte borders.  The gated
-// mode's w_scales are those of srb_mx4_gated_scales, groups of 96 in the room of 256.
-extern "C" int srb_mx4_experts_pair(const void* x, const void* x_scales, const void* w, const void* w_scales, void* out, void* out_scales,
-                                    const int* plan, int max_tiles, int slots, int experts, int features, int width, int mode, int activation,
-                                    float act_param, int* error_word, void* stream) {
-  if (max_tiles <= 0 || features <= 0) return SRB_OK;
-  if (width <= 0) SRB_FAIL("mx4_experts_pair: inner size %d must be positive", width);
-  if ((uintptr_t)w & 31) SRB_FAIL("mx4_experts_pair: codes must start on a 32-byte border");
-  if (activation < 0 || activation >= SRB_ACT_COUNT) SRB_FAIL("mx4_experts_pair: unknown activation %d", activation);
-  if (mode != MXP_F32 && mode != MXP_GATED && mode != MXP_ACT) SRB_FAIL("mx4_experts_pair: mode %d is not float, gated or activated", mode);
+// One of the experts' products over the plan's tiles.  x: parts [2, 256 max_tiles, 128 k_tiles] and their scales, 256 rows a tile.  Gated / activated:
+// out parts of that form, out_scales theirs; float: out [slots, features], rows on 16-byte borders.  The gated mode's w_scales are in
+// groups of 96 gate and 96 up rows in the room of 256.
+static int pair_experts_product(int mode, const Mx4ExpertsCall& c, const uint8_t* x, const uint8_t* x_scales, const void* w, const void* w_scales, void* out,
+                                uint8_t* out_scales, int features, int width) {
   PairMx4Args a = {};
-  a.out = out; a.out_scales = (uint8_t*)out_scales; a.rows = slots;
-  a.features = features; a.w_rows = mode == MXP_GATED ? 2 * features : features; a.k_tiles = mx4_tiles(width); a.activation = activation;
-  a.act_param = act_param; a.error_word = error_word; a.plan = plan; a.experts = experts;
-  const long long rows = 256ll * max_tiles;
-  const int out_tiles = mx4_tiles(features);
-  a.x_lo_row = (int)rows; a.xs_lo_tile = 2 * max_tiles * a.k_tiles;
-  const int covered = mode == MXP_F32 ? features : 128 * out_tiles, per_tile = mode == MXP_GATED ? MXP_HALF : MXP_N;
+  a.out = out; a.out_scales = out_scales; a.rows = c.rows * c.top; a.features = features; a.w_rows = mode == MXP_GATED ? 2 * features : features;
+  a.k_tiles = mx4_tiles(width); a.activation = c.activation; a.act_param = c.act_param; a.error_word = c.error_word; a.plan = c.plan; a.experts = c.experts;
+  const long long rows = (long long)MXP_TILE * c.max_tiles;
+  const int out_tiles = mx4_tiles(features), covered = mode == MXP_F32 ? features : 128 * out_tiles, per_tile = mode == MXP_GATED ? MXP_HALF : MXP_N;
+  a.x_lo_row = (int)rows; a.xs_lo_tile = 2 * c.max_tiles * a.k_tiles;
   a.tiles_f = (covered + per_tile - 1) / per_tile;
-  a.ws_tiles = mode == MXP_GATED ? 2 * a.tiles_f : mx4_tiles(features);
-  a.ldo = mode == MXP_F32 ? features : 128 * out_tiles;
-  a.out_part = (size_t)rows * a.ldo; a.os_part = (size_t)2 * max_tiles * out_tiles * MX4_TILE_BYTES;
-  if (2 * rows > 0x7fffffff || (long long)experts * a.w_rows > 0x7fffffff || (long long)experts * a.ws_tiles * a.k_tiles > 0x7fffffff || (long long)max_tiles * a.tiles_f > 0x3fffffff) SRB_FAIL("mx4_experts_pair: %d tiles are too many", max_tiles);
-  if (mode == MXP_F32 && (((uintptr_t)out & 15) || features % 4)) SRB_FAIL("mx4_experts_pair: rows of the result must start on 16-byte borders");
+  a.ws_tiles = mode == MXP_GATED ? 2 * a.tiles_f : out_tiles;
+  a.ldo = covered;
+  a.out_part = (size_t)rows * a.ldo; a.os_part = (size_t)2 * c.max_tiles * out_tiles * MX4_TILE_BYTES;
+  const long long w_rows = (long long)c.experts * a.w_rows, ws_tiles = (long long)c.experts * a.ws_tiles * a.k_tiles;
+  if (2 * rows > 0x7fffffff || w_rows > 0x7fffffff || ws_tiles > 0x7fffffff || 4ll * c.max_tiles * a.k_tiles > 0x7fffffff ||
+      (long long)c.max_tiles * a.tiles_f > 0x3fffffff)
+    SRB_FAIL("four-bit experts: %d tiles of rows, %lld rows of weights are too many", c.max_tiles, w_rows);
   CUtensorMap maps[5];
   if (make_bytes_map(&maps[0], x, 2 * rows, a.k_tiles * 128, MXP_ROWS) != SRB_OK ||
-      make_scales_map(&maps[1], x_scales, 4ll * max_tiles * a.k_tiles, 1) != SRB_OK ||
-      make_codes_map(&maps[2], w, (long long)experts * a.w_rows, a.k_tiles, MXP_HALF) != SRB_OK ||
-      make_scales_map(&maps[3], w_scales, (long long)experts * a.ws_tiles * a.k_tiles, 1) != SRB_OK)
+      make_scales_map(&maps[1], x_scales, 4ll * c.max_tiles * a.k_tiles, 1) != SRB_OK || make_codes_map(&maps[2], w, w_rows, a.k_tiles, MXP_HALF) != SRB_OK ||
+      make_scales_map(&maps[3], w_scales, ws_tiles, 1) != SRB_OK)
     return SRB_ERR_INVALID;
   maps[4] = maps[0];
-  if (mode == MXP_F32 && make_map(&maps[4], CU_TENSOR_MAP_DATA_TYPE_FLOAT32, out, slots, features, features * 4ll, 32, 16, CU_TENSOR_MAP_SWIZZLE_64B) != SRB_OK)
+  if (mode == MXP_F32 && make_map(&maps[4], CU_TENSOR_MAP_DATA_TYPE_FLOAT32, out, a.rows, features, features * 4ll, 32, 16, CU_TENSOR_MAP_SWIZZLE_64B) != SRB_OK)
     return SRB_ERR_INVALID;
-  cudaStream_t s = (cudaStream_t)stream;
-  const int tiles = max_tiles * a.tiles_f;
-  if (mode == MXP_F32) return launch_pair<false, MXP_F32, true>(maps, a, tiles, s);
-  if (mode == MXP_GATED) return launch_pair<false, MXP_GATED, true>(maps, a, tiles, s);
-  return launch_pair<false, MXP_ACT, true>(maps, a, tiles, s);
+  const int tiles = c.max_tiles * a.tiles_f;
+  if (mode == MXP_F32) return launch_pair<false, MXP_F32, true>(maps, a, tiles, c.stream);
+  if (mode == MXP_GATED) return launch_pair<false, MXP_GATED, true>(maps, a, tiles, c.stream);
+  return launch_pair<false, MXP_ACT, true>(maps, a, tiles, c.stream);
+}
+
+struct PairExpertsScratch {
+  uint8_t *x, *x_scales, *act, *act_scales, *y, *up_scales;
+  size_t bytes;
+  int groups;                    // of 96 gate and 96 up rows
+  PairExpertsScratch(void* memory, int entries, int max_tiles, int experts, int width, int inner, int gated) {
+    Mx4Scratch s = {(uint8_t*)memory, 0};
+    const size_t rows = 2 * (size_t)MXP_TILE * max_tiles;
+    groups = (128 * mx4_tiles(inner) + MXP_HALF - 1) / MXP_HALF;
+    x = s.take(rows * mx4_tiles(width) * 128);
+    x_scales = s.take(rows / 128 * mx4_tiles(width) * MX4_TILE_BYTES);
+    act = s.take(rows * mx4_tiles(inner) * 128);
+    act_scales = s.take(rows / 128 * mx4_tiles(inner) * MX4_TILE_BYTES);
+    y = s.take((size_t)entries * width * 4);
+    up_scales = gated ? s.take(mx4_gated_scales_bytes(experts, width, 256, groups)) : nullptr;
+    bytes = s.used;
+  }
+};
+extern "C" long long srb_mx4_experts_pair_scratch(int entries, int max_tiles, int experts, int width, int inner, int gated) {
+  return (long long)PairExpertsScratch(nullptr, entries, max_tiles, experts, width, inner, gated).bytes;
+}
+extern "C" int srb_mx4_experts_pair_tile() { return MXP_TILE; }
+
+// width is a multiple of 4.
+extern "C" int srb_mx4_experts_pair(const void* h, const int* plan, const int* slot_row, const int* entry_slot, const float* weights, const void* up,
+                                    const void* up_scales, const void* down, const void* down_scales, void* out, int rows, int top, int max_tiles,
+                                    int experts, int width, int inner, int gated, int activation, float act_param, void* scratch_memory,
+                                    int* error_word, void* stream) {
+  if (rows <= 0 || top <= 0) return SRB_OK;
+  const Mx4ExpertsCall c = {h, plan, slot_row, entry_slot, weights, up, up_scales, down, down_scales, out, rows, top, max_tiles, experts, width, inner, gated,
+                            activation, act_param, error_word, (cudaStream_t)stream};
+  if (const int status = mx4_check_experts(c)) return status;
+  if (width % 4) SRB_FAIL("mx4_experts_pair: width %d is no multiple of 4", width);
+  const PairExpertsScratch scratch(scratch_memory, rows * top, max_tiles, experts, width, inner, gated);
+  if (gated) {
+    if (const int status = mx4_launch_gated_scales(up_scales, experts, inner, width, MXP_HALF, 256, scratch.groups, plan, scratch.up_scales, c.stream)) return status;
+    up_scales = scratch.up_scales;
+  }
+  if (const int status = mx4_launch_split_slots(h, width, plan, slot_row, experts, max_tiles, scratch.x, scratch.x_scales, c.stream)) return status;
+  if (const int status = pair_experts_product(gated ? MXP_GATED : MXP_ACT, c, scratch.x, scratch.x_scales, up, up_scales, scratch.act, scratch.act_scales,
+                                              inner, width)) return status;
+  if (const int status = pair_experts_product(MXP_F32, c, scratch.act, scratch.act_scales, down, down_scales, scratch.y, nullptr, width, inner)) return status;
+  return mx4_launch_combine((const float*)scratch.y, entry_slot, weights, rows, top, width, out, c.stream);
 }

@@ -34,6 +34,15 @@ __device__ __forceinline__ float mx4_code_value(unsigned code) {
   return code & 8u ? -v : v;
 }
 
+__device__ __forceinline__ void mx4_unpack_bf16(const uint4& raw, float (&v)[8]) {
+  const unsigned w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    v[2 * i] = __uint_as_float(w[i] << 16);
+    v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+  }
+}
+
 // ---- a float as two parts of eight bits -----------------------------------------------------------------------------
 // The block-scaled products multiply four-bit entries with eight-bit ones (e4m3: four significant bits), so a row of more bits goes in as
 // two parts: the entries of a block over 2^(E - 7), E = floor(log2(largest magnitude)), rounded to e4m3, and what is left over a scale 2^5

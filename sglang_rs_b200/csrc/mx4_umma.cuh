@@ -63,7 +63,7 @@ static EncodeTiledFn encode_tiled() {
 }
 
 // A matrix [rows, columns] of elements of `type`, `pitch` bytes apart, cut into boxes.
-static int make_map(CUtensorMap* map, CUtensorMapDataType type, const void* base, long long rows, long long columns, long long pitch,
+static inline int make_map(CUtensorMap* map, CUtensorMapDataType type, const void* base, long long rows, long long columns, long long pitch,
                     int box_rows, int box_columns, CUtensorMapSwizzle swizzle) {
   EncodeTiledFn fn = encode_tiled();
   if (!fn) SRB_FAIL("four-bit products: the driver does not offer cuTensorMapEncodeTiled");
@@ -76,15 +76,15 @@ static int make_map(CUtensorMap* map, CUtensorMapDataType type, const void* base
   if (status != CUDA_SUCCESS) SRB_FAIL("four-bit products: cuTensorMapEncodeTiled failed with %d", (int)status);
   return SRB_OK;
 }
-static int make_bytes_map(CUtensorMap* map, const void* base, long long rows, long long bytes, int box_rows) {
+static inline int make_bytes_map(CUtensorMap* map, const void* base, long long rows, long long bytes, int box_rows) {
   return make_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, base, rows, bytes, bytes, box_rows, 128, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 // Codes that stand 16 to 16 bytes in shared memory, as kind mxf8f6f4 takes them (a box of 128 entries is 128 bytes a row there; the barrier
 // counts the 64 bytes of codes).  Base on a 32-byte border, `k_tiles` * 64 bytes a row.
-static int make_codes_map(CUtensorMap* map, const void* base, long long rows, int k_tiles, int box_rows) {
+static inline int make_codes_map(CUtensorMap* map, const void* base, long long rows, int k_tiles, int box_rows) {
   return make_map(map, CU_TENSOR_MAP_DATA_TYPE_16U4_ALIGN16B, base, rows, k_tiles * 128ll, k_tiles * 64ll, box_rows, 128, CU_TENSOR_MAP_SWIZZLE_128B);
 }
-static int make_scales_map(CUtensorMap* map, const void* base, long long tiles, int at_once) {
+static inline int make_scales_map(CUtensorMap* map, const void* base, long long tiles, int at_once) {
   return make_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, base, tiles, 128, 512, at_once, 128, CU_TENSOR_MAP_SWIZZLE_NONE);
 }
 

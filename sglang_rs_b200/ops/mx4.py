@@ -13,7 +13,8 @@ from typing import Optional
 import torch
 
 from ..csrc.build import load_library
-from . import (GEMM_MODES, KernelError, ROUTER_SCORING, _check, _need, _need_rows, _ptr, _stream, activation_code, dtype_code)
+from .. import ops as _ops
+from . import KernelError, ROUTER_SCORING, _check, _need, _need_rows, activation_code, dtype_code
 from .trace import traced
 
 #: entries of a row that share a scale
@@ -23,12 +24,50 @@ MX4_FEW_ROWS = 64
 #: experts' products run on pairs of CTAs where a step has more choices per expert than this
 MX4_FEW_CHOICES = 16
 
+_P, _I, _L, _F = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_float
+_LINEAR = (_P, _L, _P, _P, _P, _P, _P, _L, _I, _I, _I, _I, _P, _P, _P)
+_EXPERTS = (_P,) * 10 + (_I,) * 8 + (_F, _P, _P, _P)
+#: entry points by library and their arguments, declared once: a small call costs as long on the host as on the device
+_SIGNATURES = {
+    "mx4": {"srb_mx4_quantize": (_P, _L, _L, _I, _I, _I, _P, _P, _I, _P), "srb_mx4_dequantize": (_P, _P, _I, _I, _I, _P, _I, _P)},
+    "gemm_mx4": {"srb_mx4_linear": _LINEAR, "srb_mx4_experts": _EXPERTS, "srb_mx4_linear_scratch": (_I,) * 2,
+                 "srb_mx4_experts_scratch": (_I,) * 6, "srb_mx4_experts_tile": ()},
+    "gemm_mx4_pair": {"srb_mx4_linear_pair": _LINEAR, "srb_mx4_experts_pair": _EXPERTS, "srb_mx4_linear_pair_scratch": (_I,) * 2,
+                      "srb_mx4_experts_pair_scratch": (_I,) * 6, "srb_mx4_experts_pair_tile": ()},
+    "route_groups": {"srb_route_groups": (_P, _L, _I, _I, _P, _I, _I, _I, _I, _I, _I, _F, _F, _P, _P, _P)},
+}
+_declared: dict = {}
+
+
+def _library(name: str):
+    library = _declared.get(name)
+    if library is None:
+        library = load_library(name)
+        for function, arguments in _SIGNATURES[name].items():
+            getattr(library, function).argtypes = arguments
+            if function.endswith("_scratch"):
+                getattr(library, function).restype = _L
+        _declared[name] = library
+    return library
+
+
+def _stream():
+    """The handle of torch's current stream (of the scope's, inside one), without the object that torch makes around it: that costs
+    as much as a launch."""
+    scoped = _ops._scoped_stream
+    return scoped if scoped is not None else torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
+
 
 def _tiles(n: int) -> int:
     return -(-n // 128)
 
 
-@dataclass(frozen=True)
+def _room(n: int) -> int:
+    """Bytes of a piece of scratch memory: pieces start on 256-byte borders."""
+    return (n + 255) & ~255
+
+
+@dataclass(frozen=True, eq=False)
 class Mx4:
     """A matrix [rows, width] (or several [matrices, rows, width]) in four bits, laid out for the kernels (csrc/mx4.cuh).
 
@@ -38,6 +77,15 @@ class Mx4:
     codes: torch.Tensor
     scales: torch.Tensor
     width: int
+
+    def __post_init__(self):
+        codes, scales = self.codes, self.scales
+        if (not isinstance(codes, torch.Tensor) or not isinstance(scales, torch.Tensor) or codes.dtype != torch.uint8 or scales.dtype != torch.uint8
+                or codes.dim() not in (2, 3) or self.width <= 0 or codes.shape[-1] != 64 * _tiles(self.width) or scales.device != codes.device
+                or scales.shape != (*codes.shape[:-2], _tiles(codes.shape[-2]), _tiles(self.width), 512)
+                or not codes.is_contiguous() or not scales.is_contiguous() or codes.data_ptr() % 32 or scales.data_ptr() % 16):
+            raise KernelError(f"Mx4: codes and scales do not hold rows of {self.width}: contiguous uint8 [..., rows, 64 * ceil(width / 128)] on a "
+                              "32-byte border and [..., ceil(rows / 128), ceil(width / 128), 512] on a 16-byte border are needed")
 
     @property
     def rows(self) -> int:
@@ -61,21 +109,18 @@ def _here(what: str, *tensors: Optional[torch.Tensor]) -> None:
     """The kernels run on the current device's stream: what they read and write has to be there."""
     here = torch.cuda.current_device()
     for tensor in tensors:
-        if tensor is not None and tensor.device.index != here:
+        if tensor is not None and tensor.get_device() != here:
             raise KernelError(f"{what}: a tensor lies on {tensor.device}, the current device is cuda:{here}")
 
 
 def _need_mx4(q: Mx4, name: str, stacked: Optional[bool]) -> None:
-    """``q``'s tensors as the kernels take them (``stacked``: several matrices, one, or either)."""
+    """``q`` as the kernels take it (``stacked``: several matrices, one, or either)."""
     if not isinstance(q, Mx4):
         raise KernelError(f"{name} must be an Mx4, found {type(q).__name__}")
-    _need(q.codes, f"{name}.codes", torch.uint8); _need(q.scales, f"{name}.scales", torch.uint8)
+    if not q.codes.is_cuda:
+        raise KernelError(f"{name} must be on a CUDA device; this engine has no host path")
     if stacked is not None and (q.codes.dim() == 3) != stacked:
         raise KernelError(f"{name} must be {'a stack of matrices' if stacked else 'one matrix'}, found {q.shape}")
-    lead = q.codes.shape[:-2]
-    if (q.codes.dim() not in (2, 3) or q.width <= 0 or q.codes.shape[-1] != 64 * _tiles(q.width)
-            or q.scales.shape != (*lead, _tiles(q.rows), _tiles(q.width), 512) or q.codes.data_ptr() % 32 or q.scales.data_ptr() % 16):
-        raise KernelError(f"{name}: codes {tuple(q.codes.shape)} and scales {tuple(q.scales.shape)} do not hold rows of {q.width}")
 
 
 def mx4_from_rows(codes: torch.Tensor, scales: torch.Tensor, width: Optional[int] = None) -> Mx4:
@@ -122,10 +167,10 @@ def quantize_mx4(x: torch.Tensor) -> Mx4:
         raise KernelError("quantize_mx4: rows without entries")
     q = Mx4(torch.empty((*lead, rows, 64 * _tiles(width)), dtype=torch.uint8, device=x.device),
             torch.empty((*lead, _tiles(rows), _tiles(width), 512), dtype=torch.uint8, device=x.device), width)
-    if rows and (not lead or lead[0]):
-        lib = load_library("mx4")
-        _check(lib, lib.srb_mx4_quantize(_ptr(x), ctypes.c_longlong(x.stride(-2)), ctypes.c_longlong(x.stride(0) if lead else 0),
-                                         lead[0] if lead else 1, rows, width, _ptr(q.codes), _ptr(q.scales), code, _stream()))
+    if x.numel():
+        lib = _library("mx4")
+        _check(lib, lib.srb_mx4_quantize(x.data_ptr(), x.stride(-2), x.stride(0) if lead else 0, lead[0] if lead else 1, rows, width,
+                                         q.codes.data_ptr(), q.scales.data_ptr(), code, _stream()))
     return q
 
 
@@ -137,29 +182,9 @@ def dequantize_mx4(q: Mx4, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     _here("dequantize_mx4", q.codes, q.scales)
     out = torch.empty(q.shape, dtype=dtype, device=q.device)
     if out.numel():
-        lib = load_library("mx4")
-        _check(lib, lib.srb_mx4_dequantize(_ptr(q.codes), _ptr(q.scales), q.matrices or 1, q.rows, q.width, _ptr(out), code, _stream()))
+        lib = _library("mx4")
+        _check(lib, lib.srb_mx4_dequantize(q.codes.data_ptr(), q.scales.data_ptr(), q.matrices or 1, q.rows, q.width, out.data_ptr(), code, _stream()))
     return out
-
-
-def _parts(x: torch.Tensor):
-    """bfloat16 rows as eight rows of four bits each, and their scales (csrc/mx4.cuh)."""
-    rows, width = x.shape
-    codes = torch.empty((8 * rows, 64 * _tiles(width)), dtype=torch.uint8, device=x.device)
-    scales = torch.empty((_tiles(8 * rows), _tiles(width), 512), dtype=torch.uint8, device=x.device)
-    lib = load_library("mx4")
-    _check(lib, lib.srb_mx4_parts(_ptr(x), ctypes.c_longlong(x.stride(0)), rows, width, _ptr(codes), _ptr(scales), _stream()))
-    return codes, scales
-
-
-def _split(x: torch.Tensor):
-    """bfloat16 rows as the two eight-bit parts (and their scales) that multiply four-bit entries (csrc/mx4.cuh)."""
-    rows, width = x.shape
-    parts = torch.empty((2, rows, 128 * _tiles(width)), dtype=torch.uint8, device=x.device)
-    scales = torch.empty((2, _tiles(rows), _tiles(width), 512), dtype=torch.uint8, device=x.device)
-    lib = load_library("mx4")
-    _check(lib, lib.srb_mx4_split(_ptr(x), ctypes.c_longlong(x.stride(0)), rows, width, _ptr(parts), _ptr(scales), _stream()))
-    return parts, scales
 
 
 @traced("gemm")
@@ -194,12 +219,13 @@ def linear_mx4(x, weight: Mx4, error_word: torch.Tensor, *, bias: Optional[torch
     pitch = -(-weight.rows // 8) * 8 if many else weight.rows
     out = torch.empty((rows, pitch), dtype=out_dtype, device=weight.device)
     if out.numel():
-        lib = load_library("gemm_mx4_pair" if many else "gemm_mx4")
-        product = lib.srb_mx4_linear_pair if many else lib.srb_mx4_linear
-        held, scales = (x.codes, x.scales) if four else _split(x) if many else _parts(x)
-        _check(lib, product(_ptr(held), _ptr(scales), int(four if many else not four), _ptr(weight.codes), _ptr(weight.scales), _ptr(bias), _ptr(out),
-                            ctypes.c_longlong(out.stride(0)), rows, weight.rows, width, int(out_dtype == torch.float32),
-                            _ptr(error_word), _stream()))
+        lib = _library("gemm_mx4_pair" if many else "gemm_mx4")
+        product, needed = (lib.srb_mx4_linear_pair, lib.srb_mx4_linear_pair_scratch) if many else (lib.srb_mx4_linear, lib.srb_mx4_linear_scratch)
+        held = x.codes if four else x
+        scratch = None if four else torch.empty(needed(rows, width), dtype=torch.uint8, device=weight.device)
+        _check(lib, product(held.data_ptr(), held.stride(0), x.scales.data_ptr() if four else None, weight.codes.data_ptr(), weight.scales.data_ptr(),
+                            None if bias is None else bias.data_ptr(), out.data_ptr(), pitch, rows, weight.rows, width,
+                            out_dtype == torch.float32, None if four else scratch.data_ptr(), error_word.data_ptr(), _stream()), 1 if four else 2)
     return out if pitch == weight.rows else out[:, :weight.rows]
 
 
@@ -228,10 +254,10 @@ def choose_experts(logits: torch.Tensor, top: int, renormalize: bool = False, *,
     _here("choose_experts", logits, choice_bias)
     chosen = torch.empty((rows, top), dtype=torch.int32, device=logits.device)
     weights = torch.empty((rows, top), dtype=torch.float32, device=logits.device)
-    lib = load_library("route_groups")
-    _check(lib, lib.srb_route_groups(_ptr(logits), ctypes.c_longlong(logits.stride(0)), rows, experts, _ptr(choice_bias), int(top), int(groups),
-                                     int(top_groups), int(group_best), ROUTER_SCORING[scoring], int(renormalize), ctypes.c_float(weight_scale),
-                                     ctypes.c_float(norm_eps), _ptr(chosen), _ptr(weights), _stream()))
+    lib = _library("route_groups")
+    _check(lib, lib.srb_route_groups(logits.data_ptr(), logits.stride(0), rows, experts, None if choice_bias is None else choice_bias.data_ptr(), top,
+                                     groups, top_groups, group_best, ROUTER_SCORING[scoring], renormalize, weight_scale, norm_eps, chosen.data_ptr(),
+                                     weights.data_ptr(), _stream()))
     return chosen, weights
 
 
@@ -261,53 +287,24 @@ def chosen_experts_mx4(h: torch.Tensor, chosen: torch.Tensor, weights: torch.Ten
     if rows == 0 or top == 0:
         return torch.zeros((rows, width), dtype=torch.bfloat16, device=h.device)
     out = torch.empty((rows, width), dtype=torch.bfloat16, device=h.device)
-    device, entries, stream = h.device, rows * top, _stream()
+    entries, stream = rows * top, _stream()
     # (the pairs' result rows start on 16-byte borders)
     many = entries > MX4_FEW_CHOICES * experts and width % 4 == 0
-    tile = 256 if many else 8
-    moe, lib, split = load_library("moe"), load_library("gemm_mx4"), load_library("mx4")
-    plan = torch.empty(moe.srb_moe_plan_ints_of(rows, top, experts, tile), dtype=torch.int32, device=device)
-    slot_row = torch.empty(entries, dtype=torch.int32, device=device)
-    entry_slot = torch.empty(entries, dtype=torch.int32, device=device)
-    y = torch.empty((entries, width), dtype=torch.float32, device=device)
-    _check(moe, moe.srb_moe_plan_of(_ptr(chosen), rows, top, experts, tile, _ptr(plan), _ptr(slot_row), _ptr(entry_slot), None, None,
-                                    _ptr(error_word), stream))
+    moe, lib = load_library("moe"), _library("gemm_mx4_pair" if many else "gemm_mx4")
+    experts_of, needed, tile = ((lib.srb_mx4_experts_pair, lib.srb_mx4_experts_pair_scratch, lib.srb_mx4_experts_pair_tile) if many
+                                else (lib.srb_mx4_experts, lib.srb_mx4_experts_scratch, lib.srb_mx4_experts_tile))
+    tile = tile()
     # a tile has a slot at least
-    tiles = min(entries, moe.srb_moe_max_tiles_of(rows, top, experts, tile))
-
-    def held(size):
-        """Room for every tile's rows of ``size`` entries, and for their scales: two eight-bit parts of 256 rows, or eight four-bit ones of 8."""
-        if many:
-            return (torch.empty((2, 256 * tiles, 128 * _tiles(size)), dtype=torch.uint8, device=device),
-                    torch.empty((2, 2 * tiles, _tiles(size), 512), dtype=torch.uint8, device=device))
-        return (torch.empty((64 * tiles, 64 * _tiles(size)), dtype=torch.uint8, device=device),
-                torch.empty((_tiles(64 * tiles), _tiles(size), 512), dtype=torch.uint8, device=device))
-    (parts, scales), (act, act_scales) = held(width), held(inner)
-    up_scales, scale_rows, up_row = w_gate_up.scales, w_gate_up.rows, inner
-    if gated and (many or inner % 128):
-        # a tile's gate and up rows side by side: 96 of each for the pairs; otherwise all of them, the up rows on the border of a tile
-        group = 96 if many else 128 * _tiles(inner)
-        group_room, groups = (256, -(-128 * _tiles(inner) // 96)) if many else (2 * group, 1)
-        scale_rows, up_row = groups * group_room, group
-        up_scales = torch.empty((experts, scale_rows // 128, _tiles(width), 512), dtype=torch.uint8, device=device)
-        _check(split, split.srb_mx4_gated_scales(_ptr(w_gate_up.scales), experts, inner, width, group, group_room, groups, _ptr(plan),
-                                                 _ptr(up_scales), stream))
-    # (last ahead of the products: those for few rows read what is older than it before it is done)
-    in_slots = split.srb_mx4_split_slots if many else split.srb_mx4_parts_slots
-    _check(split, in_slots(_ptr(h), width, _ptr(plan), _ptr(slot_row), experts, tiles, _ptr(parts), _ptr(scales), stream))
-    mode, param = GEMM_MODES["gated" if gated else "act"], ctypes.c_float(activation_param)
-    if many:
-        pair = load_library("gemm_mx4_pair")
-        _check(pair, pair.srb_mx4_experts_pair(_ptr(parts), _ptr(scales), _ptr(w_gate_up.codes), _ptr(up_scales), _ptr(act),
-                                               _ptr(act_scales), _ptr(plan), tiles, entries, experts, inner, width, mode, act_code, param,
-                                               _ptr(error_word), stream))
-        _check(pair, pair.srb_mx4_experts_pair(_ptr(act), _ptr(act_scales), _ptr(w_down.codes), _ptr(w_down.scales), _ptr(y), None, _ptr(plan),
-                                               tiles, entries, experts, width, inner, GEMM_MODES["f32"], 0, param, _ptr(error_word), stream))
-    else:
-        _check(lib, lib.srb_mx4_experts(_ptr(parts), _ptr(scales), _ptr(w_gate_up.codes), _ptr(up_scales), scale_rows, up_row if gated else 0,
-                                        _ptr(act), _ptr(act_scales), _ptr(plan), tiles, experts, inner, width, mode, act_code, param,
-                                        _ptr(error_word), stream))
-        _check(lib, lib.srb_mx4_experts(_ptr(act), _ptr(act_scales), _ptr(w_down.codes), _ptr(w_down.scales), width, 0, _ptr(y), None,
-                                        _ptr(plan), tiles, experts, width, inner, GEMM_MODES["f32"], 0, param, _ptr(error_word), stream))
-    _check(lib, lib.srb_mx4_combine(_ptr(y), _ptr(entry_slot), _ptr(weights), rows, top, width, _ptr(out), stream))
+    tiles = min(entries, entries // tile + experts)
+    # one piece of memory: the plan, the row of every slot, the slot of every choice, and what the products need
+    plan_bytes, entry_bytes = _room(4 * moe.srb_moe_plan_ints_of(rows, top, experts, tile)), _room(4 * entries)
+    memory = torch.empty(plan_bytes + 2 * entry_bytes + needed(entries, tiles, experts, width, inner, gated), dtype=torch.uint8, device=h.device)
+    plan = memory.data_ptr()
+    slot_row, entry_slot, scratch = plan + plan_bytes, plan + plan_bytes + entry_bytes, plan + plan_bytes + 2 * entry_bytes
+    _check(moe, moe.srb_moe_plan_of(_P(chosen.data_ptr()), rows, top, experts, tile, _P(plan), _P(slot_row), _P(entry_slot), None, None,
+                                    _P(error_word.data_ptr()), stream if isinstance(stream, _P) else _P(stream)))
+    launches = 4 + int(gated and (many or inner % 128 != 0))
+    _check(lib, experts_of(h.data_ptr(), plan, slot_row, entry_slot, weights.data_ptr(), w_gate_up.codes.data_ptr(), w_gate_up.scales.data_ptr(),
+                           w_down.codes.data_ptr(), w_down.scales.data_ptr(), out.data_ptr(), rows, top, tiles, experts, width, inner, gated, act_code,
+                           activation_param, scratch, error_word.data_ptr(), stream), launches)
     return out
