@@ -354,8 +354,9 @@ template <bool PARTS, int MODE, bool GROUPED, int STAGES>
 static int launch_few_staged(const CUtensorMap (&maps)[4], const FewArgs& a, int blocks, cudaStream_t s) {
   using Shape = FewShape<MODE == MXF_GATED>;
   const size_t smem = 1024 + (size_t)STAGES * (Shape::stage_bytes(a.columns) + Shape::SCALE_BYTES);
+  static std::atomic<int> allowed[MX4_MAX_DEVICES];
   auto kernel = mx4_few_kernel<PARTS, MODE, GROUPED, STAGES>;
-  SRB_CUDA_CALL(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  if (const int status = mx4_allow_shared((const void*)kernel, (int)smem, allowed)) return status;
   SRB_CUDA_CALL(srb_launch_clustered(kernel, dim3(blocks), dim3(MXF_THREADS), smem, s, dim3(a.splits), maps[0], maps[1], maps[2], maps[3], a));
   return SRB_OK;
 }

@@ -399,8 +399,9 @@ static int launch_pair(const CUtensorMap (&maps)[5], const PairMx4Args& a, int m
   using Shape = PairShape<FOUR>;
   const int pairs = std::max(1, std::min(srb_sm_count() / 2, max_tiles));
   const size_t smem = (size_t)Shape::STAGES * Shape::STAGE_BYTES + MXP_EPILOGUE_WARPS * MXP_BOX_BYTES + 1024;
+  static std::atomic<int> allowed[MX4_MAX_DEVICES];
   auto kernel = mx4_pair_kernel<FOUR, MODE, GROUPED>;
-  SRB_CUDA_CALL(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  if (const int status = mx4_allow_shared((const void*)kernel, (int)smem, allowed)) return status;
   SRB_CUDA_CALL(srb_launch_clustered(kernel, dim3(2 * pairs), dim3(Shape::THREADS), smem, s, dim3(2), maps[0], maps[1], maps[2], maps[3], maps[4], a));
   return SRB_OK;
 }

@@ -16,100 +16,133 @@ SRB_DEFINE_PDL_SWITCH()
 
 #define MX4_THREADS 256
 
+// Eight entries a lane of 128 of a row, lane of 16.  Rows that do not start on 16-byte borders go through shared memory, so that neighbouring
+// lanes read and write neighbouring entries there too (5,171 rows of 2,891 floats: LATER).
+template <typename T, bool WIDE>
+__device__ __forceinline__ void mx4_read_eight(const T* __restrict__ src, int left, int lane, float (&v)[8]) {
+  if (WIDE && left >= 128) {
+    if (sizeof(T) == 2) mx4_unpack_bf16(reinterpret_cast<const uint4*>(src)[lane], v);
+    else {
+      const float4 a = reinterpret_cast<const float4*>(src)[2 * lane], b = reinterpret_cast<const float4*>(src)[2 * lane + 1];
+      v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+    }
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = lane + 16 * i < left ? srb_to_float(src[lane + 16 * i]) : 0.f;
+}
+// (behind mx4_read_eight, entries lane, lane + 16 ... become entries 8 lane, 8 lane + 1 ...)
+__device__ __forceinline__ void mx4_turn(float* staged, int lane, float (&v)[8]) {
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < 8; ++i) staged[lane + 16 * i] = v[i];
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = staged[8 * lane + i];
+}
+
+#define MX4_AT_ONCE 4            // column tiles of a row a thread takes: their loads are in flight together
+
 template <typename T, bool WIDE>
 __global__ void __launch_bounds__(MX4_THREADS)
 mx4_quantize_kernel(const T* __restrict__ x, size_t pitch, size_t matrix_pitch, int rows, int width, unsigned* __restrict__ codes,
                     unsigned* __restrict__ scales) {
+  __shared__ float staged[MX4_THREADS / 16][128 + 4];
   srb_launch_dependents();
   srb_grid_dependency_wait();
   const int k_tiles = mx4_tiles(width), row_tiles = mx4_tiles(rows);
-  const int lane = threadIdx.x & 15;                         // of the 16 that share 128 entries of a row
-  const long long item = (long long)blockIdx.x * (MX4_THREADS / 16) + (threadIdx.x >> 4);
-  const int row = (int)(item / k_tiles), kt = (int)(item % k_tiles), matrix = blockIdx.y;
-  const bool inside = row < row_tiles * 128, live = row < rows;
-  const int k = kt * 128 + lane * 8;
-  float v[8];
+  const int lane = threadIdx.x & 15, row = blockIdx.x * (MX4_THREADS / 16) + (threadIdx.x >> 4), kt0 = blockIdx.y * MX4_AT_ONCE, matrix = blockIdx.z;
+  const bool live = row < rows;
+  const T* src = x + (size_t)matrix * matrix_pitch + (size_t)row * pitch;
+  float v[MX4_AT_ONCE][8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = 0.f;
-  if (live) {
-    const T* src = x + (size_t)matrix * matrix_pitch + (size_t)row * pitch + k;
-    if (WIDE && k + 8 <= width) {
-      if (sizeof(T) == 2) mx4_unpack_bf16(*reinterpret_cast<const uint4*>(src), v);
-      else {
-        const float4 a = reinterpret_cast<const float4*>(src)[0], b = reinterpret_cast<const float4*>(src)[1];
-        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-      }
-    } else {
+  for (int j = 0; j < MX4_AT_ONCE; ++j)
+    mx4_read_eight<T, WIDE>(src + (kt0 + j) * 128, live ? width - (kt0 + j) * 128 : 0, lane, v[j]);
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (k + i < width) v[i] = srb_to_float(src[i]);
-    }
+  for (int j = 0; j < MX4_AT_ONCE; ++j) {
+    const int kt = kt0 + j;
+    if (kt >= k_tiles) break;
+    if (!WIDE || (kt + 1) * 128 > width) mx4_turn(staged[threadIdx.x >> 4], lane, v[j]);
+    // magnitudes as their bits: the largest bits are the largest magnitude, and whatever is not finite is above all that is
+    unsigned most = 0u;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) most = max(most, __float_as_uint(v[j][i]) & 0x7fffffffu);
+    most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
+    most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
+    const bool finite = most < 0x7f800000u;
+    const int exponent = max((int)(most >> 23) - 129, -127); // a subnormal's field is 0: the least scale
+    const unsigned s = finite ? (unsigned)(exponent + 127) : 255u;
+    const float inverse = __uint_as_float((unsigned)(127 - exponent) << 23);    // 2^-exponent, between 2^-125 and 2^127
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[j][i] = finite ? v[j][i] * inverse : 0.f;
+    const unsigned packed = mx4_pack_eight(v[j]);
+    // the scales of the four blocks, a byte each, in one word; blocks behind the row's end and rows behind the last get 127
+    unsigned word = (live && kt * 128 + (lane >> 2) * 32 < width ? s : 127u) << (8 * (lane >> 2));
+    word |= __shfl_xor_sync(0xffffffffu, word, 4);
+    word |= __shfl_xor_sync(0xffffffffu, word, 8);
+    if (live) codes[((size_t)matrix * rows + row) * (mx4_pitch(width) / 4) + kt * 16 + lane] = packed;
+    if (lane == 0) scales[((size_t)matrix * row_tiles * k_tiles * MX4_TILE_BYTES + mx4_scale_word(row, kt, k_tiles)) / 4] = word;
   }
-  // magnitudes as their bits: the largest bits are the largest magnitude, and whatever is not finite is above all that is
-  unsigned most = 0u;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) most = max(most, __float_as_uint(v[i]) & 0x7fffffffu);
-  most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
-  most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
-  const bool finite = most < 0x7f800000u;
-  const int exponent = max((int)(most >> 23) - 129, -127);   // a subnormal's field is 0: the least scale
-  const unsigned s = finite ? (unsigned)(exponent + 127) : 255u;
-  const float inverse = __uint_as_float((unsigned)(127 - exponent) << 23);      // 2^-exponent, between 2^-125 and 2^127
-#pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = finite ? v[i] * inverse : 0.f;
-  const unsigned packed = mx4_pack_eight(v);
-  // the scales of the four blocks, a byte each, in one word; blocks behind the row's end and rows behind the last get 127
-  unsigned word = live && kt * 128 + (lane >> 2) * 32 < width ? s : 127u;
-  word = (lane & 3) == 0 ? word << (8 * (lane >> 2)) : 0u;
-  word |= __shfl_xor_sync(0xffffffffu, word, 4);
-  word |= __shfl_xor_sync(0xffffffffu, word, 8);
-  if (!inside) return;
-  if (live) codes[((size_t)matrix * rows + row) * (mx4_pitch(width) / 4) + kt * 16 + lane] = packed;
-  if (lane == 0) scales[((size_t)matrix * row_tiles * k_tiles * MX4_TILE_BYTES + mx4_scale_word(row, kt, k_tiles)) / 4] = word;
 }
 
 template <typename T, bool WIDE>
 __global__ void __launch_bounds__(MX4_THREADS)
 mx4_dequantize_kernel(const unsigned* __restrict__ codes, const unsigned* __restrict__ scales, int rows, int width, T* __restrict__ out) {
+  __shared__ float staged[MX4_THREADS / 16][128 + 4];
   srb_launch_dependents();
   srb_grid_dependency_wait();
   const int k_tiles = mx4_tiles(width), row_tiles = mx4_tiles(rows);
-  const int lane = threadIdx.x & 15;
-  const long long item = (long long)blockIdx.x * (MX4_THREADS / 16) + (threadIdx.x >> 4);
-  const int row = (int)(item / k_tiles), kt = (int)(item % k_tiles), matrix = blockIdx.y;
-  if (row >= rows) return;
-  const unsigned packed = codes[((size_t)matrix * rows + row) * (mx4_pitch(width) / 4) + kt * 16 + lane];
-  const unsigned word = scales[((size_t)matrix * row_tiles * k_tiles * MX4_TILE_BYTES + mx4_scale_word(row, kt, k_tiles)) / 4];
-  const float scale = mx4_scale_value((word >> (8 * (lane >> 2))) & 255u);
-  const int k = kt * 128 + lane * 8;
-  T* dst = out + ((size_t)matrix * rows + row) * width + k;
-  float v[8];
+  const int lane = threadIdx.x & 15, row = blockIdx.x * (MX4_THREADS / 16) + (threadIdx.x >> 4), kt0 = blockIdx.y * MX4_AT_ONCE, matrix = blockIdx.z;
+  const bool live = row < rows;
+  unsigned packed[MX4_AT_ONCE], word[MX4_AT_ONCE];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = mx4_code_value((packed >> (4 * i)) & 15u) * scale;
-  if (WIDE && k + 8 <= width) {
-    if (sizeof(T) == 2) {
-      unsigned w[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const __nv_bfloat162 pair = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
-        w[i] = *reinterpret_cast<const unsigned*>(&pair);
-      }
-      *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
-    } else {
-      reinterpret_cast<float4*>(dst)[0] = make_float4(v[0], v[1], v[2], v[3]);
-      reinterpret_cast<float4*>(dst)[1] = make_float4(v[4], v[5], v[6], v[7]);
-    }
-    return;
+  for (int j = 0; j < MX4_AT_ONCE; ++j) {
+    const int kt = kt0 + j;
+    packed[j] = live && kt < k_tiles ? codes[((size_t)matrix * rows + row) * (mx4_pitch(width) / 4) + kt * 16 + lane] : 0u;
+    word[j] = live && kt < k_tiles ? scales[((size_t)matrix * row_tiles * k_tiles * MX4_TILE_BYTES + mx4_scale_word(row, kt, k_tiles)) / 4] : 0u;
   }
+  T* dst = out + ((size_t)matrix * rows + row) * width;
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
-    if (k + i < width) dst[i] = srb_from_float<T>(v[i]);
+  for (int j = 0; j < MX4_AT_ONCE; ++j) {
+    const int k = (kt0 + j) * 128;
+    if (k >= width) break;
+    const float scale = mx4_scale_value((word[j] >> (8 * (lane >> 2))) & 255u);
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) mx4_two_values((packed[j] >> (8 * i)) & 255u, v[2 * i], v[2 * i + 1]);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] *= scale;
+    if (WIDE && k + 128 <= width) {
+      if (!live) continue;
+      if (sizeof(T) == 2) {
+        unsigned w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const __nv_bfloat162 pair = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+          w[i] = *reinterpret_cast<const unsigned*>(&pair);
+        }
+        reinterpret_cast<uint4*>(dst + k)[lane] = make_uint4(w[0], w[1], w[2], w[3]);
+      } else {
+        reinterpret_cast<float4*>(dst + k)[2 * lane] = make_float4(v[0], v[1], v[2], v[3]);
+        reinterpret_cast<float4*>(dst + k)[2 * lane + 1] = make_float4(v[4], v[5], v[6], v[7]);
+      }
+    } else {
+      float* mine = staged[threadIdx.x >> 4];
+      __syncwarp();
+#pragma unroll
+      for (int i = 0; i < 8; ++i) mine[8 * lane + i] = v[i];
+      __syncwarp();
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (live && k + lane + 16 * i < width) dst[k + lane + 16 * i] = srb_from_float<T>(mine[lane + 16 * i]);
+    }
+  }
 }
 
-static int mx4_grid(int matrices, long long rows, int width, dim3* grid) {
-  const long long items = rows * mx4_tiles(width), blocks = (items + MX4_THREADS / 16 - 1) / (MX4_THREADS / 16);
-  if (blocks > 0x7fffffffll || matrices > 65535) SRB_FAIL("mx4: %d matrices of %lld rows of %d entries are too many", matrices, rows, width);
-  *grid = dim3((unsigned)blocks, (unsigned)matrices);
+static int mx4_grid(int matrices, int rows, int width, dim3* grid) {
+  const int row_blocks = (rows + MX4_THREADS / 16 - 1) / (MX4_THREADS / 16), k_blocks = (mx4_tiles(width) + MX4_AT_ONCE - 1) / MX4_AT_ONCE;
+  if (k_blocks > 65535 || matrices > 65535) SRB_FAIL("mx4: %d matrices of %d rows of %d entries are too many", matrices, rows, width);
+  *grid = dim3(row_blocks, k_blocks, matrices);
   return SRB_OK;
 }
 
@@ -117,8 +150,9 @@ static int mx4_grid(int matrices, long long rows, int width, dim3* grid) {
 extern "C" int srb_mx4_quantize(const void* x, long long pitch, long long matrix_pitch, int matrices, int rows, int width, void* codes,
                                 void* scales, int dtype, void* stream) {
   if (matrices <= 0 || rows <= 0 || width <= 0) return SRB_OK;
+  if (rows > 0x7fff0000) SRB_FAIL("mx4_quantize: %d rows are too many", rows);
   dim3 grid;
-  if (mx4_grid(matrices, (long long)mx4_tiles(rows) * 128, width, &grid) != SRB_OK) return SRB_ERR_INVALID;
+  if (mx4_grid(matrices, mx4_tiles(rows) * 128, width, &grid) != SRB_OK) return SRB_ERR_INVALID;
   const int element = dtype == SRB_DTYPE_F32 ? 4 : 2;
   const bool wide = ((uintptr_t)x & 15) == 0 && pitch * element % 16 == 0 && matrix_pitch * element % 16 == 0;
   cudaStream_t s = (cudaStream_t)stream;

@@ -8,6 +8,7 @@
 #pragma once
 #include "common.cuh"
 #include "tcgen05_helpers.cuh"
+#include <atomic>
 #include <mutex>
 
 #define MX_E4M3 0u
@@ -43,6 +44,20 @@ __device__ __forceinline__ void tmem_load_8(unsigned address, float (&v)[8]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
   for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(r[i]);
+}
+
+// Lets the kernel have that much shared memory, once for a device and a size (`allowed`: what a device was told last).
+#define MX4_MAX_DEVICES 64
+static inline int mx4_allow_shared(const void* kernel, int bytes, std::atomic<int>* allowed) {
+  int device = 0;
+  SRB_CUDA_CALL(cudaGetDevice(&device));
+  if (device < MX4_MAX_DEVICES && allowed[device].load() >= bytes) return SRB_OK;
+  SRB_CUDA_CALL(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  if (device < MX4_MAX_DEVICES) {
+    int told = allowed[device].load();
+    while (told < bytes && !allowed[device].compare_exchange_weak(told, bytes)) {}
+  }
+  return SRB_OK;
 }
 
 // ---- maps for TMA ----------------------------------------------------------------------------------------------------

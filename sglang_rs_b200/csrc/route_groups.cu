@@ -7,11 +7,12 @@
 //   choice  the `top` largest picks of open groups, largest first; ties go to the lower index, of groups and of experts
 //   weight  the chosen scores, divided by (their sum + norm_eps) if `renormalize`, times `scale`
 //
-// Which of two picks is larger may hang on their last bits, and a choice is whole numbers: the row is chosen in 32 bits, and once more in 64
-// where two neighbours in that order, or the last open group and the first closed one, are nearer than the 32-bit scores' error.
+// Which of two picks is larger may hang on their last bits, and a choice is whole numbers: it is that of 64-bit scores.  Where nothing is added to
+// the scores, their order is the logits' own and those are compared.  Otherwise the row is chosen by 32-bit scores, and once more by
+// 64-bit ones where two neighbours in that order, or the last open group and the first closed one, are nearer than the scores' error.
 //
-// A warp per row.  Picks lie in registers as unsigned numbers of the same order, so that a largest one of the warp is one instruction
-// (redux.sync) and its lowest index another.  Bound by instructions: about 700 a row of 256 experts.
+// A warp per row, expert lane + 32 j the lane's j-th.  Picks lie in registers as unsigned numbers of the same order, so that a largest one of the
+// warp is one instruction (redux.sync; two for 64 bits) and its lowest index another.  Bound by a row's chain of instructions: LATER.
 #include "common.cuh"
 #include <math.h>
 
@@ -31,187 +32,142 @@ struct GroupRule {
   float scale, norm_eps;
 };
 
-// numbers in the order of floats; 0 is below every float
+// Numbers in the order of the reals that they stand for; 0 is below all of them.
 __device__ __forceinline__ unsigned route_key(float v) {
   const unsigned u = __float_as_uint(v);
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 __device__ __forceinline__ float route_value(unsigned key) { return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key); }
+__device__ __forceinline__ unsigned long long route_key(double v) {
+  const unsigned long long u = (unsigned long long)__double_as_longlong(v);
+  return u >> 63 ? ~u : u | 0x8000000000000000ull;
+}
+__device__ __forceinline__ double route_value(unsigned long long key) {
+  return __longlong_as_double((long long)(key >> 63 ? key & 0x7fffffffffffffffull : ~key));
+}
+__device__ __forceinline__ unsigned route_most(unsigned key) { return __reduce_max_sync(ALL, key); }
+__device__ __forceinline__ unsigned long long route_most(unsigned long long key) {
+  const unsigned high = __reduce_max_sync(ALL, (unsigned)(key >> 32));
+  const unsigned low = __reduce_max_sync(ALL, (unsigned)(key >> 32) == high ? (unsigned)key : 0u);
+  return (unsigned long long)high << 32 | low;
+}
+template <typename R> struct RouteKey { typedef unsigned Type; };
+template <> struct RouteKey<double> { typedef unsigned long long Type; };
 
-__device__ __forceinline__ double route_max(double v) {
+__device__ __forceinline__ float route_exp(float v) { return expf(v); }
+__device__ __forceinline__ double route_exp(double v) { return exp(v); }
+__device__ __forceinline__ double route_sum(double v) {
 #pragma unroll
-  for (int offset = 16; offset > 0; offset >>= 1) v = fmax(v, __shfl_xor_sync(ALL, v, offset));
+  for (int offset = 16; offset > 0; offset >>= 1) v += __shfl_xor_sync(ALL, v, offset);
   return v;
 }
+__device__ __forceinline__ float route_sum(float v) { return srb_warp_sum(v); }
 
-// The row in 64 bits; `picks` is shared memory for its experts.  The lane k < top returns the k-th choice.
-__device__ __noinline__ int route_exactly(const float* z, const float* bias, const GroupRule& rule, double* picks, int lane) {
-  double most = -INFINITY, sum = 0.0;
-  if (rule.scoring == ROUTE_SOFTMAX) {
-    for (int e = lane; e < rule.experts; e += 32) most = fmax(most, (double)z[e]);
-    most = route_max(most);
-    for (int e = lane; e < rule.experts; e += 32) sum += exp((double)z[e] - most);
-#pragma unroll
-    for (int offset = 16; offset > 0; offset >>= 1) sum += __shfl_xor_sync(ALL, sum, offset);
-  }
-  for (int e = lane; e < rule.experts; e += 32) {
-    const double s = rule.scoring == ROUTE_SOFTMAX ? exp((double)z[e] - most) / sum : 1.0 / (1.0 + exp(-(double)z[e]));
-    const double pick = bias ? s + (double)bias[e] : s;
-    picks[e] = pick == pick ? pick : -INFINITY;
-  }
-  __syncwarp();
-  const int per_group = rule.experts / rule.groups;
-  unsigned open = ALL;
-  if (rule.groups > rule.top_groups) {
-    double mine = -INFINITY;                                 // the score of group `lane`
-    if (lane < rule.groups) {
-      double first = -INFINITY, second = -INFINITY;
-      for (int i = 0; i < per_group; ++i) {
-        const double v = picks[lane * per_group + i];
-        if (v > first) { second = first; first = v; }
-        else if (v > second) second = v;
-      }
-      mine = rule.group_best == 2 ? first + second : first;
-      if (mine != mine) mine = -INFINITY;
-    }
-    bool left = lane < rule.groups;
-    open = 0;
-    for (int k = 0; k < rule.top_groups; ++k) {
-      const double best = route_max(left ? mine : -INFINITY);
-      const int g = __ffs(__ballot_sync(ALL, left && mine == best)) - 1;
-      open |= 1u << g;
-      left = left && lane != g;
-    }
-  }
-  int choice = 0;
-  for (int k = 0; k < rule.top; ++k) {
-    double best = -INFINITY;
-    int index = 0x7fffffff;
-    for (int e = lane; e < rule.experts; e += 32) {
-      const double v = picks[e];
-      // a taken one is not a number
-      if (v == v && ((open >> (e / per_group)) & 1u) && (v > best || index == 0x7fffffff)) { best = v; index = e; }
-    }
-    const double most_left = route_max(best);
-    const int e = (int)__reduce_min_sync(ALL, best == most_left ? (unsigned)index : 0x7fffffffu);
-    if (lane == k) choice = e;
-    if (lane == 0) picks[e] = __longlong_as_double(0x7ff8000000000000ll);
-    __syncwarp();
-  }
-  return choice;
-}
-
-// The scores' relative error in 32 bits is below 2^-19 (the argument of a softmax's exponential is rounded: 2^-24 times its size, which
-// is below 24 where the score is above 2^-34; smaller picks are always looked at in 64 bits).
-__device__ __forceinline__ bool route_near(float above, float below, float bias_most) {
-  const float room = (fabsf(above) + fabsf(below) + 2.f * bias_most) * 1.9073486e-6f;
+// Whether 32-bit numbers do not tell which of two picks (or sums of two) is larger, `above` being the larger one of them.  `by_logit`: they are the logits
+// themselves, whose order is that of the scores but where the 64-bit scores are alike: both 0, or sigmoids within 2^-53 of 1.  Otherwise
+// they are off by 2^-21 of the scores that went in, or, in a softmax, 2^-19: its exponential's argument is off by 2^-24 of its size,
+// which is below 24 where the score is above 2^-34; smaller picks always count as near.
+__device__ __forceinline__ bool route_near(float above, float below, float bias_most, float most, bool by_logit, int scoring) {
+  if (by_logit) return !(below - (scoring == ROUTE_SOFTMAX ? most : 0.f) > -700.f) || (scoring == ROUTE_SIGMOID && above > 16.f && above - below < 1.f && above != below);
+  const float room = (fabsf(above) + fabsf(below) + 2.f * bias_most) * (scoring == ROUTE_SOFTMAX ? 1.9073486e-6f : 4.7683716e-7f);
   return !(above - below > room) || (bias_most == 0.f && below < 5.8207661e-11f);
 }
 
-// PER experts a lane: expert lane + 32 j is the lane's j-th.
-template <int PER>
-__global__ void __launch_bounds__(32 * ROUTE_WARPS)
-route_groups_kernel(const float* __restrict__ logits, size_t pitch, int rows, const float* __restrict__ bias, GroupRule rule,
-                    int* __restrict__ chosen, float* __restrict__ weights) {
-  extern __shared__ double route_shared[];                   // [warps][experts]
-  srb_launch_dependents();
-  srb_grid_dependency_wait();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int row = blockIdx.x * ROUTE_WARPS + warp;
-  if (row >= rows) return;
-  double* shared = route_shared + (size_t)warp * rule.experts;
-  const float* z = logits + (size_t)row * pitch;
-  float score[PER];
-  float most = -INFINITY;
-#pragma unroll
-  for (int j = 0; j < PER; ++j) {
-    score[j] = lane + 32 * j < rule.experts ? z[lane + 32 * j] : -INFINITY;
-    most = fmaxf(most, score[j]);
-  }
-  float sum = 1.f;
-  if (rule.scoring == ROUTE_SOFTMAX) {
-    most = route_value(__reduce_max_sync(ALL, route_key(most)));
-    sum = 0.f;
-#pragma unroll
-    for (int j = 0; j < PER; ++j) {
-      score[j] = expf(score[j] - most);
-      if (lane + 32 * j < rule.experts) sum += score[j];
-    }
-    sum = srb_warp_sum(sum);
-    const float inverse = 1.0f / sum;
-#pragma unroll
-    for (int j = 0; j < PER; ++j) score[j] *= inverse;
-  } else {
-#pragma unroll
-    for (int j = 0; j < PER; ++j) score[j] = 1.0f / (1.0f + expf(-score[j]));
-  }
-  unsigned key[PER];
+// The lane k < top gets the k-th choice.  R: the scores' type; in 32 bits the choice holds unless `near`.  `most` and `sum`: of a softmax, in R.  `shared`:
+// room for a key of every expert.
+template <int PER, typename R>
+__device__ __forceinline__ int route_choose(const float (&z)[PER], const float* __restrict__ bias, const GroupRule& rule, R most, R sum, bool by_logit,
+                                            void* shared, int lane, bool& near) {
+  typedef typename RouteKey<R>::Type Key;
+  constexpr bool CHECK = sizeof(R) == 4;
+  Key key[PER];
   float bias_most = 0.f;
 #pragma unroll
   for (int j = 0; j < PER; ++j) {
     const int e = lane + 32 * j;
-    float pick = score[j];
+    R pick = (R)z[j];
+    if (!by_logit) pick = rule.scoring == ROUTE_SOFTMAX ? route_exp(pick - most) / sum : (R)1 / ((R)1 + route_exp(-pick));
     if (bias && e < rule.experts) {
-      const float b = bias[e];
+      const float b = __ldg(bias + e);
       bias_most = fmaxf(bias_most, fabsf(b));
-      pick += b;
+      pick += (R)b;
     }
-    key[j] = e < rule.experts ? route_key(pick == pick ? pick : -INFINITY) : 0u;
+    key[j] = e < rule.experts ? route_key(pick == pick ? pick : (R)-INFINITY) : (Key)0;
   }
-  if (bias) bias_most = __uint_as_float(__reduce_max_sync(ALL, __float_as_uint(bias_most)));
-  bool near = false;
+  if (CHECK && bias) bias_most = __uint_as_float(__reduce_max_sync(ALL, __float_as_uint(bias_most)));
+  near = false;
   if (rule.groups > rule.top_groups) {
     const int per_group = rule.experts / rule.groups;
-    unsigned* picks = reinterpret_cast<unsigned*>(shared);
+    const bool whole = per_group % 32 == 0;                  // a group is some of the registers, of all lanes
+    Key* picks = reinterpret_cast<Key*>(shared);
+    if (!whole) {
 #pragma unroll
-    for (int j = 0; j < PER; ++j)
-      if (lane + 32 * j < rule.experts) picks[lane + 32 * j] = key[j];
-    __syncwarp();
-    unsigned mine = 0u;                                      // the score of group `lane`
-    for (int g = 0; g < rule.groups; ++g) {
-      unsigned first = 0u, second = 0u;
-      for (int i = lane; i < per_group; i += 32) {
-        const unsigned v = picks[g * per_group + i];
-        second = max(second, min(first, v));
-        first = max(first, v);
-      }
-      const unsigned best = __reduce_max_sync(ALL, first);
-      float group = route_value(best);
+      for (int j = 0; j < PER; ++j)
+        if (lane + 32 * j < rule.experts) picks[lane + 32 * j] = key[j];
+      __syncwarp();
+    }
+    Key mine = 0;                                            // the score of group `lane`
+    auto score_group = [&](int g, Key first, Key second) {
+      const Key best = route_most(first);
+      R group = route_value(best);
       if (rule.group_best == 2) {
         const int owner = __ffs(__ballot_sync(ALL, first == best)) - 1;
-        group += route_value(__reduce_max_sync(ALL, lane == owner ? second : first));
+        group += route_value(route_most(lane == owner ? second : first));
       }
-      if (lane == g) mine = route_key(group == group ? group : -INFINITY);
+      if (lane == g) mine = route_key(group == group ? group : (R)-INFINITY);
+    };
+    if (whole) {
+      const int registers = per_group / 32;
+      Key first = 0, second = 0;
+#pragma unroll
+      for (int j = 0; j < PER; ++j) {
+        second = max(second, min(first, key[j]));
+        first = max(first, key[j]);
+        if ((j + 1) % registers == 0) {
+          if (j / registers < rule.groups) score_group(j / registers, first, second);
+          first = second = 0;
+        }
+      }
+    } else {
+      for (int g = 0; g < rule.groups; ++g) {
+        Key first = 0, second = 0;
+        for (int i = lane; i < per_group; i += 32) {
+          const Key v = picks[g * per_group + i];
+          second = max(second, min(first, v));
+          first = max(first, v);
+        }
+        score_group(g, first, second);
+      }
     }
     unsigned open = 0u;
-    float last = 0.f;
-    for (int k = 0; k <= rule.top_groups; ++k) {
-      const unsigned best = __reduce_max_sync(ALL, mine);
-      const float value = route_value(best);
+    R last = 0;
+    for (int k = 0; k < rule.top_groups + (CHECK ? 1 : 0); ++k) {
+      const Key best = route_most(mine);
+      const R value = route_value(best);
       if (k == rule.top_groups) {
-        near = route_near(last, value, 2.f * bias_most);
+        near = route_near((float)last, (float)value, 2.f * bias_most, (float)most, by_logit, rule.scoring);
         break;
       }
       const int g = __ffs(__ballot_sync(ALL, mine == best)) - 1;
       open |= 1u << g;
-      if (lane == g) mine = 0u;
+      if (lane == g) mine = 0;
       last = value;
     }
 #pragma unroll
     for (int j = 0; j < PER; ++j)
-      if (lane + 32 * j < rule.experts && !((open >> ((lane + 32 * j) / per_group)) & 1u)) key[j] = 0u;
+      if (lane + 32 * j < rule.experts && !((open >> ((lane + 32 * j) / per_group)) & 1u)) key[j] = 0;
     __syncwarp();
   }
   int choice = 0;
-  float last = 0.f;
-  for (int k = 0; k <= rule.top && !near; ++k) {
-    unsigned mine = 0u;
+  R last = 0;
+  for (int k = 0; k < rule.top + (CHECK ? 1 : 0); ++k) {
+    Key mine = 0;
 #pragma unroll
     for (int j = 0; j < PER; ++j) mine = max(mine, key[j]);
-    const unsigned best = __reduce_max_sync(ALL, mine);
-    if (best == 0u) break;                                   // all are taken
-    const float value = route_value(best);
-    if (k > 0) near = route_near(last, value, bias_most);
+    const Key best = route_most(mine);
+    if (best == 0) break;                                    // all are taken
+    const R value = route_value(best);
+    if (CHECK && k > 0) near |= route_near((float)last, (float)value, bias_most, (float)most, by_logit, rule.scoring);
     last = value;
     if (k == rule.top) break;
     unsigned index = 0x7fffffffu;
@@ -221,14 +177,66 @@ route_groups_kernel(const float* __restrict__ logits, size_t pitch, int rows, co
     index = __reduce_min_sync(ALL, index);
 #pragma unroll
     for (int j = 0; j < PER; ++j)
-      if (index == (unsigned)(lane + 32 * j)) key[j] = 0u;
+      if (index == (unsigned)(lane + 32 * j)) key[j] = 0;
     if (lane == k) choice = (int)index;
   }
-  if (near) choice = route_exactly(z, bias, rule, shared, lane);
-  // the chosen scores once more, a lane each
+  return choice;
+}
+
+template <int PER>
+__device__ __noinline__ int route_choose_exactly(const float* row, const float* bias, const GroupRule& rule, void* shared, int lane) {
+  float z[PER];
+  double most = -INFINITY, sum = 0.0;
+#pragma unroll
+  for (int j = 0; j < PER; ++j) {
+    z[j] = lane + 32 * j < rule.experts ? row[lane + 32 * j] : -INFINITY;
+    most = fmax(most, (double)z[j]);
+  }
+  if (rule.scoring == ROUTE_SOFTMAX) {
+    most = route_value(route_most(route_key(most)));
+#pragma unroll
+    for (int j = 0; j < PER; ++j)
+      if (lane + 32 * j < rule.experts) sum += exp((double)z[j] - most);
+    sum = route_sum(sum);
+  }
+  bool near;
+  return route_choose<PER, double>(z, bias, rule, most, sum, false, shared, lane, near);
+}
+
+template <int PER>
+__global__ void __launch_bounds__(32 * ROUTE_WARPS)
+route_groups_kernel(const float* __restrict__ logits, size_t pitch, int rows, const float* __restrict__ bias, GroupRule rule,
+                    int* __restrict__ chosen, float* __restrict__ weights) {
+  extern __shared__ unsigned long long route_shared[];       // [warps][experts]
+  srb_launch_dependents();
+  srb_grid_dependency_wait();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int row = blockIdx.x * ROUTE_WARPS + warp;
+  if (row >= rows) return;
+  unsigned long long* shared = route_shared + (size_t)warp * rule.experts;
+  const float* from = logits + (size_t)row * pitch;
+  float z[PER];
+  float most = -INFINITY, sum = 0.f;
+#pragma unroll
+  for (int j = 0; j < PER; ++j) {
+    z[j] = lane + 32 * j < rule.experts ? from[lane + 32 * j] : -INFINITY;
+    most = fmaxf(most, z[j]);
+  }
+  if (rule.scoring == ROUTE_SOFTMAX) {
+    most = route_value(route_most(route_key(most)));
+#pragma unroll
+    for (int j = 0; j < PER; ++j)
+      if (lane + 32 * j < rule.experts) sum += expf(z[j] - most);
+    sum = route_sum(sum);
+  }
+  const bool by_logit = !bias && (rule.group_best == 1 || rule.groups == rule.top_groups);
+  bool near;
+  int choice = route_choose<PER, float>(z, bias, rule, most, sum, by_logit, shared, lane, near);
+  // (a softmax over something that is not finite has no scores)
+  if (near || (rule.scoring == ROUTE_SOFTMAX && !(sum < INFINITY))) choice = route_choose_exactly<PER>(from, bias, rule, shared, lane);
+  // the chosen scores, a lane each
   float weight = 0.f;
-  if (lane < rule.top)
-    weight = rule.scoring == ROUTE_SOFTMAX ? expf(z[choice] - most) / sum : 1.0f / (1.0f + expf(-z[choice]));
+  if (lane < rule.top) weight = rule.scoring == ROUTE_SOFTMAX ? expf(from[choice] - most) / sum : 1.0f / (1.0f + expf(-from[choice]));
   if (rule.renormalize) weight /= srb_warp_sum(weight) + rule.norm_eps;
   if (lane < rule.top) {
     chosen[(size_t)row * rule.top + lane] = choice;
@@ -239,7 +247,6 @@ route_groups_kernel(const float* __restrict__ logits, size_t pitch, int rows, co
 extern "C" int srb_route_groups(const float* logits, long long pitch, int rows, int experts, const float* bias, int top, int groups,
                                 int top_groups, int group_best, int scoring, int renormalize, float scale, float norm_eps, int* chosen,
                                 float* weights, void* stream) {
-  if (rows <= 0) return SRB_OK;
   if (experts <= 0 || experts > ROUTE_MAX_EXPERTS) SRB_FAIL("route_groups: %d experts are outside 1 .. %d", experts, ROUTE_MAX_EXPERTS);
   if (groups <= 0 || groups > ROUTE_MAX_GROUPS || experts % groups) SRB_FAIL("route_groups: %d experts in %d groups", experts, groups);
   if (top_groups <= 0 || top_groups > groups) SRB_FAIL("route_groups: %d open groups of %d", top_groups, groups);
@@ -249,10 +256,10 @@ extern "C" int srb_route_groups(const float* logits, long long pitch, int rows, 
     SRB_FAIL("route_groups: %d chosen experts are outside 1 .. min(%d, %d)", top, experts / groups * top_groups, ROUTE_MAX_TOP);
   if (scoring != ROUTE_SOFTMAX && scoring != ROUTE_SIGMOID) SRB_FAIL("route_groups: unknown scoring %d", scoring);
   if (pitch < experts) SRB_FAIL("route_groups: rows of the logits overlap");
+  if (rows <= 0) return SRB_OK;
   const GroupRule rule{experts, top, groups, top_groups, group_best, scoring, renormalize, scale, norm_eps};
   auto kernel = experts <= 64 ? route_groups_kernel<2> : experts <= 256 ? route_groups_kernel<8> : route_groups_kernel<32>;
   SRB_CUDA_CALL(srb_launch(kernel, dim3((rows + ROUTE_WARPS - 1) / ROUTE_WARPS), dim3(32 * ROUTE_WARPS), (size_t)ROUTE_WARPS * experts * 8,
                            (cudaStream_t)stream, logits, (size_t)pitch, rows, bias, rule, chosen, weights));
-  SRB_LAUNCH_CHECK("route_groups");
   return SRB_OK;
 }

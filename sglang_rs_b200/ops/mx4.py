@@ -78,6 +78,13 @@ class Mx4:
     scales: torch.Tensor
     width: int
 
+    @classmethod
+    def _made(cls, codes: torch.Tensor, scales: torch.Tensor, width: int) -> "Mx4":
+        """One whose tensors were allocated here, without looking at them again."""
+        q = object.__new__(cls)
+        q.__dict__.update(codes=codes, scales=scales, width=width)
+        return q
+
     def __post_init__(self):
         codes, scales = self.codes, self.scales
         if (not isinstance(codes, torch.Tensor) or not isinstance(scales, torch.Tensor) or codes.dtype != torch.uint8 or scales.dtype != torch.uint8
@@ -165,8 +172,8 @@ def quantize_mx4(x: torch.Tensor) -> Mx4:
     *lead, rows, width = x.shape
     if width == 0:
         raise KernelError("quantize_mx4: rows without entries")
-    q = Mx4(torch.empty((*lead, rows, 64 * _tiles(width)), dtype=torch.uint8, device=x.device),
-            torch.empty((*lead, _tiles(rows), _tiles(width), 512), dtype=torch.uint8, device=x.device), width)
+    q = Mx4._made(x.new_empty((*lead, rows, 64 * _tiles(width)), dtype=torch.uint8),
+                  x.new_empty((*lead, _tiles(rows), _tiles(width), 512), dtype=torch.uint8), width)
     if x.numel():
         lib = _library("mx4")
         _check(lib, lib.srb_mx4_quantize(x.data_ptr(), x.stride(-2), x.stride(0) if lead else 0, lead[0] if lead else 1, rows, width,
@@ -180,7 +187,7 @@ def dequantize_mx4(q: Mx4, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     _need_mx4(q, "q", None)
     code = dtype_code(dtype)
     _here("dequantize_mx4", q.codes, q.scales)
-    out = torch.empty(q.shape, dtype=dtype, device=q.device)
+    out = q.codes.new_empty(q.shape, dtype=dtype)
     if out.numel():
         lib = _library("mx4")
         _check(lib, lib.srb_mx4_dequantize(q.codes.data_ptr(), q.scales.data_ptr(), q.matrices or 1, q.rows, q.width, out.data_ptr(), code, _stream()))
@@ -217,12 +224,12 @@ def linear_mx4(x, weight: Mx4, error_word: torch.Tensor, *, bias: Optional[torch
     many = rows > MX4_FEW_ROWS
     # the kernel for many rows stores rows that start on 16-byte borders
     pitch = -(-weight.rows // 8) * 8 if many else weight.rows
-    out = torch.empty((rows, pitch), dtype=out_dtype, device=weight.device)
+    out = weight.codes.new_empty((rows, pitch), dtype=out_dtype)
     if out.numel():
         lib = _library("gemm_mx4_pair" if many else "gemm_mx4")
         product, needed = (lib.srb_mx4_linear_pair, lib.srb_mx4_linear_pair_scratch) if many else (lib.srb_mx4_linear, lib.srb_mx4_linear_scratch)
         held = x.codes if four else x
-        scratch = None if four else torch.empty(needed(rows, width), dtype=torch.uint8, device=weight.device)
+        scratch = None if four else weight.codes.new_empty(needed(rows, width))
         _check(lib, product(held.data_ptr(), held.stride(0), x.scales.data_ptr() if four else None, weight.codes.data_ptr(), weight.scales.data_ptr(),
                             None if bias is None else bias.data_ptr(), out.data_ptr(), pitch, rows, weight.rows, width,
                             out_dtype == torch.float32, None if four else scratch.data_ptr(), error_word.data_ptr(), _stream()), 1 if four else 2)
@@ -252,8 +259,7 @@ def choose_experts(logits: torch.Tensor, top: int, renormalize: bool = False, *,
     if top < 0 or top > 2**31 - 1 or rows * max(top, 1) >= 2**31:
         raise KernelError(f"choose_experts: {rows} rows of {top} choices")
     _here("choose_experts", logits, choice_bias)
-    chosen = torch.empty((rows, top), dtype=torch.int32, device=logits.device)
-    weights = torch.empty((rows, top), dtype=torch.float32, device=logits.device)
+    chosen, weights = logits.new_empty((rows, top), dtype=torch.int32), logits.new_empty((rows, top))
     lib = _library("route_groups")
     _check(lib, lib.srb_route_groups(logits.data_ptr(), logits.stride(0), rows, experts, None if choice_bias is None else choice_bias.data_ptr(), top,
                                      groups, top_groups, group_best, ROUTER_SCORING[scoring], renormalize, weight_scale, norm_eps, chosen.data_ptr(),
@@ -286,7 +292,7 @@ def chosen_experts_mx4(h: torch.Tensor, chosen: torch.Tensor, weights: torch.Ten
     _here("chosen_experts_mx4", h, chosen, weights, w_gate_up.codes, w_gate_up.scales, w_down.codes, w_down.scales, error_word)
     if rows == 0 or top == 0:
         return torch.zeros((rows, width), dtype=torch.bfloat16, device=h.device)
-    out = torch.empty((rows, width), dtype=torch.bfloat16, device=h.device)
+    out = torch.empty_like(h)
     entries, stream = rows * top, _stream()
     # (the pairs' result rows start on 16-byte borders)
     many = entries > MX4_FEW_CHOICES * experts and width % 4 == 0
