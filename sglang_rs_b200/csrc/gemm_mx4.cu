@@ -316,8 +316,10 @@ mx4_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
     srb_cluster_sync();
     const FewTile t = few_tile<GROUPED>(a, first_item);
     if (warp >= 2 && abort_flag == 0) {
-      // four features of a row a thread, from all blocks at once
-      for (int i = rank + a.splits * ((int)threadIdx.x - 64); i < t.count * 32; i += a.splits * MXF_EPILOGUE_THREADS) {
+      // four features of a row a thread, from all blocks at once; a block adds up a run of them (every a.splits-th in turn, a warp's 16 bytes
+      // lay 128 bytes apart, all in the same banks: 48 rows of 4,096 through 4,096 features in 8 parts took 14.6 us instead of 10.7)
+      const int share = (t.count * 32 + a.splits - 1) / a.splits, end = min((rank + 1) * share, t.count * 32);
+      for (int i = rank * share + (int)threadIdx.x - 64; i < end; i += MXF_EPILOGUE_THREADS) {
         float4 part[MXF_MAX_SPLITS];
 #pragma unroll
         for (int r = 0; r < MXF_MAX_SPLITS; ++r)
@@ -373,8 +375,8 @@ static int launch_few(const void* x, const void* x_scales, long long x_rows, con
   if (make_bytes_map(&maps[0], w, w_rows, a.k_tiles * 64ll, 128) != SRB_OK || make_scales_map(&maps[1], w_scales, ws_tiles, 2) != SRB_OK ||
       make_bytes_map(&maps[2], x, x_rows, a.k_tiles * 64ll, a.columns) != SRB_OK || make_scales_map(&maps[3], x_scales, x_tiles, 2) != SRB_OK)
     return SRB_ERR_INVALID;
-  // K in parts until there is about a block an SM: a block costs 5 us beside its steps, and adding up costs more the more blocks and rows there
-  // are (1 row of 4,096 through 4,096 features in 1, 2, 4 and 8 parts: 8.3, 7.1, 6.2 and 6.1 us; 48 rows 11.0, 9.6, 9.2 and 14.6)
+  // K in parts until there is about a block an SM: a block costs some 3 us beside its steps (8 rows of 4,096 through 4,096 features, 32 tiles, in 1, 2, 4
+  // and 8 parts: 9.0, 7.6, 6.6 and 7.8 us; of 12,288 18.0, 12.1, 9.8 and 9.5; one row through 24,576, 192 tiles, in 1, 2 and 4: 13.8, 16.2 and 19.0)
   const long long room = 2ll * srb_sm_count(), all_steps = (a.k_tiles + 1) / 2;
   a.splits = GROUPED ? 1 : (int)std::max(1ll, std::min(std::min<long long>(room / 2 / items, MXF_MAX_SPLITS), all_steps));
   const int blocks = (int)(a.splits > 1 ? items * a.splits : std::min(items, room));

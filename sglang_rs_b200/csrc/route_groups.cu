@@ -30,6 +30,8 @@ SRB_DEFINE_PDL_SWITCH()
 struct GroupRule {
   int experts, top, groups, top_groups, group_best, scoring, renormalize;
   float scale, norm_eps;
+  int per_group;
+  unsigned group_factor;         // e * group_factor >> 20 is e / per_group, for e < 1024
 };
 
 // Numbers in the order of the reals that they stand for; 0 is below all of them.
@@ -56,6 +58,9 @@ template <> struct RouteKey<double> { typedef unsigned long long Type; };
 
 __device__ __forceinline__ float route_exp(float v) { return expf(v); }
 __device__ __forceinline__ double route_exp(double v) { return exp(v); }
+// 1 / v, in 32 bits to 2 units of the last place
+__device__ __forceinline__ float route_over(float v) { return __fdividef(1.0f, v); }
+__device__ __forceinline__ double route_over(double v) { return 1.0 / v; }
 __device__ __forceinline__ double route_sum(double v) {
 #pragma unroll
   for (int offset = 16; offset > 0; offset >>= 1) v += __shfl_xor_sync(ALL, v, offset);
@@ -65,11 +70,11 @@ __device__ __forceinline__ float route_sum(float v) { return srb_warp_sum(v); }
 
 // Whether 32-bit numbers do not tell which of two picks (or sums of two) is larger, `above` being the larger one of them.  `by_logit`: they are the logits
 // themselves, whose order is that of the scores but where the 64-bit scores are alike: both 0, or sigmoids within 2^-53 of 1.  Otherwise
-// they are off by 2^-21 of the scores that went in, or, in a softmax, 2^-19: its exponential's argument is off by 2^-24 of its size,
+// they are off by 2^-20 of the scores that went in, or, in a softmax, 2^-19: its exponential's argument is off by 2^-24 of its size,
 // which is below 24 where the score is above 2^-34; smaller picks always count as near.
 __device__ __forceinline__ bool route_near(float above, float below, float bias_most, float most, bool by_logit, int scoring) {
   if (by_logit) return !(below - (scoring == ROUTE_SOFTMAX ? most : 0.f) > -700.f) || (scoring == ROUTE_SIGMOID && above > 16.f && above - below < 1.f && above != below);
-  const float room = (fabsf(above) + fabsf(below) + 2.f * bias_most) * (scoring == ROUTE_SOFTMAX ? 1.9073486e-6f : 4.7683716e-7f);
+  const float room = (fabsf(above) + fabsf(below) + 2.f * bias_most) * (scoring == ROUTE_SOFTMAX ? 1.9073486e-6f : 9.5367432e-7f);
   return !(above - below > room) || (bias_most == 0.f && below < 5.8207661e-11f);
 }
 
@@ -82,11 +87,12 @@ __device__ __forceinline__ int route_choose(const float (&z)[PER], const float* 
   constexpr bool CHECK = sizeof(R) == 4;
   Key key[PER];
   float bias_most = 0.f;
+  const R over_sum = (R)1 / sum;
 #pragma unroll
   for (int j = 0; j < PER; ++j) {
     const int e = lane + 32 * j;
     R pick = (R)z[j];
-    if (!by_logit) pick = rule.scoring == ROUTE_SOFTMAX ? route_exp(pick - most) / sum : (R)1 / ((R)1 + route_exp(-pick));
+    if (!by_logit) pick = rule.scoring == ROUTE_SOFTMAX ? route_exp(pick - most) * over_sum : route_over((R)1 + route_exp(-pick));
     if (bias && e < rule.experts) {
       const float b = __ldg(bias + e);
       bias_most = fmaxf(bias_most, fabsf(b));
@@ -97,7 +103,7 @@ __device__ __forceinline__ int route_choose(const float (&z)[PER], const float* 
   if (CHECK && bias) bias_most = __uint_as_float(__reduce_max_sync(ALL, __float_as_uint(bias_most)));
   near = false;
   if (rule.groups > rule.top_groups) {
-    const int per_group = rule.experts / rule.groups;
+    const int per_group = rule.per_group;
     const bool whole = per_group % 32 == 0;                  // a group is some of the registers, of all lanes
     Key* picks = reinterpret_cast<Key*>(shared);
     if (!whole) {
@@ -117,15 +123,16 @@ __device__ __forceinline__ int route_choose(const float (&z)[PER], const float* 
       if (lane == g) mine = route_key(group == group ? group : (R)-INFINITY);
     };
     if (whole) {
-      const int registers = per_group / 32;
+      int g = 0, end = per_group;
       Key first = 0, second = 0;
 #pragma unroll
       for (int j = 0; j < PER; ++j) {
         second = max(second, min(first, key[j]));
         first = max(first, key[j]);
-        if ((j + 1) % registers == 0) {
-          if (j / registers < rule.groups) score_group(j / registers, first, second);
+        if (32 * (j + 1) == end) {
+          score_group(g++, first, second);
           first = second = 0;
+          end = g < rule.groups ? end + per_group : 0;
         }
       }
     } else {
@@ -155,7 +162,7 @@ __device__ __forceinline__ int route_choose(const float (&z)[PER], const float* 
     }
 #pragma unroll
     for (int j = 0; j < PER; ++j)
-      if (lane + 32 * j < rule.experts && !((open >> ((lane + 32 * j) / per_group)) & 1u)) key[j] = 0;
+      if (lane + 32 * j < rule.experts && !((open >> ((unsigned)(lane + 32 * j) * rule.group_factor >> 20)) & 1u)) key[j] = 0;
     __syncwarp();
   }
   int choice = 0;
@@ -204,7 +211,7 @@ __device__ __noinline__ int route_choose_exactly(const float* row, const float* 
 }
 
 template <int PER>
-__global__ void __launch_bounds__(32 * ROUTE_WARPS)
+__global__ void __launch_bounds__(32 * ROUTE_WARPS, PER <= 8 ? 8 : 1)
 route_groups_kernel(const float* __restrict__ logits, size_t pitch, int rows, const float* __restrict__ bias, GroupRule rule,
                     int* __restrict__ chosen, float* __restrict__ weights) {
   extern __shared__ unsigned long long route_shared[];       // [warps][experts]
@@ -257,7 +264,8 @@ extern "C" int srb_route_groups(const float* logits, long long pitch, int rows, 
   if (scoring != ROUTE_SOFTMAX && scoring != ROUTE_SIGMOID) SRB_FAIL("route_groups: unknown scoring %d", scoring);
   if (pitch < experts) SRB_FAIL("route_groups: rows of the logits overlap");
   if (rows <= 0) return SRB_OK;
-  const GroupRule rule{experts, top, groups, top_groups, group_best, scoring, renormalize, scale, norm_eps};
+  const int per_group = experts / groups;
+  const GroupRule rule{experts, top, groups, top_groups, group_best, scoring, renormalize, scale, norm_eps, per_group, (1u << 20) / per_group + 1u};
   auto kernel = experts <= 64 ? route_groups_kernel<2> : experts <= 256 ? route_groups_kernel<8> : route_groups_kernel<32>;
   SRB_CUDA_CALL(srb_launch(kernel, dim3((rows + ROUTE_WARPS - 1) / ROUTE_WARPS), dim3(32 * ROUTE_WARPS), (size_t)ROUTE_WARPS * experts * 8,
                            (cudaStream_t)stream, logits, (size_t)pitch, rows, bias, rule, chosen, weights));

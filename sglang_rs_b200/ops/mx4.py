@@ -19,10 +19,15 @@ from .trace import traced
 
 #: entries of a row that share a scale
 MX4_BLOCK = 32
-#: up to this many rows a product runs on the kernel that has the weights on the M side (csrc/gemm_mx4.cu), above it on pairs of CTAs
+#: Up to this many rows a product runs on the kernel that has the weights on the M side (csrc/gemm_mx4.cu), above it on pairs of CTAs (us, that kernel and
+#: pairs, 4,096 x 24,576: 64 rows 30 and 36, 96 rows 39 and 37; both operands in four bits 64 rows 19 and 19, 96 rows 23 and 20) ...
 MX4_FEW_ROWS = 64
-#: experts' products run on pairs of CTAs where a step has more choices per expert than this
-MX4_FEW_CHOICES = 16
+#: ... and rows of bfloat16 up to this many there too, where the pairs' tiles would leave half of the pairs idle (4,096 x 4,096: 128 rows 14 and
+#: 20, 192 rows 20 and 21, 256 rows 22 and 21; 12,288 x 4,096: 192 rows 48 and 49; 2,048 x 2,048: 192 rows 9 and 13)
+MX4_FEW_ROWS_OF_SMALL = 192
+#: Experts' products run on pairs of CTAs where a step has more choices per expert than this (64 experts of 2,048 x 1,408: 32 choices 158 and 214, 48
+#: 223 and 225, 64 283 and 247; smaller ones cross above 96: 32 of 1,024 x 1,024 at 96 108 and 107, 8 of 1,024 x 512 30 and 43)
+MX4_FEW_CHOICES = 48
 
 _P, _I, _L, _F = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_float
 _LINEAR = (_P, _L, _P, _P, _P, _P, _P, _L, _I, _I, _I, _I, _P, _P, _P)
@@ -56,6 +61,11 @@ def _stream():
     as much as a launch."""
     scoped = _ops._scoped_stream
     return scoped if scoped is not None else torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
+
+
+def _few_rows(rows: int, features: int, four: bool) -> bool:
+    """True if a product goes to the kernel for few rows."""
+    return rows <= MX4_FEW_ROWS or (not four and rows <= MX4_FEW_ROWS_OF_SMALL and -(-features // 192) * 4 <= _ops.sm_count())
 
 
 def _tiles(n: int) -> int:
@@ -221,7 +231,7 @@ def linear_mx4(x, weight: Mx4, error_word: torch.Tensor, *, bias: Optional[torch
         if bias.shape != (weight.rows,):
             raise KernelError("linear_mx4: one bias per feature is needed")
     _here("linear_mx4", x.codes if four else x, weight.codes, weight.scales, bias, error_word)
-    many = rows > MX4_FEW_ROWS
+    many = not _few_rows(rows, weight.rows, four)
     # the kernel for many rows stores rows that start on 16-byte borders
     pitch = -(-weight.rows // 8) * 8 if many else weight.rows
     out = weight.codes.new_empty((rows, pitch), dtype=out_dtype)

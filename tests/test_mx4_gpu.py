@@ -144,7 +144,8 @@ def check_linear(x, matrix, w, bias=None, out_dtype=torch.bfloat16):
 
 SHAPES = [(1, 32, 1), (1, 128, 128), (2, 1, 3), (3, 33, 130), (5, 256, 16), (7, 1000, 129), (8, 384, 300), (9, 2050, 96), (16, 130, 257),
           (17, 640, 128), (31, 96, 511), (33, 4095, 100), (48, 512, 384), (64, 160, 640), (65, 288, 127), (100, 257, 130), (128, 512, 256),
-          (129, 130, 513), (200, 1024, 520), (257, 320, 260), (300, 72, 1030), (513, 200, 300)]
+          (129, 130, 513), (200, 1024, 520), (257, 320, 260), (300, 72, 1030), (513, 200, 300),
+          (1025, 328, 6150), (700, 1300, 9601)]
 
 
 @pytest.mark.parametrize("four", [False, True])
@@ -382,7 +383,8 @@ def expert_case(seed, rows, experts, width, inner, top, gated=True):
 
 
 @pytest.mark.parametrize("rows,experts,width,inner,top", [(1, 4, 64, 32, 1), (1, 8, 256, 128, 3), (3, 5, 130, 70, 2), (8, 16, 256, 192, 4), (20, 3, 320, 96, 3),
-                                                          (40, 2, 128, 256, 1), (70, 4, 96, 144, 2), (150, 3, 264, 136, 2), (33, 7, 257, 33, 5)])
+                                                          (40, 2, 128, 256, 1), (70, 4, 96, 144, 2), (150, 3, 264, 136, 2), (33, 7, 257, 33, 5), (200, 8, 1540, 48, 4),
+                                                          (90, 2, 192, 192, 1), (90, 2, 192, 224, 1)])
 def test_experts(rows, experts, width, inner, top):
     check_experts(*expert_case(30 + rows, rows, experts, width, inner, top))
 
