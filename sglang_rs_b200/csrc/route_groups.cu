@@ -53,20 +53,6 @@ __device__ __forceinline__ unsigned long long route_most(unsigned long long key)
   const unsigned low = __reduce_max_sync(ALL, (unsigned)(key >> 32) == high ? (unsigned)key : 0u);
   return (unsigned long long)high << 32 | low;
 }
-template <typename R> struct RouteKey { typedef unsigned Type; };
-template <> struct RouteKey<double> { typedef unsigned long long Type; };
-
-__device__ __forceinline__ float route_exp(float v) { return expf(v); }
-__device__ __forceinline__ double route_exp(double v) { return exp(v); }
-// 1 / v, in 32 bits to 2 units of the last place
-__device__ __forceinline__ float route_over(float v) { return __fdividef(1.0f, v); }
-__device__ __forceinline__ double route_over(double v) { return 1.0 / v; }
-__device__ __forceinline__ double route_sum(double v) {
-#pragma unroll
-  for (int offset = 16; offset > 0; offset >>= 1) v += __shfl_xor_sync(ALL, v, offset);
-  return v;
-}
-__device__ __forceinline__ float route_sum(float v) { return srb_warp_sum(v); }
 
 // Whether 32-bit numbers do not tell which of two picks (or sums of two) is larger, `above` being the larger one of them.  `by_logit`: they are the logits
 // themselves, whose order is that of the scores but where the 64-bit scores are alike: both 0, or sigmoids within 2^-53 of 1.  Otherwise
@@ -78,103 +64,100 @@ __device__ __forceinline__ bool route_near(float above, float below, float bias_
   return !(above - below > room) || (bias_most == 0.f && below < 5.8207661e-11f);
 }
 
-// The lane k < top gets the k-th choice.  R: the scores' type; in 32 bits the choice holds unless `near`.  `most` and `sum`: of a softmax, in R.  `shared`:
-// room for a key of every expert.
-template <int PER, typename R>
-__device__ __forceinline__ int route_choose(const float (&z)[PER], const float* __restrict__ bias, const GroupRule& rule, R most, R sum, bool by_logit,
-                                            void* shared, int lane, bool& near) {
-  typedef typename RouteKey<R>::Type Key;
-  constexpr bool CHECK = sizeof(R) == 4;
-  Key key[PER];
+// The score of a group whose largest two picks each lane has among its own.
+template <typename Key>
+__device__ __forceinline__ Key route_group_score(Key first, Key second, int group_best, int lane) {
+  const Key best = route_most(first);
+  auto sum = route_value(best);
+  if (group_best == 2) {
+    const int owner = __ffs(__ballot_sync(ALL, first == best)) - 1;
+    sum += route_value(route_most(lane == owner ? second : first));
+  }
+  return route_key(sum == sum ? sum : (decltype(sum))-INFINITY);
+}
+
+// The lane k < top gets the k-th choice by 32-bit scores; it holds unless `near`.  `most` and `sum`: of a softmax.  `picks`: room for a key of
+// every expert.
+template <int PER>
+__device__ __forceinline__ int route_choose(const float (&z)[PER], const float* __restrict__ bias, const GroupRule& rule, float most, float sum,
+                                            unsigned* picks, int lane, bool& near) {
+  const bool by_logit = !bias && (rule.group_best == 1 || rule.groups == rule.top_groups);
+  unsigned key[PER];
   float bias_most = 0.f;
-  const R over_sum = (R)1 / sum;
+  const float over_sum = __fdividef(1.0f, sum);
 #pragma unroll
   for (int j = 0; j < PER; ++j) {
     const int e = lane + 32 * j;
-    R pick = (R)z[j];
-    if (!by_logit) pick = rule.scoring == ROUTE_SOFTMAX ? route_exp(pick - most) * over_sum : route_over((R)1 + route_exp(-pick));
+    float pick = z[j];
+    if (!by_logit) pick = rule.scoring == ROUTE_SOFTMAX ? expf(pick - most) * over_sum : __fdividef(1.0f, 1.0f + expf(-pick));
     if (bias && e < rule.experts) {
       const float b = __ldg(bias + e);
       bias_most = fmaxf(bias_most, fabsf(b));
-      pick += (R)b;
+      pick += b;
     }
-    key[j] = e < rule.experts ? route_key(pick == pick ? pick : (R)-INFINITY) : (Key)0;
+    key[j] = e < rule.experts ? route_key(pick == pick ? pick : -INFINITY) : 0u;
   }
-  if (CHECK && bias) bias_most = __uint_as_float(__reduce_max_sync(ALL, __float_as_uint(bias_most)));
+  if (bias) bias_most = __uint_as_float(__reduce_max_sync(ALL, __float_as_uint(bias_most)));
   near = false;
   if (rule.groups > rule.top_groups) {
     const int per_group = rule.per_group;
-    const bool whole = per_group % 32 == 0;                  // a group is some of the registers, of all lanes
-    Key* picks = reinterpret_cast<Key*>(shared);
-    if (!whole) {
-#pragma unroll
-      for (int j = 0; j < PER; ++j)
-        if (lane + 32 * j < rule.experts) picks[lane + 32 * j] = key[j];
-      __syncwarp();
-    }
-    Key mine = 0;                                            // the score of group `lane`
-    auto score_group = [&](int g, Key first, Key second) {
-      const Key best = route_most(first);
-      R group = route_value(best);
-      if (rule.group_best == 2) {
-        const int owner = __ffs(__ballot_sync(ALL, first == best)) - 1;
-        group += route_value(route_most(lane == owner ? second : first));
-      }
-      if (lane == g) mine = route_key(group == group ? group : (R)-INFINITY);
-    };
-    if (whole) {
+    unsigned mine = 0u;                                      // the score of group `lane`
+    if (per_group % 32 == 0) {
+      // a group is some of the registers, of all lanes
       int g = 0, end = per_group;
-      Key first = 0, second = 0;
+      unsigned first = 0u, second = 0u;
 #pragma unroll
       for (int j = 0; j < PER; ++j) {
         second = max(second, min(first, key[j]));
         first = max(first, key[j]);
         if (32 * (j + 1) == end) {
-          score_group(g++, first, second);
-          first = second = 0;
-          end = g < rule.groups ? end + per_group : 0;
+          const unsigned score = route_group_score(first, second, rule.group_best, lane);
+          if (lane == g) mine = score;
+          first = second = 0u;
+          end = ++g < rule.groups ? end + per_group : 0;
         }
       }
     } else {
+#pragma unroll
+      for (int j = 0; j < PER; ++j)
+        if (lane + 32 * j < rule.experts) picks[lane + 32 * j] = key[j];
+      __syncwarp();
       for (int g = 0; g < rule.groups; ++g) {
-        Key first = 0, second = 0;
+        unsigned first = 0u, second = 0u;
         for (int i = lane; i < per_group; i += 32) {
-          const Key v = picks[g * per_group + i];
+          const unsigned v = picks[g * per_group + i];
           second = max(second, min(first, v));
           first = max(first, v);
         }
-        score_group(g, first, second);
+        const unsigned score = route_group_score(first, second, rule.group_best, lane);
+        if (lane == g) mine = score;
       }
+      __syncwarp();
     }
     unsigned open = 0u;
-    R last = 0;
-    for (int k = 0; k < rule.top_groups + (CHECK ? 1 : 0); ++k) {
-      const Key best = route_most(mine);
-      const R value = route_value(best);
-      if (k == rule.top_groups) {
-        near = route_near((float)last, (float)value, 2.f * bias_most, (float)most, by_logit, rule.scoring);
-        break;
-      }
+    float last = 0.f;
+    for (int k = 0; k < rule.top_groups; ++k) {
+      const unsigned best = route_most(mine);
       const int g = __ffs(__ballot_sync(ALL, mine == best)) - 1;
       open |= 1u << g;
-      if (lane == g) mine = 0;
-      last = value;
+      if (lane == g) mine = 0u;
+      last = route_value(best);
     }
+    near = route_near(last, route_value(route_most(mine)), 2.f * bias_most, most, by_logit, rule.scoring);
 #pragma unroll
     for (int j = 0; j < PER; ++j)
-      if (lane + 32 * j < rule.experts && !((open >> ((unsigned)(lane + 32 * j) * rule.group_factor >> 20)) & 1u)) key[j] = 0;
-    __syncwarp();
+      if (lane + 32 * j < rule.experts && !((open >> ((unsigned)(lane + 32 * j) * rule.group_factor >> 20)) & 1u)) key[j] = 0u;
   }
   int choice = 0;
-  R last = 0;
-  for (int k = 0; k < rule.top + (CHECK ? 1 : 0); ++k) {
-    Key mine = 0;
+  float last = 0.f;
+  for (int k = 0; k <= rule.top; ++k) {
+    unsigned mine = 0u;
 #pragma unroll
     for (int j = 0; j < PER; ++j) mine = max(mine, key[j]);
-    const Key best = route_most(mine);
-    if (best == 0) break;                                    // all are taken
-    const R value = route_value(best);
-    if (CHECK && k > 0) near |= route_near((float)last, (float)value, bias_most, (float)most, by_logit, rule.scoring);
+    const unsigned best = route_most(mine);
+    if (best == 0u) break;                                   // all are taken
+    const float value = route_value(best);
+    if (k > 0) near |= route_near(last, value, bias_most, most, by_logit, rule.scoring);
     last = value;
     if (k == rule.top) break;
     unsigned index = 0x7fffffffu;
@@ -184,34 +167,78 @@ __device__ __forceinline__ int route_choose(const float (&z)[PER], const float* 
     index = __reduce_min_sync(ALL, index);
 #pragma unroll
     for (int j = 0; j < PER; ++j)
-      if (index == (unsigned)(lane + 32 * j)) key[j] = 0;
+      if (index == (unsigned)(lane + 32 * j)) key[j] = 0u;
+    if (lane == k) choice = (int)index;
+  }
+  return choice;
+}
+
+// The same by 64-bit scores, for the few rows that need it: loops over the keys in shared memory and no code laid out flat, since a warp that comes here
+// waits for the instructions to be fetched.
+__device__ __noinline__ int route_choose_exactly(const float* __restrict__ z, const float* __restrict__ bias, const GroupRule& rule, unsigned long long* keys,
+                                                 int lane) {
+  double most = -INFINITY, sum = 0.0;
+  if (rule.scoring == ROUTE_SOFTMAX) {
+#pragma unroll 1
+    for (int e = lane; e < rule.experts; e += 32) most = fmax(most, (double)z[e]);
+    most = route_value(route_most(route_key(most)));
+#pragma unroll 1
+    for (int e = lane; e < rule.experts; e += 32) sum += exp((double)z[e] - most);
+#pragma unroll 1
+    for (int offset = 16; offset > 0; offset >>= 1) sum += __shfl_xor_sync(ALL, sum, offset);
+  }
+#pragma unroll 1
+  for (int e = lane; e < rule.experts; e += 32) {
+    const bool softmax = rule.scoring == ROUTE_SOFTMAX;
+    const double power = exp(softmax ? (double)z[e] - most : -(double)z[e]);
+    double pick = (softmax ? power : 1.0) / (softmax ? sum : 1.0 + power);
+    if (bias) pick += (double)bias[e];
+    keys[e] = route_key(pick == pick ? pick : (double)-INFINITY);
+  }
+  __syncwarp();
+  if (rule.groups > rule.top_groups) {
+    unsigned long long mine = 0;
+#pragma unroll 1
+    for (int g = 0; g < rule.groups; ++g) {
+      unsigned long long first = 0, second = 0;
+#pragma unroll 1
+      for (int i = lane; i < rule.per_group; i += 32) {
+        const unsigned long long v = keys[g * rule.per_group + i];
+        second = max(second, min(first, v));
+        first = max(first, v);
+      }
+      const unsigned long long score = route_group_score(first, second, rule.group_best, lane);
+      if (lane == g) mine = score;
+    }
+    unsigned open = 0u;
+#pragma unroll 1
+    for (int k = 0; k < rule.top_groups; ++k) {
+      const int g = __ffs(__ballot_sync(ALL, mine == route_most(mine))) - 1;
+      open |= 1u << g;
+      if (lane == g) mine = 0;
+    }
+    __syncwarp();
+#pragma unroll 1
+    for (int e = lane; e < rule.experts; e += 32)
+      if (!((open >> ((unsigned)e * rule.group_factor >> 20)) & 1u)) keys[e] = 0;
+  }
+  int choice = 0;
+#pragma unroll 1
+  for (int k = 0; k < rule.top; ++k) {
+    unsigned long long best = 0;
+    unsigned index = 0x7fffffffu;
+#pragma unroll 1
+    for (int e = lane; e < rule.experts; e += 32)
+      if (keys[e] > best) { best = keys[e]; index = (unsigned)e; }
+    index = __reduce_min_sync(ALL, best == route_most(best) ? index : 0x7fffffffu);
+    if (lane == (int)(index & 31u)) keys[index] = 0;         // the lane that reads it
     if (lane == k) choice = (int)index;
   }
   return choice;
 }
 
 template <int PER>
-__device__ __noinline__ int route_choose_exactly(const float* row, const float* bias, const GroupRule& rule, void* shared, int lane) {
-  float z[PER];
-  double most = -INFINITY, sum = 0.0;
-#pragma unroll
-  for (int j = 0; j < PER; ++j) {
-    z[j] = lane + 32 * j < rule.experts ? row[lane + 32 * j] : -INFINITY;
-    most = fmax(most, (double)z[j]);
-  }
-  if (rule.scoring == ROUTE_SOFTMAX) {
-    most = route_value(route_most(route_key(most)));
-#pragma unroll
-    for (int j = 0; j < PER; ++j)
-      if (lane + 32 * j < rule.experts) sum += exp((double)z[j] - most);
-    sum = route_sum(sum);
-  }
-  bool near;
-  return route_choose<PER, double>(z, bias, rule, most, sum, false, shared, lane, near);
-}
-
-template <int PER>
-__global__ void __launch_bounds__(32 * ROUTE_WARPS, PER <= 8 ? 8 : 1)
+__global__ void __launch_bounds__(32 * ROUTE_WARPS, PER <= 8 ? 10 : 1)
 route_groups_kernel(const float* __restrict__ logits, size_t pitch, int rows, const float* __restrict__ bias, GroupRule rule,
                     int* __restrict__ chosen, float* __restrict__ weights) {
   extern __shared__ unsigned long long route_shared[];       // [warps][experts]
@@ -234,13 +261,12 @@ route_groups_kernel(const float* __restrict__ logits, size_t pitch, int rows, co
 #pragma unroll
     for (int j = 0; j < PER; ++j)
       if (lane + 32 * j < rule.experts) sum += expf(z[j] - most);
-    sum = route_sum(sum);
+    sum = srb_warp_sum(sum);
   }
-  const bool by_logit = !bias && (rule.group_best == 1 || rule.groups == rule.top_groups);
   bool near;
-  int choice = route_choose<PER, float>(z, bias, rule, most, sum, by_logit, shared, lane, near);
+  int choice = route_choose<PER>(z, bias, rule, most, sum, reinterpret_cast<unsigned*>(shared), lane, near);
   // (a softmax over something that is not finite has no scores)
-  if (near || (rule.scoring == ROUTE_SOFTMAX && !(sum < INFINITY))) choice = route_choose_exactly<PER>(from, bias, rule, shared, lane);
+  if (near || (rule.scoring == ROUTE_SOFTMAX && !(sum < INFINITY))) choice = route_choose_exactly(from, bias, rule, shared, lane);
   // the chosen scores, a lane each
   float weight = 0.f;
   if (lane < rule.top) weight = rule.scoring == ROUTE_SOFTMAX ? expf(from[choice] - most) / sum : 1.0f / (1.0f + expf(-from[choice]));
