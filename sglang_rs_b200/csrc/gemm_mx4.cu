@@ -7,7 +7,10 @@
 // mxf8f6f4, W's entries have to stand 16 to 16 bytes in shared memory; TMA sets them so, but in pieces of 64 bytes, half of what it moves
 // otherwise: LATER.)
 //
-// A step is 256 entries of K.  All of it comes by TMA: the rows of W and X, and both sides' scales in the tiles that mx4.cuh lays them out in,
+// One row the blocks turn into parts themselves, in the four warps that wait for the sums otherwise: a launch less (one row through 4,096 x 24,576 12.1 us
+// instead of 13.8, 12,288 x 4,096 8.5 instead of 9.7; two rows 15.4 and 11.1 us: they keep the warps longer than the launch takes).
+//
+// A step is 256 entries of K.  All (else) of it comes by TMA: the rows of W and X, and both sides' scales in the tiles that mx4.cuh lays them out in,
 // which the issuing thread copies to tensor memory ahead of the step's products.
 //
 // Two blocks an SM.  K is cut where the row tiles are fewer than the SMs: the blocks of a cluster take a part each, leave their sums in shared
@@ -32,6 +35,7 @@ SRB_DEFINE_PDL_SWITCH()
 #define MXF_TOKENS 64            // rows of X of a tile, at most: in four bits
 #define MXF_PART_TOKENS 16       // ... in parts
 #define MXF_SLOTS 8              // ... over experts
+#define MXF_FUSED_TOKENS 1       // up to as many rows of bfloat16 are turned into parts by the product's own blocks
 #define MXF_THREADS 192
 #define MXF_EPILOGUE_THREADS 128
 #define MXF_W_BYTES 16384        // 128 rows x 256 entries
@@ -44,6 +48,9 @@ SRB_DEFINE_PDL_SWITCH()
 #define MXF_ACT 5      // ... of act(x w^T)
 
 struct FewArgs {
+  const __nv_bfloat16* x;        // FUSED: rows of bfloat16, `ldx` elements apart, of `width` entries; on 16-byte borders if x_wide
+  size_t ldx;
+  int width, x_wide;
   const float* bias;
   void* out;
   uint8_t* out_scales;           // of parts
@@ -100,6 +107,29 @@ __device__ __forceinline__ unsigned few_transpose(unsigned word, int lane) {
   return word;
 }
 
+// 256 entries of a row of X, 8 a lane, as parts (mx4.cuh) in a stage: rows 8 * token .. + 7 of 128 bytes, swizzled, and their scales, a byte for
+// each 32 entries in each part's word of the two tiles of 128 entries.
+__device__ __forceinline__ void few_make_parts(const uint4& raw, int token, int lane, unsigned x_to, unsigned xs_to) {
+  float v[8];
+  mx4_unpack_bf16(raw, v);
+  unsigned most = 0u;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) most = max(most, __float_as_uint(v[i]) & 0x7fffffffu);
+  most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
+  most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
+  const unsigned first = mx4_first_scale(most);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = mx4_over_first_scale(v[i], first);
+#pragma unroll
+  for (int part = 0; part < MX4_PARTS; ++part) {
+    const unsigned row = (unsigned)(token * MX4_PARTS + part);
+    asm volatile("st.shared.b32 [%0], %1;" ::"r"(x_to + row * 128 + ((((unsigned)lane >> 2) ^ (row & 7u)) << 4) + (lane & 3) * 4), "r"(mx4_next_part(v)) : "memory");
+    if ((lane & 3) == 0)
+      asm volatile("st.shared.u8 [%0], %1;" ::"r"(xs_to + (lane >> 4) * 512 + (row & 31u) * 16 + (row >> 5) * 4 + ((lane >> 2) & 3)),
+                   "r"(mx4_part_scale(first, part)) : "memory");
+  }
+}
+
 // What a tile is, the same in every role.
 struct FewTile {
   int matrix, feature0;
@@ -125,7 +155,7 @@ __device__ __forceinline__ FewTile few_tile(const FewArgs& a, int item) {
   return t;
 }
 
-template <bool PARTS, int MODE, bool GROUPED, int STAGES>
+template <bool PARTS, int MODE, bool GROUPED, int STAGES, bool FUSED>
 __global__ void __launch_bounds__(MXF_THREADS, 2)
 mx4_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_ws, const __grid_constant__ CUtensorMap map_x,
                const __grid_constant__ CUtensorMap map_xs, const FewArgs a) {
@@ -149,7 +179,7 @@ mx4_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
   if (threadIdx.x == 0) {
     abort_flag = 0;
     for (int s = 0; s < STAGES; ++s) {
-      mbar_init(smem_u32(&full_bar[s]), 1);
+      mbar_init(smem_u32(&full_bar[s]), FUSED ? 1 + a.tokens : 1);
       mbar_init(smem_u32(&empty_bar[s]), 1);
     }
     for (int b = 0; b < 2; ++b) {
@@ -160,7 +190,7 @@ mx4_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
   }
   if (warp == 1) tmem_alloc(smem_u32(&tmem_holder), 256);
   srb_launch_dependents();
-  if (!PARTS) srb_grid_dependency_wait();
+  if (!PARTS || FUSED) srb_grid_dependency_wait();
   // (With parts the kernel ahead is the one that made them, or the product ahead of this one behind it.  That kernel lets the next one start once
   // all kernels ahead of it are done, so W and the plan, which are older, may be read at once; X is awaited below.)
   const int items = (GROUPED ? a.plan[0] : a.tiles_t) * a.tiles_f;
@@ -178,7 +208,7 @@ mx4_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
       const unsigned bar = smem_u32(&full_bar[s]), to = stages + s * stage_bytes, scales_to = scales + s * Shape::SCALE_BYTES;
       const int w_row = t.matrix * a.w_rows + t.feature0, ws_tile = (t.matrix * a.ws_tiles + (t.feature0 >> 7)) * a.k_tiles;
       if (elect_one()) {
-        mbar_expect_tx(bar, stage_bytes + Shape::SCALE_BYTES);
+        mbar_expect_tx(bar, FUSED ? Shape::SIDES * (MXF_W_BYTES + 1024) : stage_bytes + Shape::SCALE_BYTES);
         tma_load_2d(to, &map_w, bar, step * 128, w_row);
         if (GATED) tma_load_2d(to + MXF_W_BYTES, &map_w, bar, step * 128, w_row + a.features);
         tma_load_2d(scales_to, &map_ws, bar, 0, ws_tile + 2 * step);
@@ -197,7 +227,7 @@ mx4_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
     };
     // the first steps' W ahead of the wait for X
     int early = 0;
-    if (PARTS) {
+    if (PARTS && !FUSED) {
       if (first_item < items) {
         const FewTile t = few_tile<GROUPED>(a, first_item);
         early = min(steps, STAGES);
@@ -214,7 +244,7 @@ mx4_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
           if (!ok) break;
           load_w(t, s, step0 + i);
         }
-        load_x(t, s, step0 + i);
+        if (!FUSED) load_x(t, s, step0 + i);
       }
     }
     if (abort_flag && round > 0) {
@@ -273,6 +303,36 @@ mx4_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
       const int b = local % buffers;
       const FewTile t = few_tile<GROUPED>(a, item);
       const int feature = t.feature0 + in_tile;
+      if (FUSED) {
+        // a step's 256 entries of a row at a time, by the four warps in turn, the next ones on their way while these become parts
+        auto load = [&](int job) {
+          const int k = (step0 + job / a.tokens) * 256 + lane * 8;
+          const __nv_bfloat16* src = a.x + (size_t)(job % a.tokens) * a.ldx + k;
+          uint4 raw = make_uint4(0u, 0u, 0u, 0u);
+          if (a.x_wide && k + 8 <= a.width) return *reinterpret_cast<const uint4*>(src);
+          unsigned short* to = reinterpret_cast<unsigned short*>(&raw);
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (k + i < a.width) to[i] = reinterpret_cast<const unsigned short*>(src)[i];
+          return raw;
+        };
+        const int jobs = steps * a.tokens;
+        uint4 raw = make_uint4(0u, 0u, 0u, 0u), next = raw;
+        bool ok = true;
+        if (warp - 2 < jobs) raw = load(warp - 2);
+        for (int job = warp - 2; job < jobs; job += 4, raw = next) {
+          const unsigned round = (unsigned)(local * steps + job / a.tokens);
+          const int s = (int)(round % STAGES);
+          if (job + 4 < jobs) next = load(job + 4);
+          ok = mbar_wait_warp(smem_u32(&empty_bar[s]), ((round / STAGES) & 1u) ^ 1u, &abort_flag);
+          if (!ok) break;
+          few_make_parts(raw, job % a.tokens, lane, stages + s * stage_bytes + Shape::SIDES * MXF_W_BYTES, scales + s * Shape::SCALE_BYTES + 1024 * Shape::SIDES);
+          fence_proxy_async_shared();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(smem_u32(&full_bar[s]));
+        }
+        if (!ok) break;
+      }
       if (!mbar_wait_warp(smem_u32(&acc_full[b]), (unsigned)(local / buffers) & 1u, &abort_flag)) break;
       tc_fence_after();
       const unsigned sums = lane_address + b * buffer_columns;
@@ -352,40 +412,43 @@ mx4_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
   }
 }
 
-template <bool PARTS, int MODE, bool GROUPED, int STAGES>
+template <bool PARTS, int MODE, bool GROUPED, int STAGES, bool FUSED>
 static int launch_few_staged(const CUtensorMap (&maps)[4], const FewArgs& a, int blocks, cudaStream_t s) {
   using Shape = FewShape<MODE == MXF_GATED>;
   const size_t smem = 1024 + (size_t)STAGES * (Shape::stage_bytes(a.columns) + Shape::SCALE_BYTES);
   static std::atomic<int> allowed[MX4_MAX_DEVICES];
-  auto kernel = mx4_few_kernel<PARTS, MODE, GROUPED, STAGES>;
+  auto kernel = mx4_few_kernel<PARTS, MODE, GROUPED, STAGES, FUSED>;
   if (const int status = mx4_allow_shared((const void*)kernel, (int)smem, allowed)) return status;
   SRB_CUDA_CALL(srb_launch_clustered(kernel, dim3(blocks), dim3(MXF_THREADS), smem, s, dim3(a.splits), maps[0], maps[1], maps[2], maps[3], a));
   return SRB_OK;
 }
 
 // x: codes [x_rows, 64 k_tiles] (parts or not) and their scales.  Stages for as much shared memory as two blocks an SM leave.
-template <bool PARTS, int MODE, bool GROUPED>
+template <bool PARTS, int MODE, bool GROUPED, bool FUSED = false>
 static int launch_few(const void* x, const void* x_scales, long long x_rows, const void* w, const void* w_scales, FewArgs& a, cudaStream_t s) {
   const long long matrices = std::max(a.experts, 1), w_rows = matrices * a.w_rows, ws_tiles = matrices * a.ws_tiles * a.k_tiles;
   const long long items = (long long)a.tiles_t * a.tiles_f, x_tiles = (x_rows + 127) / 128 * a.k_tiles;
-  if (((uintptr_t)w | (uintptr_t)x) & 15) SRB_FAIL("mx4_few: codes must start on a 16-byte border");
+  if (((uintptr_t)w | (FUSED ? 0 : (uintptr_t)x)) & 15) SRB_FAIL("mx4_few: codes must start on a 16-byte border");
   if (w_rows > 0x7fffffff || ws_tiles > 0x7fffffff || x_rows > 0x7fffffff || x_tiles > 0x7fffffff || items > 0x3fffffff)
     SRB_FAIL("mx4_few: %lld rows of weights and %lld of inputs are too many", w_rows, x_rows);
   CUtensorMap maps[4];
   if (make_bytes_map(&maps[0], w, w_rows, a.k_tiles * 64ll, 128) != SRB_OK || make_scales_map(&maps[1], w_scales, ws_tiles, 2) != SRB_OK ||
-      make_bytes_map(&maps[2], x, x_rows, a.k_tiles * 64ll, a.columns) != SRB_OK || make_scales_map(&maps[3], x_scales, x_tiles, 2) != SRB_OK)
+      (!FUSED && (make_bytes_map(&maps[2], x, x_rows, a.k_tiles * 64ll, a.columns) != SRB_OK || make_scales_map(&maps[3], x_scales, x_tiles, 2) != SRB_OK)))
     return SRB_ERR_INVALID;
+  if (FUSED) maps[2] = maps[3] = maps[0];
   // K in parts until there is about a block an SM: a block costs some 3 us beside its steps (8 rows of 4,096 through 4,096 features, 32 tiles, in 1, 2, 4
   // and 8 parts: 9.0, 7.6, 6.6 and 7.8 us; of 12,288 18.0, 12.1, 9.8 and 9.5; one row through 24,576, 192 tiles, in 1, 2 and 4: 13.8, 16.2 and 19.0)
   const long long room = 2ll * srb_sm_count(), all_steps = (a.k_tiles + 1) / 2;
   a.splits = GROUPED ? 1 : (int)std::max(1ll, std::min(std::min<long long>(room / 2 / items, MXF_MAX_SPLITS), all_steps));
   const int blocks = (int)(a.splits > 1 ? items * a.splits : std::min(items, room));
-  if (MODE == MXF_GATED) return launch_few_staged<PARTS, MODE, GROUPED, 2>(maps, a, blocks, s);
-  return a.columns <= 64 ? launch_few_staged<PARTS, MODE, GROUPED, 4>(maps, a, blocks, s) : launch_few_staged<PARTS, MODE, GROUPED, 3>(maps, a, blocks, s);
+  if constexpr (MODE == MXF_GATED) return launch_few_staged<PARTS, MODE, GROUPED, 2, false>(maps, a, blocks, s);
+  else if constexpr (FUSED) return launch_few_staged<PARTS, MODE, GROUPED, 5, true>(maps, a, blocks, s);
+  else return a.columns <= 64 ? launch_few_staged<PARTS, MODE, GROUPED, 4, false>(maps, a, blocks, s) : launch_few_staged<PARTS, MODE, GROUPED, 3, false>(maps, a, blocks, s);
 }
 
 // ---- entries: `scratch` has srb_mx4_linear_scratch bytes (none are needed for rows in four bits) ----------------------------
 extern "C" long long srb_mx4_linear_scratch(int rows, int width) {
+  if (rows <= MXF_FUSED_TOKENS) return 0;
   Mx4Scratch scratch = {};
   scratch.take((size_t)rows * MX4_PARTS * mx4_pitch(width));
   scratch.take((size_t)mx4_tiles(rows * MX4_PARTS) * mx4_tiles(width) * MX4_TILE_BYTES);
@@ -408,6 +471,11 @@ extern "C" int srb_mx4_linear(const void* x, long long ldx, const void* x_scales
   cudaStream_t s = (cudaStream_t)stream;
   if (!parts)
     return out_float ? launch_few<false, MXF_F32, false>(x, x_scales, rows, w, w_scales, a, s) : launch_few<false, MXF_BF16, false>(x, x_scales, rows, w, w_scales, a, s);
+  if (rows <= MXF_FUSED_TOKENS) {
+    a.x = (const __nv_bfloat16*)x; a.ldx = (size_t)ldx; a.width = width; a.x_wide = mx4_wide(x, ldx);
+    return out_float ? launch_few<true, MXF_F32, false, true>(x, nullptr, 8ll * rows, w, w_scales, a, s)
+                     : launch_few<true, MXF_BF16, false, true>(x, nullptr, 8ll * rows, w, w_scales, a, s);
+  }
   Mx4Scratch scratch = {(uint8_t*)scratch_memory, 0};
   uint8_t* codes = scratch.take((size_t)rows * MX4_PARTS * mx4_pitch(width));
   uint8_t* scales = scratch.take((size_t)mx4_tiles(rows * MX4_PARTS) * a.k_tiles * MX4_TILE_BYTES);

@@ -239,10 +239,11 @@ def linear_mx4(x, weight: Mx4, error_word: torch.Tensor, *, bias: Optional[torch
         lib = _library("gemm_mx4_pair" if many else "gemm_mx4")
         product, needed = (lib.srb_mx4_linear_pair, lib.srb_mx4_linear_pair_scratch) if many else (lib.srb_mx4_linear, lib.srb_mx4_linear_scratch)
         held = x.codes if four else x
-        scratch = None if four else weight.codes.new_empty(needed(rows, width))
+        needed = 0 if four else needed(rows, width)
+        scratch = weight.codes.new_empty(needed) if needed else None
         _check(lib, product(held.data_ptr(), held.stride(0), x.scales.data_ptr() if four else None, weight.codes.data_ptr(), weight.scales.data_ptr(),
                             None if bias is None else bias.data_ptr(), out.data_ptr(), pitch, rows, weight.rows, width,
-                            out_dtype == torch.float32, None if four else scratch.data_ptr(), error_word.data_ptr(), _stream()), 1 if four else 2)
+                            out_dtype == torch.float32, scratch.data_ptr() if needed else None, error_word.data_ptr(), _stream()), 2 if needed else 1)
     return out if pitch == weight.rows else out[:, :weight.rows]
 
 
