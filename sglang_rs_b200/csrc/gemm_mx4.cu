@@ -436,10 +436,12 @@ static int launch_few(const void* x, const void* x_scales, long long x_rows, con
       (!FUSED && (make_bytes_map(&maps[2], x, x_rows, a.k_tiles * 64ll, a.columns) != SRB_OK || make_scales_map(&maps[3], x_scales, x_tiles, 2) != SRB_OK)))
     return SRB_ERR_INVALID;
   if (FUSED) maps[2] = maps[3] = maps[0];
-  // K in parts until there is about a block an SM: a block costs some 3 us beside its steps (8 rows of 4,096 through 4,096 features, 32 tiles, in 1, 2, 4
-  // and 8 parts: 9.0, 7.6, 6.6 and 7.8 us; of 12,288 18.0, 12.1, 9.8 and 9.5; one row through 24,576, 192 tiles, in 1, 2 and 4: 13.8, 16.2 and 19.0)
-  const long long room = 2ll * srb_sm_count(), all_steps = (a.k_tiles + 1) / 2;
-  a.splits = GROUPED ? 1 : (int)std::max(1ll, std::min(std::min<long long>(room / 2 / items, MXF_MAX_SPLITS), all_steps));
+  // K in parts until there is about a block an SM, or two parts where that makes two: a block costs some 3 us beside its steps (8 rows of 4,096 through
+  // 4,096 features, 32 tiles, in 1, 2, 4 and 8 parts: 9.0, 7.6, 6.6 and 7.8 us; of 12,288 18.0, 12.1, 9.8 and 9.5; through 12,288 features, 96
+  // tiles, in 1, 2 and 3: 9.4, 9.1 and 12.9; one row through 24,576, 192 tiles, in 1, 2 and 4: 13.8, 16.2 and 19.0)
+  const long long sms = srb_sm_count(), room = 2 * sms, all_steps = (a.k_tiles + 1) / 2;
+  const long long wanted = std::max(sms / items, std::min(room / items, 2ll));
+  a.splits = GROUPED ? 1 : (int)std::max(1ll, std::min(std::min<long long>(wanted, MXF_MAX_SPLITS), all_steps));
   const int blocks = (int)(a.splits > 1 ? items * a.splits : std::min(items, room));
   if constexpr (MODE == MXF_GATED) return launch_few_staged<PARTS, MODE, GROUPED, 2, false>(maps, a, blocks, s);
   else if constexpr (FUSED) return launch_few_staged<PARTS, MODE, GROUPED, 5, true>(maps, a, blocks, s);

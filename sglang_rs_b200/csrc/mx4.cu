@@ -45,7 +45,7 @@ __device__ __forceinline__ void mx4_turn(float* staged, int lane, float (&v)[8])
 template <typename T, bool WIDE, int AT_ONCE>
 __global__ void __launch_bounds__(MX4_THREADS)
 mx4_quantize_kernel(const T* __restrict__ x, size_t pitch, size_t matrix_pitch, int rows, int width, unsigned* __restrict__ codes,
-                    unsigned* __restrict__ scales) {
+                    uint8_t* __restrict__ scales) {
   __shared__ float staged[MX4_THREADS / 16][128 + 4];
   srb_launch_dependents();
   srb_grid_dependency_wait();
@@ -69,18 +69,16 @@ mx4_quantize_kernel(const T* __restrict__ x, size_t pitch, size_t matrix_pitch, 
     most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
     most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
     const bool finite = most < 0x7f800000u;
-    const int exponent = max((int)(most >> 23) - 129, -127); // a subnormal's field is 0: the least scale
-    const unsigned s = finite ? (unsigned)(exponent + 127) : 255u;
-    const float inverse = __uint_as_float((unsigned)(127 - exponent) << 23);    // 2^-exponent, between 2^-125 and 2^127
+    const unsigned s = finite ? max(most >> 23, 2u) - 2u : 255u;       // a subnormal's field is 0: the least scale
+    const float inverse = __uint_as_float((254u - s) << 23); // 1 / 2^(s - 127), between 2^-125 and 2^127
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[j][i] = finite ? v[j][i] * inverse : 0.f;
-    const unsigned packed = mx4_pack_eight(v[j]);
-    // the scales of the four blocks, a byte each, in one word; blocks behind the row's end and rows behind the last get 127
-    unsigned word = (live && kt * 128 + (lane >> 2) * 32 < width ? s : 127u) << (8 * (lane >> 2));
-    word |= __shfl_xor_sync(0xffffffffu, word, 4);
-    word |= __shfl_xor_sync(0xffffffffu, word, 8);
+    for (int i = 0; i < 8; ++i) v[j][i] *= inverse;
+    const unsigned packed = finite ? mx4_pack_eight(v[j]) : 0u;
     if (live) codes[((size_t)matrix * rows + row) * (mx4_pitch(width) / 4) + kt * 16 + lane] = packed;
-    if (lane == 0) scales[((size_t)matrix * row_tiles * k_tiles * MX4_TILE_BYTES + mx4_scale_word(row, kt, k_tiles)) / 4] = word;
+    // a block's scale by its first lane; blocks behind the row's end and rows behind the last get 127
+    if ((lane & 3) == 0)
+      scales[(size_t)matrix * row_tiles * k_tiles * MX4_TILE_BYTES + mx4_scale_word(row, kt, k_tiles) + (lane >> 2)] =
+          (uint8_t)(live && kt * 128 + lane * 8 < width ? s : 127u);
   }
 }
 
@@ -154,7 +152,7 @@ static int launch_quantize(const void* x, size_t pitch, size_t matrix_pitch, boo
                            int at_once, cudaStream_t s) {
   auto kernel = wide ? (at_once == 4 ? mx4_quantize_kernel<T, true, 4> : mx4_quantize_kernel<T, true, 1>)
                      : (at_once == 4 ? mx4_quantize_kernel<T, false, 4> : mx4_quantize_kernel<T, false, 1>);
-  SRB_CUDA_CALL(srb_launch(kernel, grid, dim3(MX4_THREADS), 0, s, (const T*)x, pitch, matrix_pitch, rows, width, (unsigned*)codes, (unsigned*)scales));
+  SRB_CUDA_CALL(srb_launch(kernel, grid, dim3(MX4_THREADS), 0, s, (const T*)x, pitch, matrix_pitch, rows, width, (unsigned*)codes, (uint8_t*)scales));
   return SRB_OK;
 }
 template <typename T>
