@@ -486,38 +486,35 @@ extern "C" int srb_mx4_linear(const void* x, long long ldx, const void* x_scales
                    : launch_few<true, MXF_BF16, false>(codes, scales, 8ll * rows, w, w_scales, a, s);
 }
 
-// Scratch of a call on the experts, in the order in which it is taken: rows of the slots, what is between the products, the results, and
-// gate/up scales with the up rows on the border of a tile, where they do not begin there.
+// Scratch of a call on the experts, in the order in which it is taken: rows of the slots, what is between the products, and gate/up scales with the up rows on the border of a tile, where they do not begin there.
 struct FewExpertsScratch {
-  uint8_t *x, *x_scales, *act, *act_scales, *y, *up_scales;
+  uint8_t *x, *x_scales, *act, *act_scales, *up_scales;
   size_t bytes;
-  FewExpertsScratch(void* memory, int entries, int max_tiles, int experts, int width, int inner, int gated) {
+  FewExpertsScratch(void* memory, int max_tiles, int experts, int width, int inner, int gated) {
     Mx4Scratch s = {(uint8_t*)memory, 0};
     const size_t rows = (size_t)MXF_SLOTS * MX4_PARTS * max_tiles, row_tiles = (rows + 127) / 128;
     x = s.take(rows * mx4_pitch(width));
     x_scales = s.take(row_tiles * mx4_tiles(width) * MX4_TILE_BYTES);
     act = s.take(rows * mx4_pitch(inner));
     act_scales = s.take(row_tiles * mx4_tiles(inner) * MX4_TILE_BYTES);
-    y = s.take((size_t)entries * width * 4);
     up_scales = gated && inner % 128 ? s.take(mx4_gated_scales_bytes(experts, width, 256 * mx4_tiles(inner), 1)) : nullptr;
     bytes = s.used;
   }
 };
-extern "C" long long srb_mx4_experts_scratch(int entries, int max_tiles, int experts, int width, int inner, int gated) {
-  return (long long)FewExpertsScratch(nullptr, entries, max_tiles, experts, width, inner, gated).bytes;
+extern "C" long long srb_mx4_experts_scratch(int max_tiles, int experts, int width, int inner, int gated) {
+  return (long long)FewExpertsScratch(nullptr, max_tiles, experts, width, inner, gated).bytes;
 }
 extern "C" int srb_mx4_experts_tile() { return MXF_SLOTS; }
 
-// `plan` (tiles of srb_mx4_experts_tile slots, at most max_tiles), slot_row and entry_slot are those of csrc/moe.cu.
-extern "C" int srb_mx4_experts(const void* h, const int* plan, const int* slot_row, const int* entry_slot, const float* weights, const void* up,
-                               const void* up_scales, const void* down, const void* down_scales, void* out, int rows, int top, int max_tiles,
-                               int experts, int width, int inner, int gated, int activation, float act_param, void* scratch_memory,
-                               int* error_word, void* stream) {
-  if (rows <= 0 || top <= 0) return SRB_OK;
-  const Mx4ExpertsCall c = {h, plan, slot_row, entry_slot, weights, up, up_scales, down, down_scales, out, rows, top, max_tiles, experts, width, inner, gated,
-                            activation, act_param, error_word, (cudaStream_t)stream};
+// `plan` (tiles of srb_mx4_experts_tile slots, at most max_tiles) and slot_row are those of csrc/moe.cu; y float [slots, width] gets the slots' results.
+extern "C" int srb_mx4_experts(const void* h, const int* plan, const int* slot_row, const void* up, const void* up_scales, const void* down,
+                               const void* down_scales, float* y, int max_tiles, int slots, int experts, int width, int inner, int gated,
+                               int activation, float act_param, void* scratch_memory, int* error_word, void* stream) {
+  if (max_tiles <= 0) return SRB_OK;
+  const Mx4ExpertsCall c = {h, plan, slot_row, up, up_scales, down, down_scales, y, max_tiles, slots, experts, width, inner, gated, activation, act_param,
+                            error_word, (cudaStream_t)stream};
   if (const int status = mx4_check_experts(c)) return status;
-  const FewExpertsScratch scratch(scratch_memory, rows * top, max_tiles, experts, width, inner, gated);
+  const FewExpertsScratch scratch(scratch_memory, max_tiles, experts, width, inner, gated);
   const long long x_rows = (long long)MXF_SLOTS * MX4_PARTS * max_tiles;
   FewArgs a = {};
   a.activation = activation; a.act_param = act_param; a.error_word = error_word; a.plan = plan; a.experts = experts; a.tiles_t = max_tiles;
@@ -538,8 +535,13 @@ extern "C" int srb_mx4_experts(const void* h, const int* plan, const int* slot_r
   if (const int status = gated ? launch_few<true, MXF_GATED, true>(scratch.x, scratch.x_scales, x_rows, up, up_scales, first, c.stream)
                                : launch_few<true, MXF_ACT, true>(scratch.x, scratch.x_scales, x_rows, up, up_scales, first, c.stream)) return status;
   FewArgs second = a;
-  second.out = scratch.y; second.features = second.w_rows = width; second.k_tiles = mx4_tiles(inner); second.ws_tiles = second.tiles_f = mx4_tiles(width);
+  second.out = y; second.features = second.w_rows = width; second.k_tiles = mx4_tiles(inner); second.ws_tiles = second.tiles_f = mx4_tiles(width);
   second.ldo = width;
-  if (const int status = launch_few<true, MXF_F32, true>(scratch.act, scratch.act_scales, x_rows, down, down_scales, second, c.stream)) return status;
-  return mx4_launch_combine((const float*)scratch.y, entry_slot, weights, rows, top, width, out, c.stream);
+  return launch_few<true, MXF_F32, true>(scratch.act, scratch.act_scales, x_rows, down, down_scales, second, c.stream);
+}
+
+// out bfloat16 [rows, width]: the weighted sum of every row's results.
+extern "C" int srb_mx4_combine(const float* y, const int* entry_slot, const float* weights, int rows, int top, int width, void* out, void* stream) {
+  if (rows <= 0 || width <= 0) return SRB_OK;
+  return mx4_launch_combine(y, entry_slot, weights, rows, top, width, out, (cudaStream_t)stream);
 }

@@ -455,7 +455,7 @@ extern "C" int srb_mx4_linear_pair(const void* x, long long ldx, const void* x_s
 static int pair_experts_product(int mode, const Mx4ExpertsCall& c, const uint8_t* x, const uint8_t* x_scales, const void* w, const void* w_scales, void* out,
                                 uint8_t* out_scales, int features, int width) {
   PairMx4Args a = {};
-  a.out = out; a.out_scales = out_scales; a.rows = c.rows * c.top; a.features = features; a.w_rows = mode == MXP_GATED ? 2 * features : features;
+  a.out = out; a.out_scales = out_scales; a.rows = c.slots; a.features = features; a.w_rows = mode == MXP_GATED ? 2 * features : features;
   a.k_tiles = mx4_tiles(width); a.activation = c.activation; a.act_param = c.act_param; a.error_word = c.error_word; a.plan = c.plan; a.experts = c.experts;
   const long long rows = (long long)MXP_TILE * c.max_tiles;
   const int out_tiles = mx4_tiles(features), covered = mode == MXP_F32 ? features : 128 * out_tiles, per_tile = mode == MXP_GATED ? MXP_HALF : MXP_N;
@@ -483,10 +483,10 @@ static int pair_experts_product(int mode, const Mx4ExpertsCall& c, const uint8_t
 }
 
 struct PairExpertsScratch {
-  uint8_t *x, *x_scales, *act, *act_scales, *y, *up_scales;
+  uint8_t *x, *x_scales, *act, *act_scales, *up_scales;
   size_t bytes;
   int groups;                    // of 96 gate and 96 up rows
-  PairExpertsScratch(void* memory, int entries, int max_tiles, int experts, int width, int inner, int gated) {
+  PairExpertsScratch(void* memory, int max_tiles, int experts, int width, int inner, int gated) {
     Mx4Scratch s = {(uint8_t*)memory, 0};
     const size_t rows = 2 * (size_t)MXP_TILE * max_tiles;
     groups = (128 * mx4_tiles(inner) + MXP_HALF - 1) / MXP_HALF;
@@ -494,27 +494,25 @@ struct PairExpertsScratch {
     x_scales = s.take(rows / 128 * mx4_tiles(width) * MX4_TILE_BYTES);
     act = s.take(rows * mx4_tiles(inner) * 128);
     act_scales = s.take(rows / 128 * mx4_tiles(inner) * MX4_TILE_BYTES);
-    y = s.take((size_t)entries * width * 4);
     up_scales = gated ? s.take(mx4_gated_scales_bytes(experts, width, 256, groups)) : nullptr;
     bytes = s.used;
   }
 };
-extern "C" long long srb_mx4_experts_pair_scratch(int entries, int max_tiles, int experts, int width, int inner, int gated) {
-  return (long long)PairExpertsScratch(nullptr, entries, max_tiles, experts, width, inner, gated).bytes;
+extern "C" long long srb_mx4_experts_pair_scratch(int max_tiles, int experts, int width, int inner, int gated) {
+  return (long long)PairExpertsScratch(nullptr, max_tiles, experts, width, inner, gated).bytes;
 }
 extern "C" int srb_mx4_experts_pair_tile() { return MXP_TILE; }
 
-// width is a multiple of 4.
-extern "C" int srb_mx4_experts_pair(const void* h, const int* plan, const int* slot_row, const int* entry_slot, const float* weights, const void* up,
-                                    const void* up_scales, const void* down, const void* down_scales, void* out, int rows, int top, int max_tiles,
-                                    int experts, int width, int inner, int gated, int activation, float act_param, void* scratch_memory,
-                                    int* error_word, void* stream) {
-  if (rows <= 0 || top <= 0) return SRB_OK;
-  const Mx4ExpertsCall c = {h, plan, slot_row, entry_slot, weights, up, up_scales, down, down_scales, out, rows, top, max_tiles, experts, width, inner, gated,
-                            activation, act_param, error_word, (cudaStream_t)stream};
+// As srb_mx4_experts; width is a multiple of 4.
+extern "C" int srb_mx4_experts_pair(const void* h, const int* plan, const int* slot_row, const void* up, const void* up_scales, const void* down,
+                                    const void* down_scales, float* y, int max_tiles, int slots, int experts, int width, int inner, int gated,
+                                    int activation, float act_param, void* scratch_memory, int* error_word, void* stream) {
+  if (max_tiles <= 0) return SRB_OK;
+  const Mx4ExpertsCall c = {h, plan, slot_row, up, up_scales, down, down_scales, y, max_tiles, slots, experts, width, inner, gated, activation, act_param,
+                            error_word, (cudaStream_t)stream};
   if (const int status = mx4_check_experts(c)) return status;
   if (width % 4) SRB_FAIL("mx4_experts_pair: width %d is no multiple of 4", width);
-  const PairExpertsScratch scratch(scratch_memory, rows * top, max_tiles, experts, width, inner, gated);
+  const PairExpertsScratch scratch(scratch_memory, max_tiles, experts, width, inner, gated);
   if (gated) {
     if (const int status = mx4_launch_gated_scales(up_scales, experts, inner, width, MXP_HALF, 256, scratch.groups, plan, scratch.up_scales, c.stream)) return status;
     up_scales = scratch.up_scales;
@@ -522,6 +520,59 @@ extern "C" int srb_mx4_experts_pair(const void* h, const int* plan, const int* s
   if (const int status = mx4_launch_split_slots(h, width, plan, slot_row, experts, max_tiles, scratch.x, scratch.x_scales, c.stream)) return status;
   if (const int status = pair_experts_product(gated ? MXP_GATED : MXP_ACT, c, scratch.x, scratch.x_scales, up, up_scales, scratch.act, scratch.act_scales,
                                               inner, width)) return status;
-  if (const int status = pair_experts_product(MXP_F32, c, scratch.act, scratch.act_scales, down, down_scales, scratch.y, nullptr, width, inner)) return status;
-  return mx4_launch_combine((const float*)scratch.y, entry_slot, weights, rows, top, width, out, c.stream);
+  return pair_experts_product(MXP_F32, c, scratch.act, scratch.act_scales, down, down_scales, y, nullptr, width, inner);
+}
+
+// A plan's experts between the two kernels: those with up to `limit` slots get tiles of `few_tile` slots in `few`, the others of 256 in `many`.  Both
+// are plans like the first: number of tiles, first slots, (expert, first slot) of every tile.  One block, an expert a thread.
+__global__ void __launch_bounds__(1024)
+mx4_divide_plan_kernel(const int* __restrict__ plan, int experts, int limit, int few_tile, int max_few, int max_many, int* __restrict__ few,
+                       int* __restrict__ many, int* error_word) {
+  __shared__ int before[2][32];
+  srb_launch_dependents();
+  srb_grid_dependency_wait();
+  const int e = threadIdx.x, lane = e & 31, warp = e >> 5;
+  const int first = plan[1 + min(e, experts)], slots = e < experts ? plan[1 + e + 1] - first : 0;
+  const int tiles[2] = {slots <= limit ? (slots + few_tile - 1) / few_tile : 0, slots > limit ? (slots + MXP_TILE - 1) / MXP_TILE : 0};
+  int run[2] = {tiles[0], tiles[1]};
+#pragma unroll
+  for (int kind = 0; kind < 2; ++kind) {
+#pragma unroll
+    for (int offset = 1; offset < 32; offset <<= 1) {
+      const int other = __shfl_up_sync(0xffffffffu, run[kind], offset);
+      if (lane >= offset) run[kind] += other;
+    }
+    if (lane == 31) before[kind][warp] = run[kind];
+  }
+  __syncthreads();
+  int* plans[2] = {few, many};
+#pragma unroll
+  for (int kind = 0; kind < 2; ++kind) {
+    const int size = kind ? MXP_TILE : few_tile, most = kind ? max_many : max_few;
+    int at = run[kind] - tiles[kind], all = 0;
+    for (int w = 0; w < 32; ++w) {
+      if (w < warp) at += before[kind][w];
+      all += before[kind][w];
+    }
+    if (e == 0) {
+      plans[kind][0] = min(all, most);
+      if (all > most) atomicOr(error_word, SRB_FLAG_BAD_SLOT);
+    }
+    if (e < experts) plans[kind][1 + e] = first;
+    if (e == experts - 1) plans[kind][1 + experts] = first + slots;
+    int* list = plans[kind] + 1 + experts + 1;
+    for (int t = 0; t < tiles[kind]; ++t)
+      if (at + t < most) {
+        list[2 * (at + t)] = e;
+        list[2 * (at + t) + 1] = first + t * size;
+      }
+  }
+}
+extern "C" int srb_mx4_divide_plan(const int* plan, int experts, int limit, int few_tile, int max_few, int max_many, int* few, int* many, int* error_word,
+                                   void* stream) {
+  if (experts <= 0 || experts > 1024) SRB_FAIL("mx4_divide_plan: %d experts are outside 1 .. 1024", experts);
+  if (limit < 0 || few_tile <= 0) SRB_FAIL("mx4_divide_plan: experts of up to %d slots in tiles of %d", limit, few_tile);
+  SRB_CUDA_CALL(srb_launch(mx4_divide_plan_kernel, dim3(1), dim3(1024), 0, (cudaStream_t)stream, plan, experts, limit, few_tile, max_few, max_many, few, many,
+                           error_word));
+  return SRB_OK;
 }

@@ -287,13 +287,12 @@ struct Mx4Scratch {
 
 // What a call on the experts has, for both libraries.
 struct Mx4ExpertsCall {
-  const void* h;                 // bfloat16 [rows, width]
-  const int *plan, *slot_row, *entry_slot;
-  const float* weights;          // [rows, top]
+  const void* h;                 // bfloat16 rows of `width`
+  const int *plan, *slot_row;
   const void *up, *up_scales;    // [experts, 2 * inner or inner, width]
   const void *down, *down_scales;// [experts, width, inner]
-  void* out;                     // bfloat16 [rows, width]
-  int rows, top, max_tiles, experts, width, inner, gated, activation;
+  float* y;                      // [slots, width]
+  int max_tiles, slots, experts, width, inner, gated, activation;
   float act_param;
   int* error_word;
   cudaStream_t stream;

@@ -25,20 +25,28 @@ MX4_FEW_ROWS = 64
 #: ... and rows of bfloat16 up to this many there too, where the pairs' tiles would leave half of the pairs idle (4,096 x 4,096: 128 rows 14 and
 #: 20, 192 rows 20 and 21, 256 rows 22 and 21; 12,288 x 4,096: 192 rows 48 and 49; 2,048 x 2,048: 192 rows 9 and 13)
 MX4_FEW_ROWS_OF_SMALL = 192
-#: Experts' products run on pairs of CTAs where a step has more choices per expert than this (64 experts of 2,048 x 1,408: 32 choices 158 and 214, 48
-#: 223 and 225, 64 283 and 247; smaller ones cross above 96: 32 of 1,024 x 1,024 at 96 108 and 107, 8 of 1,024 x 512 30 and 43)
-MX4_FEW_CHOICES = 48
+#: The experts' products run on the kernel for few rows while choices per expert * bytes of an expert's codes stay below this (that kernel reads an expert's
+#: matrices, from L2, for every 8 of its rows; us, it and pairs: 64 experts of 2,048 x 1,408 with 32 choices each 160 and 221, 48 227 and 231; 32 of
+#: 1,024 x 1,024 with 64 82 and 106, 96 109 and 111; 16 of 2,048 x 704 with 64 62 and 84, 96 85 and 91; 8 of 1,024 x 512 with 96 29 and 41, 192 43 and 46)
+MX4_FEW_BYTES = 160 << 20
+#: above it, from this many experts on, they are divided on the device, those with up to MX4_FEW_SLOTS rows going to the kernel for few rows all the same: a tile
+#: of 256 rows costs the pairs as much with one row (all on pairs and divided, choices spread unevenly: 64 experts of 2,048 x 1,408 with 48 each 231 and 199,
+#: 192 376 and 356, and 433 and 392 again and again, where the chip's power limit counts; 32 of 1,024 x 1,024 with 64 106 and 94; but 8 of 1,024 x 512
+#: with 48 44 and 57: three launches more)
+MX4_DIVIDE_EXPERTS = 32
+MX4_FEW_SLOTS = 48
 
 _P, _I, _L, _F = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_float
 _LINEAR = (_P, _L, _P, _P, _P, _P, _P, _L, _I, _I, _I, _I, _P, _P, _P)
-_EXPERTS = (_P,) * 10 + (_I,) * 8 + (_F, _P, _P, _P)
+_EXPERTS = (_P,) * 8 + (_I,) * 7 + (_F, _P, _P, _P)
 #: entry points by library and their arguments, declared once: a small call costs as long on the host as on the device
 _SIGNATURES = {
     "mx4": {"srb_mx4_quantize": (_P, _L, _L, _I, _I, _I, _P, _P, _I, _P), "srb_mx4_dequantize": (_P, _P, _I, _I, _I, _P, _I, _P)},
     "gemm_mx4": {"srb_mx4_linear": _LINEAR, "srb_mx4_experts": _EXPERTS, "srb_mx4_linear_scratch": (_I,) * 2,
-                 "srb_mx4_experts_scratch": (_I,) * 6, "srb_mx4_experts_tile": ()},
+                 "srb_mx4_experts_scratch": (_I,) * 5, "srb_mx4_experts_tile": (), "srb_mx4_combine": (_P, _P, _P, _I, _I, _I, _P, _P)},
     "gemm_mx4_pair": {"srb_mx4_linear_pair": _LINEAR, "srb_mx4_experts_pair": _EXPERTS, "srb_mx4_linear_pair_scratch": (_I,) * 2,
-                      "srb_mx4_experts_pair_scratch": (_I,) * 6, "srb_mx4_experts_pair_tile": ()},
+                      "srb_mx4_experts_pair_scratch": (_I,) * 5, "srb_mx4_experts_pair_tile": (),
+                      "srb_mx4_divide_plan": (_P, _I, _I, _I, _I, _I, _P, _P, _P, _P)},
     "route_groups": {"srb_route_groups": (_P, _L, _I, _I, _P, _I, _I, _I, _I, _I, _I, _F, _F, _P, _P, _P)},
 }
 _declared: dict = {}
@@ -304,24 +312,44 @@ def chosen_experts_mx4(h: torch.Tensor, chosen: torch.Tensor, weights: torch.Ten
     if rows == 0 or top == 0:
         return torch.zeros((rows, width), dtype=torch.bfloat16, device=h.device)
     out = torch.empty_like(h)
-    entries, stream = rows * top, _stream()
+    entries, stream, error = rows * top, _stream(), error_word.data_ptr()
     # (the pairs' result rows start on 16-byte borders)
-    many = entries > MX4_FEW_CHOICES * experts and width % 4 == 0
-    moe, lib = load_library("moe"), _library("gemm_mx4_pair" if many else "gemm_mx4")
-    experts_of, needed, tile = ((lib.srb_mx4_experts_pair, lib.srb_mx4_experts_pair_scratch, lib.srb_mx4_experts_pair_tile) if many
-                                else (lib.srb_mx4_experts, lib.srb_mx4_experts_scratch, lib.srb_mx4_experts_tile))
-    tile = tile()
-    # a tile has a slot at least
-    tiles = min(entries, entries // tile + experts)
-    # one piece of memory: the plan, the row of every slot, the slot of every choice, and what the products need
-    plan_bytes, entry_bytes = _room(4 * moe.srb_moe_plan_ints_of(rows, top, experts, tile)), _room(4 * entries)
-    memory = torch.empty(plan_bytes + 2 * entry_bytes + needed(entries, tiles, experts, width, inner, gated), dtype=torch.uint8, device=h.device)
-    plan = memory.data_ptr()
-    slot_row, entry_slot, scratch = plan + plan_bytes, plan + plan_bytes + entry_bytes, plan + plan_bytes + 2 * entry_bytes
-    _check(moe, moe.srb_moe_plan_of(_P(chosen.data_ptr()), rows, top, experts, tile, _P(plan), _P(slot_row), _P(entry_slot), None, None,
-                                    _P(error_word.data_ptr()), stream if isinstance(stream, _P) else _P(stream)))
-    launches = 4 + int(gated and (many or inner % 128 != 0))
-    _check(lib, experts_of(h.data_ptr(), plan, slot_row, entry_slot, weights.data_ptr(), w_gate_up.codes.data_ptr(), w_gate_up.scales.data_ptr(),
-                           w_down.codes.data_ptr(), w_down.scales.data_ptr(), out.data_ptr(), rows, top, tiles, experts, width, inner, gated, act_code,
-                           activation_param, scratch, error_word.data_ptr(), stream), launches)
+    many = entries * (w_gate_up.codes.numel() + w_down.codes.numel()) > MX4_FEW_BYTES * experts * experts and width % 4 == 0
+    divided = many and experts >= MX4_DIVIDE_EXPERTS
+    moe, lib, pair = load_library("moe"), _library("gemm_mx4"), _library("gemm_mx4_pair") if many else None
+    few_tile = lib.srb_mx4_experts_tile()
+    tile = pair.srb_mx4_experts_pair_tile() if many else few_tile
+    # a tile has a slot at least; divided, an expert of the pairs has more than MX4_FEW_SLOTS, one of the others no more
+    tiles = min(entries, entries // tile + (min(experts, entries // (MX4_FEW_SLOTS + 1)) if divided else experts))
+    few_tiles = min(entries, entries // few_tile + experts, experts * -(-MX4_FEW_SLOTS // few_tile)) if divided else 0 if many else tiles
+    # one piece of memory: the plan, the row of every slot, the slot of every choice, the slots' results, and what the products need
+    memory = []
+
+    def take(size: int) -> int:
+        memory.append(_room(size))
+        return sum(memory[:-1])
+    plan_at, slot_row_at = take(4 * moe.srb_moe_plan_ints_of(rows, top, experts, tile)), take(4 * entries)
+    entry_slot_at, y_at = take(4 * entries), take(4 * entries * width)
+    few_at = take(lib.srb_mx4_experts_scratch(few_tiles, experts, width, inner, gated))
+    if many:
+        pair_at = take(pair.srb_mx4_experts_pair_scratch(tiles, experts, width, inner, gated))
+    if divided:
+        few_plan_at, pair_plan_at = take(4 * (experts + 2 + 2 * few_tiles)), take(4 * (experts + 2 + 2 * tiles))
+    held = torch.empty(sum(memory), dtype=torch.uint8, device=h.device)
+    at = held.data_ptr()
+    plan, slot_row, entry_slot, y = at + plan_at, at + slot_row_at, at + entry_slot_at, at + y_at
+    _check(moe, moe.srb_moe_plan_of(_P(chosen.data_ptr()), rows, top, experts, tile, _P(plan), _P(slot_row), _P(entry_slot), None, None, _P(error),
+                                    stream if isinstance(stream, _P) else _P(stream)))
+    matrices = (w_gate_up.codes.data_ptr(), w_gate_up.scales.data_ptr(), w_down.codes.data_ptr(), w_down.scales.data_ptr(), y)
+    sizes = (entries, experts, width, inner, gated, act_code, activation_param)
+    few_plan = pair_plan = plan
+    if divided:
+        few_plan, pair_plan = at + few_plan_at, at + pair_plan_at
+        _check(pair, pair.srb_mx4_divide_plan(plan, experts, MX4_FEW_SLOTS, few_tile, few_tiles, tiles, few_plan, pair_plan, error, stream))
+    if few_tiles:
+        _check(lib, lib.srb_mx4_experts(h.data_ptr(), few_plan, slot_row, *matrices, few_tiles, *sizes, at + few_at, error, stream),
+               3 + int(gated and inner % 128 != 0))
+    if many:
+        _check(pair, pair.srb_mx4_experts_pair(h.data_ptr(), pair_plan, slot_row, *matrices, tiles, *sizes, at + pair_at, error, stream), 3 + int(gated))
+    _check(lib, lib.srb_mx4_combine(y, entry_slot, weights.data_ptr(), rows, top, width, out.data_ptr(), stream))
     return out

@@ -6,6 +6,7 @@ import torch
 
 import plain_mx4 as pm
 from sglang_rs_b200 import ops
+from sglang_rs_b200.ops import mx4
 
 pytestmark = pytest.mark.gpu
 
@@ -387,6 +388,30 @@ def expert_case(seed, rows, experts, width, inner, top, gated=True):
                                                           (90, 2, 192, 192, 1), (90, 2, 192, 224, 1)])
 def test_experts(rows, experts, width, inner, top):
     check_experts(*expert_case(30 + rows, rows, experts, width, inner, top))
+
+
+KERNELS = dict(few=dict(MX4_FEW_BYTES=1 << 62), pairs=dict(MX4_FEW_BYTES=0, MX4_DIVIDE_EXPERTS=1 << 20),
+               divided=dict(MX4_FEW_BYTES=0, MX4_DIVIDE_EXPERTS=1, MX4_FEW_SLOTS=20))
+
+
+@pytest.mark.parametrize("kernels", KERNELS)
+@pytest.mark.parametrize("rows,experts,width,inner,top", [(1, 4, 64, 32, 1), (70, 4, 96, 144, 2), (130, 12, 264, 136, 2), (200, 8, 1540, 48, 4), (90, 2, 192, 224, 1)])
+def test_experts_on_each_kernel(rows, experts, width, inner, top, kernels, monkeypatch):
+    for name, value in KERNELS[kernels].items():
+        monkeypatch.setattr(mx4, name, value)
+    h, chosen, weights, up, down = expert_case(80 + rows, rows, experts, width, inner, top)
+    if experts > top:
+        chosen[: rows * 3 // 4][chosen[: rows * 3 // 4] == experts - 1] = 0      # few rows for one of them
+    check_experts(h, chosen, weights, up, down)
+    check_experts(*expert_case(81 + rows, rows, experts, width, inner, top, gated=False), "gelu_tanh", gated=False)
+
+
+@pytest.mark.parametrize("rows,four", [(3, False), (3, True), (200, False), (200, True)])
+def test_products_on_the_other_kernel(rows, four, monkeypatch):
+    monkeypatch.setattr(mx4, "MX4_FEW_ROWS", 1000 if rows > 64 else 0)
+    monkeypatch.setattr(mx4, "MX4_FEW_ROWS_OF_SMALL", 0)
+    x, (matrix, w) = rows_of(rows, rows, 520), random_matrix(90, 330, 520)
+    check_linear(ops.quantize_mx4(x) if four else x, matrix, w)
 
 
 @pytest.mark.parametrize("rows", [5, 100])
