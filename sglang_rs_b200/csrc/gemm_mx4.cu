@@ -5,7 +5,7 @@
 // every instruction the SMs issue.  A row of bfloat16 is eight rows of four bits here (mx4.cuh, PARTS), columns of their own whose sums the
 // epilogue adds: the tensor cores have time for that, a step with few rows being bound by the bytes of W.  (As two eight-bit parts, kind
 // mxf8f6f4, W's entries have to stand 16 to 16 bytes in shared memory; TMA sets them so, but in pieces of 64 bytes, half of what it moves
-// otherwise: LATER.)
+// otherwise, and the matrices of 8 rows' experts, 64 of 2,048 x 1,408, took 66 us instead of 33.)
 //
 // One row the blocks turn into parts themselves, in the four warps that wait for the sums otherwise: a launch less (one row through 4,096 x 24,576 12.1 us
 // instead of 13.8, 12,288 x 4,096 8.5 instead of 9.7; two rows 15.4 and 11.1 us: they keep the warps longer than the launch takes).
@@ -35,7 +35,6 @@ SRB_DEFINE_PDL_SWITCH()
 #define MXF_TOKENS 64            // rows of X of a tile, at most: in four bits
 #define MXF_PART_TOKENS 16       // ... in parts
 #define MXF_SLOTS 8              // ... over experts
-#define MXF_FUSED_TOKENS 1       // up to as many rows of bfloat16 are turned into parts by the product's own blocks
 #define MXF_THREADS 192
 #define MXF_EPILOGUE_THREADS 128
 #define MXF_W_BYTES 16384        // 128 rows x 256 entries
@@ -48,8 +47,7 @@ SRB_DEFINE_PDL_SWITCH()
 #define MXF_ACT 5      // ... of act(x w^T)
 
 struct FewArgs {
-  const __nv_bfloat16* x;        // FUSED: rows of bfloat16, `ldx` elements apart, of `width` entries; on 16-byte borders if x_wide
-  size_t ldx;
+  const __nv_bfloat16* x;        // FUSED: the one row of bfloat16, of `width` entries, on a 16-byte border if x_wide
   int width, x_wide;
   const float* bias;
   void* out;
@@ -107,9 +105,9 @@ __device__ __forceinline__ unsigned few_transpose(unsigned word, int lane) {
   return word;
 }
 
-// 256 entries of a row of X, 8 a lane, as parts (mx4.cuh) in a stage: rows 8 * token .. + 7 of 128 bytes, swizzled, and their scales, a byte for
-// each 32 entries in each part's word of the two tiles of 128 entries.
-__device__ __forceinline__ void few_make_parts(const uint4& raw, int token, int lane, unsigned x_to, unsigned xs_to) {
+// 256 entries of a row of X, 8 a lane, as parts (mx4.cuh) in a stage: rows 0 .. 7 of 128 bytes, swizzled, and their scales, a byte for each 32 entries
+// in each part's word of the two tiles of 128 entries.
+__device__ __forceinline__ void few_make_parts(const uint4& raw, int lane, unsigned x_to, unsigned xs_to) {
   float v[8];
   mx4_unpack_bf16(raw, v);
   unsigned most = 0u;
@@ -122,11 +120,10 @@ __device__ __forceinline__ void few_make_parts(const uint4& raw, int token, int 
   for (int i = 0; i < 8; ++i) v[i] = mx4_over_first_scale(v[i], first);
 #pragma unroll
   for (int part = 0; part < MX4_PARTS; ++part) {
-    const unsigned row = (unsigned)(token * MX4_PARTS + part);
-    asm volatile("st.shared.b32 [%0], %1;" ::"r"(x_to + row * 128 + ((((unsigned)lane >> 2) ^ (row & 7u)) << 4) + (lane & 3) * 4), "r"(mx4_next_part(v)) : "memory");
+    const unsigned row = (unsigned)part;
+    asm volatile("st.shared.b32 [%0], %1;" ::"r"(x_to + row * 128 + ((((unsigned)lane >> 2) ^ row) << 4) + (lane & 3) * 4), "r"(mx4_next_part(v)) : "memory");
     if ((lane & 3) == 0)
-      asm volatile("st.shared.u8 [%0], %1;" ::"r"(xs_to + (lane >> 4) * 512 + (row & 31u) * 16 + (row >> 5) * 4 + ((lane >> 2) & 3)),
-                   "r"(mx4_part_scale(first, part)) : "memory");
+      asm volatile("st.shared.u8 [%0], %1;" ::"r"(xs_to + (lane >> 4) * 512 + row * 16 + ((lane >> 2) & 3)), "r"(mx4_part_scale(first, part)) : "memory");
   }
 }
 
@@ -179,7 +176,7 @@ mx4_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
   if (threadIdx.x == 0) {
     abort_flag = 0;
     for (int s = 0; s < STAGES; ++s) {
-      mbar_init(smem_u32(&full_bar[s]), FUSED ? 1 + a.tokens : 1);
+      mbar_init(smem_u32(&full_bar[s]), FUSED ? 2 : 1);
       mbar_init(smem_u32(&empty_bar[s]), 1);
     }
     for (int b = 0; b < 2; ++b) {
@@ -304,29 +301,27 @@ mx4_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
       const FewTile t = few_tile<GROUPED>(a, item);
       const int feature = t.feature0 + in_tile;
       if (FUSED) {
-        // a step's 256 entries of a row at a time, by the four warps in turn, the next ones on their way while these become parts
-        auto load = [&](int job) {
-          const int k = (step0 + job / a.tokens) * 256 + lane * 8;
-          const __nv_bfloat16* src = a.x + (size_t)(job % a.tokens) * a.ldx + k;
+        // the row's parts, a step's 256 entries at a time by the four warps in turn, the next ones on their way while these are made
+        auto load = [&](int i) {
+          const int k = (step0 + i) * 256 + lane * 8;
           uint4 raw = make_uint4(0u, 0u, 0u, 0u);
-          if (a.x_wide && k + 8 <= a.width) return *reinterpret_cast<const uint4*>(src);
+          if (a.x_wide && k + 8 <= a.width) return *reinterpret_cast<const uint4*>(a.x + k);
           unsigned short* to = reinterpret_cast<unsigned short*>(&raw);
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
-            if (k + i < a.width) to[i] = reinterpret_cast<const unsigned short*>(src)[i];
+          for (int j = 0; j < 8; ++j)
+            if (k + j < a.width) to[j] = reinterpret_cast<const unsigned short*>(a.x)[k + j];
           return raw;
         };
-        const int jobs = steps * a.tokens;
         uint4 raw = make_uint4(0u, 0u, 0u, 0u), next = raw;
         bool ok = true;
-        if (warp - 2 < jobs) raw = load(warp - 2);
-        for (int job = warp - 2; job < jobs; job += 4, raw = next) {
-          const unsigned round = (unsigned)(local * steps + job / a.tokens);
+        if (warp - 2 < steps) raw = load(warp - 2);
+        for (int i = warp - 2; i < steps; i += 4, raw = next) {
+          const unsigned round = (unsigned)(local * steps + i);
           const int s = (int)(round % STAGES);
-          if (job + 4 < jobs) next = load(job + 4);
+          if (i + 4 < steps) next = load(i + 4);
           ok = mbar_wait_warp(smem_u32(&empty_bar[s]), ((round / STAGES) & 1u) ^ 1u, &abort_flag);
           if (!ok) break;
-          few_make_parts(raw, job % a.tokens, lane, stages + s * stage_bytes + Shape::SIDES * MXF_W_BYTES, scales + s * Shape::SCALE_BYTES + 1024 * Shape::SIDES);
+          few_make_parts(raw, lane, stages + s * stage_bytes + Shape::SIDES * MXF_W_BYTES, scales + s * Shape::SCALE_BYTES + 1024 * Shape::SIDES);
           fence_proxy_async_shared();
           __syncwarp();
           if (lane == 0) mbar_arrive(smem_u32(&full_bar[s]));
@@ -450,7 +445,7 @@ static int launch_few(const void* x, const void* x_scales, long long x_rows, con
 
 // ---- entries: `scratch` has srb_mx4_linear_scratch bytes (none are needed for rows in four bits) ----------------------------
 extern "C" long long srb_mx4_linear_scratch(int rows, int width) {
-  if (rows <= MXF_FUSED_TOKENS) return 0;
+  if (rows == 1) return 0;
   Mx4Scratch scratch = {};
   scratch.take((size_t)rows * MX4_PARTS * mx4_pitch(width));
   scratch.take((size_t)mx4_tiles(rows * MX4_PARTS) * mx4_tiles(width) * MX4_TILE_BYTES);
@@ -473,8 +468,8 @@ extern "C" int srb_mx4_linear(const void* x, long long ldx, const void* x_scales
   cudaStream_t s = (cudaStream_t)stream;
   if (!parts)
     return out_float ? launch_few<false, MXF_F32, false>(x, x_scales, rows, w, w_scales, a, s) : launch_few<false, MXF_BF16, false>(x, x_scales, rows, w, w_scales, a, s);
-  if (rows <= MXF_FUSED_TOKENS) {
-    a.x = (const __nv_bfloat16*)x; a.ldx = (size_t)ldx; a.width = width; a.x_wide = mx4_wide(x, ldx);
+  if (rows == 1) {
+    a.x = (const __nv_bfloat16*)x; a.width = width; a.x_wide = mx4_wide(x, 0);
     return out_float ? launch_few<true, MXF_F32, false, true>(x, nullptr, 8ll * rows, w, w_scales, a, s)
                      : launch_few<true, MXF_BF16, false, true>(x, nullptr, 8ll * rows, w, w_scales, a, s);
   }

@@ -13,7 +13,6 @@
 #include <stdint.h>
 
 #define MX4_TILE_BYTES 512       // scales of 128 rows x 128 entries
-#define MX4_BLOCK 32
 
 __host__ __device__ __forceinline__ int mx4_tiles(int n) { return (n + 127) / 128; }
 // 64 bytes per 128 entries begun
@@ -27,13 +26,6 @@ __host__ __device__ __forceinline__ size_t mx4_scale_word(int row, int kt, int k
 __device__ __forceinline__ float mx4_scale_value(unsigned s) {
   return s == 255u ? __uint_as_float(0x7fc00000u) : s == 0u ? __uint_as_float(0x00400000u) : __uint_as_float(s << 23);
 }
-// the value of a code: below 1 the half is the only one
-__device__ __forceinline__ float mx4_code_value(unsigned code) {
-  const unsigned magnitude = code & 7u;
-  const float v = magnitude < 2u ? 0.5f * (float)magnitude : __uint_as_float(((126u + (magnitude >> 1)) << 23) | ((magnitude & 1u) << 22));
-  return code & 8u ? -v : v;
-}
-
 __device__ __forceinline__ void mx4_unpack_bf16(const uint4& raw, float (&v)[8]) {
   const unsigned w[4] = {raw.x, raw.y, raw.z, raw.w};
 #pragma unroll

@@ -37,14 +37,6 @@ __device__ __forceinline__ void tmem_copy_scales(unsigned tmem, unsigned long lo
 __device__ __forceinline__ unsigned long long scales_descriptor(unsigned address) {
   return (unsigned long long)((address & 0x3ffffu) >> 4) | ((unsigned long long)(128u >> 4) << 32) | (1ull << 46);
 }
-__device__ __forceinline__ void tmem_load_8(unsigned address, float (&v)[8]) {
-  unsigned r[8];
-  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]) : "r"(address) : "memory");
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(r[i]);
-}
 
 // Lets the kernel have that much shared memory, once for a device and a size (`allowed`: what a device was told last).
 #define MX4_MAX_DEVICES 64

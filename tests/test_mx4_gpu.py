@@ -169,6 +169,14 @@ def test_products_with_a_bias_and_in_32_bits(rows, width, features, four):
     check_linear(x, matrix, w, bias, torch.float32)
 
 
+@pytest.mark.parametrize("rows,four", [(1, False), (1, True), (2, False), (20, False), (64, True)])
+def test_more_tiles_than_blocks(rows, four):
+    """A head's many features: every block takes several tiles, the sums of one stored while the next one's are taken."""
+    x = rows_of(rows, rows, 264)
+    matrix, w = random_matrix(91, 79 * 1024 + 3, 264)
+    check_linear(ops.quantize_mx4(x) if four else x, matrix, w)
+
+
 @pytest.mark.parametrize("rows", [3, 40, 200])
 def test_rows_of_a_wider_matrix(rows):
     wide = rows_of(6, rows, 700)
@@ -395,7 +403,8 @@ KERNELS = dict(few=dict(MX4_FEW_BYTES=1 << 62), pairs=dict(MX4_FEW_BYTES=0, MX4_
 
 
 @pytest.mark.parametrize("kernels", KERNELS)
-@pytest.mark.parametrize("rows,experts,width,inner,top", [(1, 4, 64, 32, 1), (70, 4, 96, 144, 2), (130, 12, 264, 136, 2), (200, 8, 1540, 48, 4), (90, 2, 192, 224, 1)])
+@pytest.mark.parametrize("rows,experts,width,inner,top", [(1, 4, 64, 32, 1), (70, 4, 96, 144, 2), (130, 12, 264, 136, 2), (200, 8, 1540, 48, 4), (90, 2, 192, 224, 1),
+                                                          (200, 9, 256, 640, 4)])
 def test_experts_on_each_kernel(rows, experts, width, inner, top, kernels, monkeypatch):
     for name, value in KERNELS[kernels].items():
         monkeypatch.setattr(mx4, name, value)
