@@ -57,11 +57,12 @@ __device__ __forceinline__ unsigned long long route_most(unsigned long long key)
 
 // Whether 32-bit numbers do not tell which of two picks (or sums of two) is larger, `above` being the larger one of them.  `by_logit`: they are the logits
 // themselves, whose order is that of the scores but where the 64-bit scores are alike: both 0, or sigmoids within 2^-53 of 1.  Otherwise
-// they are off by 2^-20 of the scores that went in, or, in a softmax, 2^-19: its exponential's argument is off by 2^-24 of its size,
-// which is below 24 where the score is above 2^-34; smaller picks always count as near.
+// they are off by at most 1.25 2^-22 of the scores that went in (the exponential by 2^-23 of itself, the sum under the division, the division and the sum
+// with the bias by 2^-24 each), or, in a softmax, 2^-20: its exponential's argument is off by 2^-24 of its size, which is below 24 where
+// the score is above 2^-34, the sum by 2^-22 and the quick division by 2^-22; smaller picks always count as near.
 __device__ __forceinline__ bool route_near(float above, float below, float bias_most, float most, bool by_logit, int scoring) {
   if (by_logit) return !(below - (scoring == ROUTE_SOFTMAX ? most : 0.f) > -700.f) || (scoring == ROUTE_SIGMOID && above > 16.f && above - below < 1.f && above != below);
-  const float room = (fabsf(above) + fabsf(below) + 2.f * bias_most) * (scoring == ROUTE_SOFTMAX ? 1.9073486e-6f : 9.5367432e-7f);
+  const float room = (fabsf(above) + fabsf(below) + 2.f * bias_most) * (scoring == ROUTE_SOFTMAX ? 1.9073486e-6f : 3.6e-7f);
   return !(above - below > room) || (bias_most == 0.f && below < 5.8207661e-11f);
 }
 
@@ -90,7 +91,7 @@ __device__ __forceinline__ int route_choose(const float (&z)[PER], const float* 
   for (int j = 0; j < PER; ++j) {
     const int e = lane + 32 * j;
     float pick = z[j];
-    if (!by_logit) pick = rule.scoring == ROUTE_SOFTMAX ? expf(pick - most) * over_sum : __fdividef(1.0f, 1.0f + expf(-pick));
+    if (!by_logit) pick = rule.scoring == ROUTE_SOFTMAX ? expf(pick - most) * over_sum : 1.0f / (1.0f + expf(-pick));
     if (bias && e < rule.experts) {
       const float b = __ldg(bias + e);
       bias_most = fmaxf(bias_most, fabsf(b));
@@ -174,8 +175,8 @@ __device__ __forceinline__ int route_choose(const float (&z)[PER], const float* 
   return choice;
 }
 
-// The same by 64-bit scores, for the few rows that need it: loops over the keys in shared memory and no code laid out flat, since a warp that comes here
-// waits for the instructions to be fetched.
+// The same by 64-bit scores, for the few rows that need it: loops over the keys in shared memory, with little code laid out flat, since a warp that comes
+// here waits for the instructions to be fetched.
 __device__ __noinline__ int route_choose_exactly(const float* __restrict__ z, const float* __restrict__ bias, const GroupRule& rule, unsigned long long* keys,
                                                  int lane) {
   double most = -INFINITY, sum = 0.0;
@@ -188,7 +189,7 @@ __device__ __noinline__ int route_choose_exactly(const float* __restrict__ z, co
 #pragma unroll 1
     for (int offset = 16; offset > 0; offset >>= 1) sum += __shfl_xor_sync(ALL, sum, offset);
   }
-#pragma unroll 1
+#pragma unroll 4
   for (int e = lane; e < rule.experts; e += 32) {
     const bool softmax = rule.scoring == ROUTE_SOFTMAX;
     const double power = exp(softmax ? (double)z[e] - most : -(double)z[e]);
@@ -228,7 +229,7 @@ __device__ __noinline__ int route_choose_exactly(const float* __restrict__ z, co
   for (int k = 0; k < rule.top; ++k) {
     unsigned long long best = 0;
     unsigned index = 0x7fffffffu;
-#pragma unroll 1
+#pragma unroll 4
     for (int e = lane; e < rule.experts; e += 32)
       if (keys[e] > best) { best = keys[e]; index = (unsigned)e; }
     index = __reduce_min_sync(ALL, best == route_most(best) ? index : 0x7fffffffu);

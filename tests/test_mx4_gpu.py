@@ -316,6 +316,24 @@ def test_choices(case, rows):
     check_choice(logits, case, bias)
 
 
+@pytest.mark.parametrize("case", [c for c in CHOICES if c["experts"] <= 257])
+def test_choices_of_more_rows_than_warps(case):
+    """Rows in pairs, the last by itself: the same as in small calls."""
+    rows = 44 * torch.cuda.get_device_properties(0).multi_processor_count + 1
+    logits = torch.randn(rows, case["experts"], generator=generator(92)).cuda() * 2
+    logits[::97] = 0.5
+    logits[5, ::2], logits[6, 1::2] = math.nan, -math.inf
+    bias = torch.randn(case["experts"], generator=generator(3)).cuda() * case["bias"] if "bias" in case else None
+    options = dict(scoring=case.get("scoring", "softmax"), choice_bias=bias, groups=case.get("groups", 1), top_groups=case.get("top_groups", 1),
+                   group_best=case.get("group_best", 1))
+    chosen, weights = ops.choose_experts(logits, case["top"], True, **options)
+    for first in range(0, rows, 1024):
+        few, same = ops.choose_experts(logits[first:first + 1024], case["top"], True, **options)
+        assert torch.equal(chosen[first:first + 1024], few)
+        assert torch.equal(weights[first:first + 1024].nan_to_num(7.0), same.nan_to_num(7.0))
+    check_choice(logits[-300:], case, bias)
+
+
 @pytest.mark.parametrize("case", CHOICES)
 def test_choices_between_equals_and_all_but_equals(case):
     experts = case["experts"]
