@@ -12,7 +12,7 @@
 //
 // Over experts (GROUPED) a tile is up to 256 slots of one expert (the plan of csrc/moe.cu); X and the parts that the gated mode leaves have room
 // for 256 rows a tile, so that a tile's scales are whole tiles.  Gated: the even CTA brings gate rows, the odd one the up rows of the same 96 features,
-// whose scales come regrouped (srb_mx4_gated_scales: 96 and 96 rows are no whole tiles; a word a row by cp.async instead kept the tensor cores
+// whose scales come regrouped (mx4_gated_scales_kernel: 96 and 96 rows are no whole tiles; a word a row by cp.async instead kept the tensor cores
 // waiting, 296 us instead of some 215 for the gate/up of 12,288 slots, 64 experts of 2,048 x 1,408).
 //
 // Bound by the tensor cores under the chip's power limit: 2,048 rows of bfloat16 through 4,096 x 24,576 in 262 us for some milliseconds (1,570 TFLOP/s of

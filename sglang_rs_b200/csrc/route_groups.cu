@@ -8,12 +8,14 @@
 //   weight  the chosen scores, divided by (their sum + norm_eps) if `renormalize`, times `scale`
 //
 // Which of two picks is larger may hang on their last bits, and a choice is whole numbers: it is that of 64-bit scores.  Where nothing is added to
-// the scores, their order is the logits' own and those are compared.  Otherwise the row is chosen by 32-bit scores, and once more by
-// 64-bit ones where two neighbours in that order, or the last open group and the first closed one, are nearer than the scores' error.
+// the scores, their order is the logits' own and those are compared.  Otherwise the row is chosen by 32-bit scores.  Where two neighbours in that order
+// are nearer than the scores' error, the chosen experts and those behind them as near are put in the order of their 64-bit scores; a softmax, and a
+// row where the last open group and the first closed one are as near, is chosen once more by 64-bit scores of all experts.
 //
 // A warp per row, expert lane + 32 j the lane's j-th.  Picks lie in registers as unsigned numbers of the same order, so that a largest one of the
 // warp is one instruction (redux.sync; two for 64 bits) and its lowest index another.  Bound by a row's chain of instructions, some 1,600 for 256
-// experts in 8 groups: 64 rows 6 us, 8,192 rows 24 (their bytes take 1.4); a row that needs 64 bits takes 8 more by itself.
+// experts in 8 groups: 64 rows 6.4 us, 8,192 rows 19 to 20 (their bytes take 1.4; 22 where every
+// doubt costs the whole row); a row that is chosen once more takes 8 to 11 more by itself.
 #include "common.cuh"
 #include <math.h>
 
@@ -56,12 +58,16 @@ __device__ __forceinline__ unsigned long long route_most(unsigned long long key)
 }
 
 // Whether 32-bit numbers do not tell which of two picks (or sums of two) is larger, `above` being the larger one of them.  `by_logit`: they are the logits
-// themselves, whose order is that of the scores but where the 64-bit scores are alike: both 0, or sigmoids within 2^-53 of 1.  Otherwise
+// themselves, whose order is that of the scores but where 64-bit scores are alike: both 0; sigmoids near 1 (2^-53 apart is e^-36, and logits
+// below 36 that are 1 apart differ by more); logits so near 0 that the exponential does not see them apart (below 1e-5 two may be nearer
+// than 9e-13, and an argument of up to 700 is good to 2e-13).  Otherwise
 // they are off by at most 1.25 2^-22 of the scores that went in (the exponential by 2^-23 of itself, the sum under the division, the division and the sum
-// with the bias by 2^-24 each), or, in a softmax, 2^-20: its exponential's argument is off by 2^-24 of its size, which is below 24 where
-// the score is above 2^-34, the sum by 2^-22 and the quick division by 2^-22; smaller picks always count as near.
+// with the bias by 2^-24 each; 2^-24 more where two picks are added), or, in a softmax, 2^-20: its exponential's argument is off by 2^-24 of its size,
+// which is below 24 where the score is above 2^-34, the sum by 2^-22 and the quick division by 2^-22; smaller picks always count as near.
 __device__ __forceinline__ bool route_near(float above, float below, float bias_most, float most, bool by_logit, int scoring) {
-  if (by_logit) return !(below - (scoring == ROUTE_SOFTMAX ? most : 0.f) > -700.f) || (scoring == ROUTE_SIGMOID && above > 16.f && above - below < 1.f && above != below);
+  if (by_logit)
+    return !(below - (scoring == ROUTE_SOFTMAX ? most : 0.f) > -700.f) || (fabsf(above) < 1e-5f && above - below < 9e-13f) ||
+           (scoring == ROUTE_SIGMOID && above > 16.f && !(above - below >= 1.f && below <= 36.f));
   const float room = (fabsf(above) + fabsf(below) + 2.f * bias_most) * (scoring == ROUTE_SOFTMAX ? 1.9073486e-6f : 3.6e-7f);
   return !(above - below > room) || (bias_most == 0.f && below < 5.8207661e-11f);
 }
@@ -78,11 +84,12 @@ __device__ __forceinline__ Key route_group_score(Key first, Key second, int grou
   return route_key(sum == sum ? sum : (decltype(sum))-INFINITY);
 }
 
-// The lane k < top gets the k-th choice by 32-bit scores; it holds unless `near`.  `most` and `sum`: of a softmax.  `picks`: room for a key of
-// every expert.
+// The lane k < top gets the k-th choice by 32-bit scores; it holds unless `near_groups` or `near`: then the groups are in doubt, or the order of the
+// `count` experts that the lanes k < count hold, which go on behind the top ones as long as neighbours are near (32 of them: there may be
+// more).  `most` and `sum`: of a softmax.  `picks`: room for a key of every expert.
 template <int PER>
 __device__ __forceinline__ int route_choose(const float (&z)[PER], const float* __restrict__ bias, const GroupRule& rule, float most, float sum,
-                                            unsigned* picks, int lane, bool& near) {
+                                            unsigned* picks, int lane, bool& near_groups, bool& near, int& count) {
   const bool by_logit = !bias && (rule.group_best == 1 || rule.groups == rule.top_groups);
   unsigned key[PER];
   float bias_most = 0.f;
@@ -90,7 +97,7 @@ __device__ __forceinline__ int route_choose(const float (&z)[PER], const float* 
 #pragma unroll
   for (int j = 0; j < PER; ++j) {
     const int e = lane + 32 * j;
-    float pick = z[j];
+    float pick = z[j] + 0.f;                                 // -0 lies where 0 does
     if (!by_logit) pick = rule.scoring == ROUTE_SOFTMAX ? expf(pick - most) * over_sum : 1.0f / (1.0f + expf(-pick));
     if (bias && e < rule.experts) {
       const float b = __ldg(bias + e);
@@ -100,7 +107,7 @@ __device__ __forceinline__ int route_choose(const float (&z)[PER], const float* 
     key[j] = e < rule.experts ? route_key(pick == pick ? pick : -INFINITY) : 0u;
   }
   if (bias) bias_most = __uint_as_float(__reduce_max_sync(ALL, __float_as_uint(bias_most)));
-  near = false;
+  near_groups = near = false;
   if (rule.groups > rule.top_groups) {
     const int per_group = rule.per_group;
     unsigned mine = 0u;                                      // the score of group `lane`
@@ -137,31 +144,45 @@ __device__ __forceinline__ int route_choose(const float (&z)[PER], const float* 
       __syncwarp();
     }
     unsigned open = 0u;
-    float last = 0.f;
+    float first = 0.f, last = 0.f;
     for (int k = 0; k < rule.top_groups; ++k) {
       const unsigned best = route_most(mine);
+      if (k == 0) first = route_value(best);
       const int g = __ffs(__ballot_sync(ALL, mine == best)) - 1;
       open |= 1u << g;
       if (lane == g) mine = 0u;
       last = route_value(best);
     }
-    near = route_near(last, route_value(route_most(mine)), 2.f * bias_most, most, by_logit, rule.scoring);
+    near_groups = route_near(last, route_value(route_most(mine)), 2.f * bias_most, most, by_logit, rule.scoring);
+    // logits that are all alike are in their order
+    if (near_groups && by_logit) {
+      const float lowest = route_value(__reduce_min_sync(ALL, mine ? mine : ALL));
+      near_groups = !(first == lowest && lowest > -INFINITY);
+    }
 #pragma unroll
     for (int j = 0; j < PER; ++j)
       if (lane + 32 * j < rule.experts && !((open >> ((unsigned)(lane + 32 * j) * rule.group_factor >> 20)) & 1u)) key[j] = 0u;
   }
   int choice = 0;
   float last = 0.f;
-  for (int k = 0; k <= rule.top; ++k) {
+  for (count = 0;; ++count) {
     unsigned mine = 0u;
 #pragma unroll
     for (int j = 0; j < PER; ++j) mine = max(mine, key[j]);
     const unsigned best = route_most(mine);
     if (best == 0u) break;                                   // all are taken
     const float value = route_value(best);
-    if (k > 0) near |= route_near(last, value, bias_most, most, by_logit, rule.scoring);
+    const bool close = count > 0 && route_near(last, value, bias_most, most, by_logit, rule.scoring);
+    if (count >= rule.top && !close) break;
+    near |= close && !(by_logit && last == value && value > -INFINITY);      // equal logits are in their order, a NaN is not at minus infinity's
+    if (count == 32) {                                       // no lane is left: the run goes on as it is, or is in doubt
+      unsigned lowest = ALL;
+#pragma unroll
+      for (int j = 0; j < PER; ++j) lowest = min(lowest, key[j] ? key[j] : ALL);
+      near |= close && __reduce_min_sync(ALL, lowest) != best;
+      break;
+    }
     last = value;
-    if (k == rule.top) break;
     unsigned index = 0x7fffffffu;
 #pragma unroll
     for (int j = PER - 1; j >= 0; --j)
@@ -170,7 +191,7 @@ __device__ __forceinline__ int route_choose(const float (&z)[PER], const float* 
 #pragma unroll
     for (int j = 0; j < PER; ++j)
       if (index == (unsigned)(lane + 32 * j)) key[j] = 0u;
-    if (lane == k) choice = (int)index;
+    if (lane == count) choice = (int)index;
   }
   return choice;
 }
@@ -239,6 +260,27 @@ __device__ __noinline__ int route_choose_exactly(const float* __restrict__ z, co
   return choice;
 }
 
+// The lanes k < count hold experts whose sigmoids go into the order of their 64-bit picks.
+__device__ __noinline__ int route_reorder(const float* __restrict__ z, const float* __restrict__ bias, int choice, int count, int lane) {
+  unsigned long long key = 0;
+  if (lane < count) {
+    double pick = 1.0 / (1.0 + exp(-(double)z[choice]));
+    if (bias) pick += (double)bias[choice];
+    key = route_key(pick == pick ? pick : (double)-INFINITY);
+  }
+  int rank = 0, ordered = choice;
+  for (int i = 0; i < count; ++i) {
+    const unsigned long long other = __shfl_sync(ALL, key, i);
+    const int expert = __shfl_sync(ALL, choice, i);          // by all lanes, before anything depends on the lane
+    rank += other > key || (other == key && expert < choice) ? 1 : 0;
+  }
+  for (int i = 0; i < count; ++i) {
+    const int at = __shfl_sync(ALL, rank, i), expert = __shfl_sync(ALL, choice, i);
+    if (lane == at) ordered = expert;
+  }
+  return ordered;
+}
+
 template <int PER>
 __global__ void __launch_bounds__(32 * ROUTE_WARPS, PER <= 8 ? 10 : 1)
 route_groups_kernel(const float* __restrict__ logits, size_t pitch, int rows, const float* __restrict__ bias, GroupRule rule,
@@ -265,10 +307,15 @@ route_groups_kernel(const float* __restrict__ logits, size_t pitch, int rows, co
       if (lane + 32 * j < rule.experts) sum += expf(z[j] - most);
     sum = srb_warp_sum(sum);
   }
-  bool near;
-  int choice = route_choose<PER>(z, bias, rule, most, sum, reinterpret_cast<unsigned*>(shared), lane, near);
-  // (a softmax over something that is not finite has no scores)
-  if (near || (rule.scoring == ROUTE_SOFTMAX && !(sum < INFINITY))) choice = route_choose_exactly(from, bias, rule, shared, lane);
+  bool near_groups, near;
+  int count;
+  int choice = route_choose<PER>(z, bias, rule, most, sum, reinterpret_cast<unsigned*>(shared), lane, near_groups, near, count);
+  // a few neighbours in doubt are put in order among themselves; groups, more of them, and a softmax, whose sum has all experts in it (and no scores
+  // where something is not finite), take the whole row
+  if (near_groups || (near && (count == 32 || rule.scoring == ROUTE_SOFTMAX)) || (rule.scoring == ROUTE_SOFTMAX && !(sum < INFINITY)))
+    choice = route_choose_exactly(from, bias, rule, shared, lane);
+  else if (near)
+    choice = route_reorder(from, bias, choice, count, lane);
   // the chosen scores, a lane each
   float weight = 0.f;
   if (lane < rule.top) weight = rule.scoring == ROUTE_SOFTMAX ? expf(from[choice] - most) / sum : 1.0f / (1.0f + expf(-from[choice]));

@@ -318,7 +318,7 @@ def test_choices(case, rows):
 
 @pytest.mark.parametrize("case", [c for c in CHOICES if c["experts"] <= 257])
 def test_choices_of_more_rows_than_warps(case):
-    """Rows in pairs, the last by itself: the same as in small calls."""
+    """Many rows: the same as in small calls."""
     rows = 44 * torch.cuda.get_device_properties(0).multi_processor_count + 1
     logits = torch.randn(rows, case["experts"], generator=generator(92)).cuda() * 2
     logits[::97] = 0.5
@@ -343,6 +343,34 @@ def test_choices_between_equals_and_all_but_equals(case):
     logits[20:40] += 2.0 ** -20 * torch.randint(-3, 4, (20, experts), generator=g).float()
     bias = torch.randint(-1, 2, (experts,), generator=g).float().cuda() * case["bias"] if "bias" in case else None
     check_choice(logits.cuda(), case, bias)
+
+
+@pytest.mark.parametrize("groups,top_groups", [(1, 1), (8, 3)])
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("top", [1, 6, 24])
+def test_choices_where_scores_of_unlike_logits_are_alike(scoring, groups, top_groups, top):
+    """Sigmoids of 1 and of 0, exponentials of 1 and of 0: the lower index goes first, as it does between equal logits."""
+    g = generator(41)
+    levels = [torch.tensor([17.0, 30.5, 36.0, 37.0, 38.5, 40.0, 100.0]), torch.tensor([0.0, 1e-20, -1e-20, 3e-25, 1e-39, 0.0, -0.0]),
+              torch.tensor([-720.0, -750.0, -800.0, -900.0, -750.0, -1e4, -math.inf]), torch.tensor([40.0, 38.5, 0.0, 1e-20, -800.0, -900.0, 3.0])]
+    logits = torch.cat([level[torch.randint(0, 7, (40, 64), generator=g)] for level in levels])
+    logits[-3:] = 0.0
+    if scoring == "softmax":
+        logits[80:120, 5] = 1.0                               # a row of minus infinities has no softmax
+    check_choice(logits.cuda(), dict(experts=64, top=top, groups=groups, top_groups=top_groups, scoring=scoring), None)
+
+
+@pytest.mark.parametrize("top", [1, 7, 8, 31, 32])
+def test_choices_in_runs_of_all_but_equals(top):
+    """Runs of five experts whose biased sigmoids are some 2^-24 apart: inside the chosen ones, over their end, and behind the 32nd."""
+    g = generator(42)
+    steps = (torch.arange(64) // 5 * 0.4 - 2.5).double()
+    bias = 0.2 * torch.randn(64, generator=g)
+    logits = torch.empty(200, 64)
+    for row in logits:
+        score = torch.sigmoid(steps[torch.randperm(64, generator=g)]) - bias.double() + 0.3
+        row.copy_(torch.logit(score.clamp(0.01, 0.99)).float())
+    check_choice(logits.cuda(), dict(experts=64, top=top, scoring="sigmoid"), bias.cuda())
 
 
 def test_choices_among_masked_experts():
