@@ -73,7 +73,7 @@ mx4_split_slots_kernel(const __nv_bfloat16* __restrict__ x, int width, const int
                        int max_tiles, uint8_t* __restrict__ parts, uint8_t* __restrict__ scales) {
   srb_launch_dependents();
   srb_grid_dependency_wait();
-  const int tile = blockIdx.y, in_tile = blockIdx.x * (MX4_ROWS_THREADS / 16) + (threadIdx.x >> 4), lane = threadIdx.x & 15;
+  const int tile = blockIdx.x / 16, in_tile = blockIdx.x % 16 * (MX4_ROWS_THREADS / 16) + (threadIdx.x >> 4), lane = threadIdx.x & 15;
   if (tile >= plan[0]) return;
   const int expert = plan[1 + experts + 1 + 2 * tile], slot = plan[1 + experts + 1 + 2 * tile + 1] + in_tile;
   const int end = plan[1 + expert + 1];                      // (a tile's place is below 256)
@@ -137,12 +137,12 @@ mx4_parts_slots_kernel(const __nv_bfloat16* __restrict__ x, int width, const int
                        unsigned* __restrict__ codes, uint8_t* __restrict__ scales) {
   srb_grid_dependency_wait();
   srb_launch_dependents();                                  // (only now: the product starts on what is older than this kernel)
-  const int tile = blockIdx.y, kt = blockIdx.x, in_tile = threadIdx.x >> 4, lane = threadIdx.x & 15;
+  const int k_tiles = mx4_tiles(width), tile = blockIdx.x / k_tiles, kt = blockIdx.x % k_tiles, in_tile = threadIdx.x >> 4, lane = threadIdx.x & 15;
   if (tile >= plan[0]) return;
   const int expert = plan[1 + experts + 1 + 2 * tile], slot = plan[1 + experts + 1 + 2 * tile + 1] + in_tile;
   const bool live = slot < plan[1 + expert + 1];
   const int k = kt * 128 + lane * 8;
-  mx4_parts_of_eight<WIDE>(x + (size_t)(live ? slot_row[slot] : 0) * width + k, width - k, live, lane, (tile * 8 + in_tile) * MX4_PARTS, kt, gridDim.x,
+  mx4_parts_of_eight<WIDE>(x + (size_t)(live ? slot_row[slot] : 0) * width + k, width - k, live, lane, (tile * 8 + in_tile) * MX4_PARTS, kt, k_tiles,
                            codes, scales);
 }
 
@@ -234,8 +234,8 @@ static inline int mx4_launch_split(const void* x, long long pitch, int rows, int
 }
 static inline int mx4_launch_split_slots(const void* x, int width, const int* plan, const int* slot_row, int experts, int max_tiles, uint8_t* parts,
                                   uint8_t* scales, cudaStream_t s) {
-  if (max_tiles > 65535) SRB_FAIL("four-bit experts: %d tiles are too many", max_tiles);
-  SRB_CUDA_CALL(srb_launch(mx4_wide(x, width) ? mx4_split_slots_kernel<true> : mx4_split_slots_kernel<false>, dim3(256 / 16, max_tiles),
+  if (max_tiles > 1 << 22) SRB_FAIL("four-bit experts: %d tiles are too many", max_tiles);
+  SRB_CUDA_CALL(srb_launch(mx4_wide(x, width) ? mx4_split_slots_kernel<true> : mx4_split_slots_kernel<false>, dim3(256 / 16 * max_tiles),
                            dim3(MX4_ROWS_THREADS), 0, s, (const __nv_bfloat16*)x, width, plan, slot_row, experts, max_tiles, parts, scales));
   return SRB_OK;
 }
@@ -249,8 +249,9 @@ static inline int mx4_launch_parts(const void* x, long long pitch, int rows, int
 }
 static inline int mx4_launch_parts_slots(const void* x, int width, const int* plan, const int* slot_row, int experts, int max_tiles, uint8_t* codes,
                                   uint8_t* scales, cudaStream_t s) {
-  if (max_tiles > 65535) SRB_FAIL("four-bit experts: %d tiles are too many", max_tiles);
-  SRB_CUDA_CALL(srb_launch(mx4_wide(x, width) ? mx4_parts_slots_kernel<true> : mx4_parts_slots_kernel<false>, dim3(mx4_tiles(width), max_tiles),
+  const long long blocks = (long long)max_tiles * mx4_tiles(width);
+  if (max_tiles > 1 << 24 || blocks > 0x7fffffff) SRB_FAIL("four-bit experts: %d tiles are too many", max_tiles);
+  SRB_CUDA_CALL(srb_launch(mx4_wide(x, width) ? mx4_parts_slots_kernel<true> : mx4_parts_slots_kernel<false>, dim3((unsigned)blocks),
                            dim3(128), 0, s, (const __nv_bfloat16*)x, width, plan, slot_row, experts, (unsigned*)codes, scales));
   return SRB_OK;
 }

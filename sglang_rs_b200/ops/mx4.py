@@ -19,6 +19,8 @@ from .trace import traced
 
 #: entries of a row that share a scale
 MX4_BLOCK = 32
+#: the largest size of a matrix: the kernels count rows and entries in 32 bits, in whole tiles
+MX4_MOST = 2**31 - 2**16
 #: Up to this many rows a product runs on the kernel that has the weights on the M side (csrc/gemm_mx4.cu), above it on pairs of CTAs (us, that kernel and
 #: pairs, 4,096 x 24,576: 64 rows 30 and 36, 96 rows 39 and 37; both operands in four bits 64 rows 19 and 19, 96 rows 23 and 20) ...
 MX4_FEW_ROWS = 64
@@ -190,6 +192,8 @@ def quantize_mx4(x: torch.Tensor) -> Mx4:
     *lead, rows, width = x.shape
     if width == 0:
         raise KernelError("quantize_mx4: rows without entries")
+    if max(x.shape) > MX4_MOST:
+        raise KernelError(f"quantize_mx4: sizes {tuple(x.shape)} are too large")
     q = Mx4._made(x.new_empty((*lead, rows, 64 * _tiles(width)), dtype=torch.uint8),
                   x.new_empty((*lead, _tiles(rows), _tiles(width), 512), dtype=torch.uint8), width)
     if x.numel():
@@ -205,6 +209,8 @@ def dequantize_mx4(q: Mx4, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     _need_mx4(q, "q", None)
     code = dtype_code(dtype)
     _here("dequantize_mx4", q.codes, q.scales)
+    if max(q.shape) > MX4_MOST:
+        raise KernelError(f"dequantize_mx4: sizes {q.shape} are too large")
     out = q.codes.new_empty(q.shape, dtype=dtype)
     if out.numel():
         lib = _library("mx4")
@@ -237,6 +243,8 @@ def linear_mx4(x, weight: Mx4, error_word: torch.Tensor, *, bias: Optional[torch
     _need(error_word, "error_word", torch.int32)
     out_dtype = torch.bfloat16 if out_dtype is None else out_dtype
     dtype_code(out_dtype)
+    if rows > MX4_MOST or weight.rows > MX4_MOST or width > MX4_MOST:
+        raise KernelError(f"linear_mx4: {rows} rows of {width} and a weight {weight.shape} are too large")
     if weight.width != width:
         raise KernelError(f"linear_mx4: rows of {width} and a weight {weight.shape} do not fit")
     if bias is not None:
@@ -311,8 +319,8 @@ def chosen_experts_mx4(h: torch.Tensor, chosen: torch.Tensor, weights: torch.Ten
     if (w_gate_up.shape != (experts, (2 if gated else 1) * inner, width) or w_down.rows != width or experts < 1 or experts > 1024):
         raise KernelError(f"chosen_experts_mx4: h {tuple(h.shape)}, w_gate_up {w_gate_up.shape} and w_down {w_down.shape} do not fit "
                           "(at most 1024 experts)")
-    if rows * max(top, 1) >= 2**31:
-        raise KernelError(f"chosen_experts_mx4: {rows} rows of {top} choices")
+    if rows * max(top, 1) >= 2**31 or max(width, 2 * inner) > MX4_MOST:
+        raise KernelError(f"chosen_experts_mx4: {rows} rows of {top} choices, width {width}, inner {inner} are too large")
     _here("chosen_experts_mx4", h, chosen, weights, w_gate_up.codes, w_gate_up.scales, w_down.codes, w_down.scales, error_word)
     if rows == 0 or top == 0:
         return torch.zeros((rows, width), dtype=torch.bfloat16, device=h.device)

@@ -289,6 +289,14 @@ def test_refusals():
             call()
 
 
+def test_more_rows_than_the_kernels_count_are_refused():
+    x = torch.empty(2 ** 31 - 1, 1, dtype=torch.bfloat16, device="cuda")
+    matrix, _ = random_matrix(20, 64, 1)
+    for call in (lambda: ops.quantize_mx4(x), lambda: ops.linear_mx4(x, matrix, word())):
+        with pytest.raises(ops.KernelError, match="too large"):
+            call()
+
+
 # ------------------------------------------------------------------------------------------- the router in groups
 CHOICES = [dict(experts=8, top=2), dict(experts=1, top=1), dict(experts=64, top=6, renormalize=True),
            dict(experts=256, top=8, groups=8, top_groups=4, group_best=2, scoring="sigmoid", bias=0.1, renormalize=True, scale=2.5),
@@ -486,6 +494,18 @@ def test_experts_chosen_twice_by_nobody_and_outside(rows):
     assert (got[1] == 0).all()
     everywhere = torch.full_like(chosen, -1)
     assert (check_experts(h, everywhere, weights, up, down) == 0).all()
+
+
+def test_more_tiles_of_experts_than_a_grid_is_high():
+    rows, experts, width, inner = 270_000, 64, 128, 64
+    h = torch.randn(rows, width, generator=generator(61)).bfloat16().cuda()
+    chosen = torch.randint(0, experts, (rows, 2), generator=generator(62), dtype=torch.int32).cuda()
+    weights = torch.rand(rows, 2, generator=generator(63)).cuda()
+    (up, _), (down, _), error = random_matrix(64, experts, 2 * inner, width), random_matrix(65, experts, width, inner), word()
+    got = ops.chosen_experts_mx4(h, chosen, weights, up, down, "silu", error)
+    for some in (slice(0, 500), slice(rows // 2, rows // 2 + 500), slice(rows - 500, rows)):
+        assert torch.equal(got[some], ops.chosen_experts_mx4(h[some], chosen[some], weights[some], up, down, "silu", error))
+    ops.raise_on_error_word(error)
 
 
 def test_experts_of_no_rows_and_of_no_choice():
