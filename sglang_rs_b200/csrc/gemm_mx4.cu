@@ -40,7 +40,6 @@ SRB_DEFINE_PDL_SWITCH()
 #define MXF_W_BYTES 16384        // 128 rows x 256 entries
 #define MXF_MAX_SPLITS 8         // blocks of a cluster
 #define MXF_SUMS 128             // columns of tensor memory: scales lie behind
-#define MXF_PLACES 4             // of a step's scales in tensor memory
 #define MXF_BF16 0     // out bfloat16 = x w^T + bias
 #define MXF_F32 1      // out float
 #define MXF_GATED 2    // out parts of act(x gate^T) * (x up^T), the up rows `features` behind the gate rows
@@ -159,6 +158,7 @@ mx4_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
   constexpr bool GATED = MODE == MXF_GATED, OUT_PARTS = MODE == MXF_GATED || MODE == MXF_ACT;
   constexpr int A_TOKEN = PARTS ? MX4_PARTS : 1;             // columns of a row of X
   using Shape = FewShape<GATED>;
+  static_assert(STAGES * Shape::PLACE_COLUMNS <= 256 - MXF_SUMS, "a place for scales a stage");
   extern __shared__ unsigned char smem_unaligned[];
   unsigned char* smem = reinterpret_cast<unsigned char*>(((uintptr_t)smem_unaligned + 1023) & ~(uintptr_t)1023);
   __shared__ __align__(8) unsigned long long full_bar[STAGES], empty_bar[STAGES], acc_full[2], acc_empty[2];
@@ -268,7 +268,8 @@ mx4_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
         ok = mbar_wait_warp(smem_u32(&full_bar[s]), (round / STAGES) & 1u, &abort_flag);
         if (!ok) break;
         tc_fence_after();
-        const unsigned at = stages + s * stage_bytes, place = tmem + MXF_SUMS + (round % MXF_PLACES) * Shape::PLACE_COLUMNS;
+        // (a place for scales a stage: who took them last is done when the stage is free)
+        const unsigned at = stages + s * stage_bytes, place = tmem + MXF_SUMS + s * Shape::PLACE_COLUMNS;
         const unsigned long long w_desc = smem_descriptor(at), x_desc = smem_descriptor(at + Shape::SIDES * MXF_W_BYTES);
         const unsigned products = 2 * (step0 + i) + 1 < a.k_tiles ? 4u : 2u;
         if (elect_one()) {
