@@ -66,11 +66,11 @@ def _library(name: str):
     return library
 
 
-def _stream():
-    """The handle of torch's current stream (of the scope's, inside one), without the object that torch makes around it: that costs
-    as much as a launch."""
+def _stream(device: int):
+    """The handle of torch's current stream there (of the scope's, inside one), without the object that torch makes around it: that
+    costs as much as a launch."""
     scoped = _ops._scoped_stream
-    return scoped if scoped is not None else torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
+    return scoped if scoped is not None else torch._C._cuda_getCurrentRawStream(device)
 
 
 def _few_rows(rows: int, features: int, four: bool) -> bool:
@@ -132,12 +132,13 @@ class Mx4:
         return self.codes.device
 
 
-def _here(what: str, *tensors: Optional[torch.Tensor]) -> None:
-    """The kernels run on the current device's stream: what they read and write has to be there."""
+def _here(what: str, *tensors: Optional[torch.Tensor]) -> int:
+    """The current device.  The kernels run on its stream: what they read and write has to be there."""
     here = torch.cuda.current_device()
     for tensor in tensors:
         if tensor is not None and tensor.get_device() != here:
             raise KernelError(f"{what}: a tensor lies on {tensor.device}, the current device is cuda:{here}")
+    return here
 
 
 def _need_mx4(q: Mx4, name: str, stacked: Optional[bool]) -> None:
@@ -183,24 +184,26 @@ def quantize_mx4(x: torch.Tensor) -> Mx4:
     Per block of 32 entries the scale is 2^(floor(log2(largest magnitude)) - 2), at least 2^-127; entries go to the nearest
     value of the format, ties to the even mantissa, magnitudes above 6 scales to 6 (the specification's conversion).  A block
     with an infinity or something that is not a number becomes a block of such."""
-    if x.dim() == 3:
+    stacked = x.dim() == 3
+    if stacked:
         _need(x, "x")
     else:
         _need_rows(x, "x")
     code = dtype_code(x.dtype)
-    _here("quantize_mx4", x)
-    *lead, rows, width = x.shape
+    here = _here("quantize_mx4", x)
+    matrices, (rows, width) = x.shape[0] if stacked else 1, x.shape[1:] if stacked else x.shape
     if width == 0:
         raise KernelError("quantize_mx4: rows without entries")
-    if max(x.shape) > MX4_MOST:
+    if rows > MX4_MOST or width > MX4_MOST or matrices > MX4_MOST:
         raise KernelError(f"quantize_mx4: sizes {tuple(x.shape)} are too large")
-    q = Mx4._made(x.new_empty((*lead, rows, 64 * _tiles(width)), dtype=torch.uint8),
-                  x.new_empty((*lead, _tiles(rows), _tiles(width), 512), dtype=torch.uint8), width)
-    if x.numel():
+    k_tiles, lead = -(-width // 128), (matrices,) if stacked else ()
+    codes = x.new_empty((*lead, rows, 64 * k_tiles), dtype=torch.uint8)
+    scales = x.new_empty((*lead, -(-rows // 128), k_tiles, 512), dtype=torch.uint8)
+    if matrices and rows:
         lib = _library("mx4")
-        _check(lib, lib.srb_mx4_quantize(x.data_ptr(), x.stride(-2), x.stride(0) if lead else 0, lead[0] if lead else 1, rows, width,
-                                         q.codes.data_ptr(), q.scales.data_ptr(), code, _stream()))
-    return q
+        _check(lib, lib.srb_mx4_quantize(x.data_ptr(), x.stride(-2), x.stride(0) if stacked else 0, matrices, rows, width, codes.data_ptr(),
+                                         scales.data_ptr(), code, _stream(here)))
+    return Mx4._made(codes, scales, width)
 
 
 @traced("quantize")
@@ -208,13 +211,16 @@ def dequantize_mx4(q: Mx4, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """The values that ``q`` stands for, in bfloat16 (exact: a code times a power of two) or float32."""
     _need_mx4(q, "q", None)
     code = dtype_code(dtype)
-    _here("dequantize_mx4", q.codes, q.scales)
-    if max(q.shape) > MX4_MOST:
+    codes, width = q.codes, q.width
+    here = _here("dequantize_mx4", codes, q.scales)
+    lead = codes.shape[:-1]
+    rows, matrices = lead[-1], lead[0] if len(lead) == 2 else 1
+    if rows > MX4_MOST or width > MX4_MOST or matrices > MX4_MOST:
         raise KernelError(f"dequantize_mx4: sizes {q.shape} are too large")
-    out = q.codes.new_empty(q.shape, dtype=dtype)
-    if out.numel():
+    out = codes.new_empty((*lead, width), dtype=dtype)
+    if rows and matrices:
         lib = _library("mx4")
-        _check(lib, lib.srb_mx4_dequantize(q.codes.data_ptr(), q.scales.data_ptr(), q.matrices or 1, q.rows, q.width, out.data_ptr(), code, _stream()))
+        _check(lib, lib.srb_mx4_dequantize(codes.data_ptr(), q.scales.data_ptr(), matrices, rows, width, out.data_ptr(), code, _stream(here)))
     return out
 
 
@@ -233,39 +239,40 @@ def linear_mx4(x, weight: Mx4, error_word: torch.Tensor, *, bias: Optional[torch
     four = isinstance(x, Mx4)
     if four:
         _need_mx4(x, "x", False)
-        rows, width = x.shape
+        held, rows, width = x.codes, x.codes.shape[0], x.width
     else:
         if x.dtype == torch.float32:
             raise KernelError("linear_mx4: float32 rows are not taken; multiply dequantize_mx4(weight, torch.float32) by linear")
         _need_rows(x, "x", torch.bfloat16)
-        rows, width = x.shape
+        held, (rows, width) = x, x.shape
     _need_mx4(weight, "weight", False)
+    codes = weight.codes
+    features = codes.shape[0]
     _need(error_word, "error_word", torch.int32)
     out_dtype = torch.bfloat16 if out_dtype is None else out_dtype
     dtype_code(out_dtype)
-    if rows > MX4_MOST or weight.rows > MX4_MOST or width > MX4_MOST:
+    if rows > MX4_MOST or features > MX4_MOST or width > MX4_MOST:
         raise KernelError(f"linear_mx4: {rows} rows of {width} and a weight {weight.shape} are too large")
     if weight.width != width:
         raise KernelError(f"linear_mx4: rows of {width} and a weight {weight.shape} do not fit")
     if bias is not None:
         _need(bias, "bias", torch.float32)
-        if bias.shape != (weight.rows,):
+        if bias.shape != (features,):
             raise KernelError("linear_mx4: one bias per feature is needed")
-    _here("linear_mx4", x.codes if four else x, weight.codes, weight.scales, bias, error_word)
-    many = not _few_rows(rows, weight.rows, four)
+    here = _here("linear_mx4", held, codes, weight.scales, bias, error_word)
+    many = not _few_rows(rows, features, four)
     # the kernel for many rows stores rows that start on 16-byte borders
-    pitch = -(-weight.rows // 8) * 8 if many else weight.rows
-    out = weight.codes.new_empty((rows, pitch), dtype=out_dtype)
-    if out.numel():
+    pitch = -(-features // 8) * 8 if many else features
+    out = codes.new_empty((rows, pitch), dtype=out_dtype)
+    if rows and features:
         lib = _library("gemm_mx4_pair" if many else "gemm_mx4")
         product, needed = (lib.srb_mx4_linear_pair, lib.srb_mx4_linear_pair_scratch) if many else (lib.srb_mx4_linear, lib.srb_mx4_linear_scratch)
-        held = x.codes if four else x
         needed = 0 if four else needed(rows, width)
-        scratch = weight.codes.new_empty(needed) if needed else None
-        _check(lib, product(held.data_ptr(), held.stride(0), x.scales.data_ptr() if four else None, weight.codes.data_ptr(), weight.scales.data_ptr(),
-                            None if bias is None else bias.data_ptr(), out.data_ptr(), pitch, rows, weight.rows, width,
-                            out_dtype == torch.float32, scratch.data_ptr() if needed else None, error_word.data_ptr(), _stream()), 2 if needed else 1)
-    return out if pitch == weight.rows else out[:, :weight.rows]
+        scratch = codes.new_empty(needed) if needed else None
+        _check(lib, product(held.data_ptr(), held.stride(0), x.scales.data_ptr() if four else None, codes.data_ptr(), weight.scales.data_ptr(),
+                            None if bias is None else bias.data_ptr(), out.data_ptr(), pitch, rows, features, width,
+                            out_dtype == torch.float32, scratch.data_ptr() if needed else None, error_word.data_ptr(), _stream(here)), 2 if needed else 1)
+    return out if pitch == features else out[:, :features]
 
 
 @traced("routed_experts")
@@ -290,12 +297,12 @@ def choose_experts(logits: torch.Tensor, top: int, renormalize: bool = False, *,
             raise KernelError("choose_experts: one choice bias per expert is needed")
     if top < 0 or top > 2**31 - 1 or rows * max(top, 1) >= 2**31:
         raise KernelError(f"choose_experts: {rows} rows of {top} choices")
-    _here("choose_experts", logits, choice_bias)
+    here = _here("choose_experts", logits, choice_bias)
     chosen, weights = logits.new_empty((rows, top), dtype=torch.int32), logits.new_empty((rows, top))
     lib = _library("route_groups")
     _check(lib, lib.srb_route_groups(logits.data_ptr(), logits.stride(0), rows, experts, None if choice_bias is None else choice_bias.data_ptr(), top,
                                      groups, top_groups, group_best, ROUTER_SCORING[scoring], renormalize, weight_scale, norm_eps, chosen.data_ptr(),
-                                     weights.data_ptr(), _stream()))
+                                     weights.data_ptr(), _stream(here)))
     return chosen, weights
 
 
@@ -321,11 +328,11 @@ def chosen_experts_mx4(h: torch.Tensor, chosen: torch.Tensor, weights: torch.Ten
                           "(at most 1024 experts)")
     if rows * max(top, 1) >= 2**31 or max(width, 2 * inner) > MX4_MOST:
         raise KernelError(f"chosen_experts_mx4: {rows} rows of {top} choices, width {width}, inner {inner} are too large")
-    _here("chosen_experts_mx4", h, chosen, weights, w_gate_up.codes, w_gate_up.scales, w_down.codes, w_down.scales, error_word)
+    here = _here("chosen_experts_mx4", h, chosen, weights, w_gate_up.codes, w_gate_up.scales, w_down.codes, w_down.scales, error_word)
     if rows == 0 or top == 0:
         return torch.zeros((rows, width), dtype=torch.bfloat16, device=h.device)
     out = torch.empty_like(h)
-    entries, stream, error = rows * top, _stream(), error_word.data_ptr()
+    entries, stream, error = rows * top, _stream(here), error_word.data_ptr()
     # (the pairs' result rows start on 16-byte borders)
     many = entries * (w_gate_up.codes.numel() + w_down.codes.numel()) > MX4_FEW_BYTES * experts * experts and width % 4 == 0
     divided = many and experts >= MX4_DIVIDE_EXPERTS
