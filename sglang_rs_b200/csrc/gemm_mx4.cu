@@ -507,7 +507,7 @@ extern "C" int srb_mx4_experts(const void* h, const int* plan, const int* slot_r
                                const void* down_scales, float* y, int max_tiles, int slots, int experts, int width, int inner, int gated,
                                int activation, float act_param, void* scratch_memory, int* error_word, void* stream) {
   if (max_tiles <= 0) return SRB_OK;
-  const Mx4ExpertsCall c = {h, plan, slot_row, up, up_scales, down, down_scales, y, max_tiles, slots, experts, width, inner, gated, activation, act_param,
+  const Mx4ExpertsCall c = {h, plan, up, up_scales, down, down_scales, y, max_tiles, slots, experts, width, inner, gated, activation, act_param,
                             error_word, (cudaStream_t)stream};
   if (const int status = mx4_check_experts(c)) return status;
   const FewExpertsScratch scratch(scratch_memory, max_tiles, experts, width, inner, gated);
@@ -522,7 +522,9 @@ extern "C" int srb_mx4_experts(const void* h, const int* plan, const int* slot_r
   first.ws_tiles = mx4_tiles(first.w_rows); first.up_tile = inner / 128;
   if (scratch.up_scales) {
     const int group = 128 * mx4_tiles(inner);
-    if (const int status = mx4_launch_gated_scales(up_scales, experts, inner, width, group, 2 * group, 1, plan, scratch.up_scales, c.stream)) return status;
+    Mx4GatedScales regroup;
+    if (const int status = mx4_make_gated_scales(&regroup, up_scales, experts, inner, width, group, 2 * group, 1, 0, scratch.up_scales)) return status;
+    if (const int status = mx4_launch_gated_scales(regroup, experts, plan, c.stream)) return status;
     up_scales = scratch.up_scales;
     first.ws_tiles = 2 * mx4_tiles(inner); first.up_tile = mx4_tiles(inner);
   }

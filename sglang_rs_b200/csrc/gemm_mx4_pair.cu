@@ -12,13 +12,14 @@
 //
 // Over experts (GROUPED) a tile is up to 256 slots of one expert (the plan of csrc/moe.cu); X and the parts that the gated mode leaves have room
 // for 256 rows a tile, so that a tile's scales are whole tiles.  Gated: the even CTA brings gate rows, the odd one the up rows of the same 96 features,
-// whose scales come regrouped (mx4_gated_scales_kernel: 96 and 96 rows are no whole tiles; a word a row by cp.async instead kept the tensor cores
+// whose scales come regrouped (mx4_gated_scales: 96 and 96 rows are no whole tiles; a word a row by cp.async instead kept the tensor cores
 // waiting, 296 us instead of some 215 for the gate/up of 12,288 slots, 64 experts of 2,048 x 1,408).
 //
 // Bound by the tensor cores under the chip's power limit: 2,048 rows of bfloat16 through 4,096 x 24,576 in 262 us for some milliseconds (1,570 TFLOP/s of
-// the product, twice that of the parts' products: 0.96 of the library's bfloat16 rate), 300 again and again; both operands in four bits 94 and 109 us
-// (4,400 TFLOP/s), 8 us of it the rows' quantising.  Tiles of 384 rows of W in one buffer, which bring X half as often, took the same (260, 93) and,
-// with nothing stored meanwhile, 432 instead of 372 us for the experts above: L2 is not what bounds.
+// the product, twice that of the parts' products: 0.96 of the library's bfloat16 rate), 300 again and again.  Both operands in four bits by what L2 brings,
+// 10.7 TB/s: 91 to 94 us and 109 again and again (4,400 TFLOP/s), 8 us of it the rows' quantising; with 5 stages instead of 6 101, without the
+// copies of scales no less.  Tiles of 384 rows of W in one buffer, which bring X half as often, took the same (260, 93): nothing is multiplied while
+// they are stored.
 //
 // Warps: 0 TMA, 1 products (even CTA) and tensor memory, 2-13 epilogue: a quarter of the lanes and a third of the columns each.  Waits are
 // bounded; one that runs out flags SRB_FLAG_WAIT_TIMEOUT.
@@ -509,21 +510,24 @@ extern "C" long long srb_mx4_experts_pair_scratch(int max_tiles, int experts, in
 }
 extern "C" int srb_mx4_experts_pair_tile() { return MXP_TILE; }
 
-// As srb_mx4_experts; width is a multiple of 4.
-extern "C" int srb_mx4_experts_pair(const void* h, const int* plan, const int* slot_row, const void* up, const void* up_scales, const void* down,
-                                    const void* down_scales, float* y, int max_tiles, int slots, int experts, int width, int inner, int gated,
+// As srb_mx4_experts, from the slots of the `rows` rows' choices, `top` each, instead of the slots' rows; experts of up to `few_slots` slots
+// have no tile in the plan; width is a multiple of 4.
+extern "C" int srb_mx4_experts_pair(const void* h, const int* plan, const int* entry_slot, const void* up, const void* up_scales, const void* down,
+                                    const void* down_scales, float* y, int max_tiles, int rows, int top, int few_slots, int experts, int width, int inner, int gated,
                                     int activation, float act_param, void* scratch_memory, int* error_word, void* stream) {
   if (max_tiles <= 0) return SRB_OK;
-  const Mx4ExpertsCall c = {h, plan, slot_row, up, up_scales, down, down_scales, y, max_tiles, slots, experts, width, inner, gated, activation, act_param,
+  const Mx4ExpertsCall c = {h, plan, up, up_scales, down, down_scales, y, max_tiles, rows * top, experts, width, inner, gated, activation, act_param,
                             error_word, (cudaStream_t)stream};
   if (const int status = mx4_check_experts(c)) return status;
   if (width % 4) SRB_FAIL("mx4_experts_pair: width %d is no multiple of 4", width);
   const PairExpertsScratch scratch(scratch_memory, max_tiles, experts, width, inner, gated);
+  Mx4GatedScales regroup = {};
   if (gated) {
-    if (const int status = mx4_launch_gated_scales(up_scales, experts, inner, width, MXP_HALF, 256, scratch.groups, plan, scratch.up_scales, c.stream)) return status;
+    if (const int status = mx4_make_gated_scales(&regroup, up_scales, experts, inner, width, MXP_HALF, 256, scratch.groups, few_slots, scratch.up_scales)) return status;
     up_scales = scratch.up_scales;
   }
-  if (const int status = mx4_launch_split_slots(h, width, plan, slot_row, experts, max_tiles, scratch.x, scratch.x_scales, c.stream)) return status;
+  if (const int status = mx4_launch_split_slots(h, rows, width, plan, entry_slot, top, experts, max_tiles, scratch.x, scratch.x_scales, regroup, gated ? experts : 0,
+                                                c.stream)) return status;
   if (const int status = pair_experts_product(gated ? MXP_GATED : MXP_ACT, c, scratch.x, scratch.x_scales, up, up_scales, scratch.act, scratch.act_scales,
                                               inner, width)) return status;
   return pair_experts_product(MXP_F32, c, scratch.act, scratch.act_scales, down, down_scales, y, nullptr, width, inner);

@@ -20,12 +20,12 @@ __device__ __forceinline__ void mx4_load_eight(const __nv_bfloat16* __restrict__
   }
 }
 
-// Eight entries of 128 of a row (lane of 16) as the two eight-bit parts of mx4.cuh, to `dst` and `dst + part`, and the row's scale words.
-template <bool WIDE>
-__device__ __forceinline__ void mx4_split_eight(const __nv_bfloat16* __restrict__ src, int left, bool live, int lane, uint8_t* dst, size_t part,
-                                                uint8_t* word, size_t scale_part) {
-  float v[8];
-  mx4_load_eight<WIDE>(src, left, live, v);
+// Eight entries of 128 of a row (lane of 16) as the two eight-bit parts of mx4.cuh, and the row's scale words.
+struct Mx4SplitEight {
+  uint2 high, low;
+  unsigned high_word, low_word;
+};
+__device__ __forceinline__ Mx4SplitEight mx4_split_eight(const float (&v)[8], int lane) {
   unsigned most = 0u;
 #pragma unroll
   for (int i = 0; i < 8; ++i) most = max(most, __float_as_uint(v[i]) & 0x7fffffffu);
@@ -35,18 +35,23 @@ __device__ __forceinline__ void mx4_split_eight(const __nv_bfloat16* __restrict_
   unsigned h[4], l[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) mx8_split(v[2 * i], v[2 * i + 1], high, low, h[i], l[i]);
-  unsigned high_word = (lane & 3) == 0 ? high << (8 * (lane >> 2)) : 0u, low_word = (lane & 3) == 0 ? low << (8 * (lane >> 2)) : 0u;
+  // (the lanes of a block have the same)
+  Mx4SplitEight e = {make_uint2(h[0] | h[1] << 16, h[2] | h[3] << 16), make_uint2(l[0] | l[1] << 16, l[2] | l[3] << 16), high << (8 * (lane >> 2)),
+                     low << (8 * (lane >> 2))};
 #pragma unroll
   for (int offset = 4; offset <= 8; offset <<= 1) {
-    high_word |= __shfl_xor_sync(0xffffffffu, high_word, offset);
-    low_word |= __shfl_xor_sync(0xffffffffu, low_word, offset);
+    e.high_word |= __shfl_xor_sync(0xffffffffu, e.high_word, offset);
+    e.low_word |= __shfl_xor_sync(0xffffffffu, e.low_word, offset);
   }
-  if (!live) return;
-  *reinterpret_cast<uint2*>(dst) = make_uint2(h[0] | h[1] << 16, h[2] | h[3] << 16);
-  *reinterpret_cast<uint2*>(dst + part) = make_uint2(l[0] | l[1] << 16, l[2] | l[3] << 16);
+  return e;
+}
+// to `dst` and `dst + part`, `word` and `word + scale_part`
+__device__ __forceinline__ void mx4_store_split(const Mx4SplitEight& e, int lane, uint8_t* dst, size_t part, uint8_t* word, size_t scale_part) {
+  *reinterpret_cast<uint2*>(dst) = e.high;
+  *reinterpret_cast<uint2*>(dst + part) = e.low;
   if (lane == 0) {
-    *reinterpret_cast<unsigned*>(word) = high_word;
-    *reinterpret_cast<unsigned*>(word + scale_part) = low_word;
+    *reinterpret_cast<unsigned*>(word) = e.high_word;
+    *reinterpret_cast<unsigned*>(word + scale_part) = e.low_word;
   }
 }
 
@@ -60,33 +65,108 @@ mx4_split_kernel(const __nv_bfloat16* __restrict__ x, size_t pitch, int rows, in
   const int k_tiles = mx4_tiles(width), lane = threadIdx.x & 15;
   const long long item = (long long)blockIdx.x * (MX4_ROWS_THREADS / 16) + (threadIdx.x >> 4);
   const int row = (int)(item / k_tiles), kt = (int)(item % k_tiles), k = kt * 128 + lane * 8;
-  mx4_split_eight<WIDE>(x + (size_t)row * pitch + k, width - k, row < rows, lane, parts + ((size_t)row * k_tiles * 128 + k),
-                        (size_t)rows * k_tiles * 128, scales + mx4_scale_word(row, kt, k_tiles),
-                        (size_t)mx4_tiles(rows) * k_tiles * MX4_TILE_BYTES);
+  float v[8];
+  mx4_load_eight<WIDE>(x + (size_t)row * pitch + k, width - k, row < rows, v);
+  const Mx4SplitEight e = mx4_split_eight(v, lane);
+  if (row < rows)
+    mx4_store_split(e, lane, parts + ((size_t)row * k_tiles * 128 + k), (size_t)rows * k_tiles * 128, scales + mx4_scale_word(row, kt, k_tiles),
+                    (size_t)mx4_tiles(rows) * k_tiles * MX4_TILE_BYTES);
 }
 
-// The same in the order of a plan's tiles (csrc/moe.cu) of 256 slots, with room for 256 rows a tile: parts [2, 256 tiles, ...].  16 lanes a
-// slot, 16 slots a block.
-template <bool WIDE>
-__global__ void __launch_bounds__(MX4_ROWS_THREADS)
-mx4_split_slots_kernel(const __nv_bfloat16* __restrict__ x, int width, const int* __restrict__ plan, const int* __restrict__ slot_row, int experts,
-                       int max_tiles, uint8_t* __restrict__ parts, uint8_t* __restrict__ scales) {
+// Scales of stacked gate and up rows (2 * inner rows a matrix) in groups: `group` gate rows, the `group` up rows of the same features, room for
+// `room` rows (a multiple of 128) a group.  A product tile's scales are whole tiles then, wherever the up rows begin.  Matrices whose
+// slots the product does not take are left out.  A thread has the 16 bytes of four rows, 32 apart.
+struct Mx4GatedScales {
+  const unsigned* scales;
+  int inner, group, room, groups, k_tiles, blocks;           // blocks of MX4_ROWS_THREADS a matrix
+  int left_out;                  // matrices with so many slots or fewer are left out
+  uint4* out;
+};
+__device__ __forceinline__ void mx4_gated_scales(const Mx4GatedScales& g, const int* __restrict__ plan, int matrix, int block) {
+  if (plan[1 + matrix + 1] - plan[1 + matrix] <= g.left_out) return;
+  const int tiles = g.groups * (g.room / 128), item = block * MX4_ROWS_THREADS + threadIdx.x;
+  if (item >= tiles * g.k_tiles * 32) return;
+  const int kt = item / 32 % g.k_tiles, tile = item / 32 / g.k_tiles;
+  const size_t from = (size_t)matrix * mx4_tiles(2 * g.inner) * g.k_tiles * MX4_TILE_BYTES;
+  unsigned w[4];
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const int row = tile * 128 + q * 32 + (item & 31), n = row % g.room, feature = row / g.room * g.group + (n < g.group ? n : n - g.group);
+    w[q] = n < 2 * g.group && feature < g.inner
+               ? g.scales[(from + mx4_scale_word(n < g.group ? feature : g.inner + feature, kt, g.k_tiles)) / 4] : 0x7f7f7f7fu;
+  }
+  g.out[((size_t)(matrix * tiles + tile) * g.k_tiles + kt) * (MX4_TILE_BYTES / 16) + (item & 31)] = make_uint4(w[0], w[1], w[2], w[3]);
+}
+__global__ void __launch_bounds__(MX4_ROWS_THREADS) mx4_gated_scales_kernel(const Mx4GatedScales g, const int* __restrict__ plan) {
   srb_launch_dependents();
   srb_grid_dependency_wait();
-  const int tile = blockIdx.x / 16, in_tile = blockIdx.x % 16 * (MX4_ROWS_THREADS / 16) + (threadIdx.x >> 4), lane = threadIdx.x & 15;
-  if (tile >= plan[0]) return;
-  const int expert = plan[1 + experts + 1 + 2 * tile], slot = plan[1 + experts + 1 + 2 * tile + 1] + in_tile;
-  const int end = plan[1 + expert + 1];                      // (a tile's place is below 256)
-  if (slot - (in_tile & 1) >= end) return;                   // neither half of the warp has a slot
-  const bool live = slot < end;
-  const int k_tiles = mx4_tiles(width), row = tile * 256 + in_tile;
+  mx4_gated_scales(g, plan, blockIdx.x / g.blocks, blockIdx.x % g.blocks);
+}
+
+// The split into the order of a plan's tiles (csrc/moe.cu) of 256 slots, with room for 256 rows a tile: parts [2, 256 tiles, ...].  16 lanes have
+// four column tiles of a row, their loads in flight together, split them once and store them for every choice of the row whose slot is in a tile (2,048
+// rows of 2,048 with 6 choices: 16 us; slot by slot, each splitting again, 28).  The blocks behind those regroup scales (`g`; both are
+// ahead of the same product, and one launch takes less than two).
+#define MX4_SPLIT_AT_ONCE 4
+template <bool WIDE>
+__global__ void __launch_bounds__(MX4_ROWS_THREADS)
+mx4_split_slots_kernel(const __nv_bfloat16* __restrict__ x, int rows, int width, const int* __restrict__ plan, const int* __restrict__ entry_slot, int top,
+                       int experts, int max_tiles, int split_blocks, uint8_t* __restrict__ parts, uint8_t* __restrict__ scales, const Mx4GatedScales g) {
+  srb_launch_dependents();
+  srb_grid_dependency_wait();
+  if ((int)blockIdx.x >= split_blocks) {
+    const int item = blockIdx.x - split_blocks;
+    mx4_gated_scales(g, plan, item / g.blocks, item % g.blocks);
+    return;
+  }
+  const int k_tiles = mx4_tiles(width), k_pieces = (k_tiles + MX4_SPLIT_AT_ONCE - 1) / MX4_SPLIT_AT_ONCE, lane = threadIdx.x & 15;
+  const long long item = (long long)blockIdx.x * (MX4_ROWS_THREADS / 16) + (threadIdx.x >> 4);
+  const int kt0 = (int)(item % k_pieces) * MX4_SPLIT_AT_ONCE;
+  const bool live = item / k_pieces < rows;
+  const int row = live ? (int)(item / k_pieces) : rows - 1;
+  const __nv_bfloat16* src = x + (size_t)row * width + kt0 * 128 + lane * 8;
+  float v[MX4_SPLIT_AT_ONCE][8];
+  if (WIDE && (kt0 + MX4_SPLIT_AT_ONCE) * 128 <= width) {
+    uint4 raw[MX4_SPLIT_AT_ONCE];
+#pragma unroll
+    for (int j = 0; j < MX4_SPLIT_AT_ONCE; ++j) raw[j] = *reinterpret_cast<const uint4*>(src + j * 128);
+#pragma unroll
+    for (int j = 0; j < MX4_SPLIT_AT_ONCE; ++j) mx4_unpack_bf16(raw[j], v[j]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < MX4_SPLIT_AT_ONCE; ++j) mx4_load_eight<WIDE>(src + j * 128, width - (kt0 + j) * 128 - lane * 8, true, v[j]);
+  }
+  Mx4SplitEight e[MX4_SPLIT_AT_ONCE];
+#pragma unroll
+  for (int j = 0; j < MX4_SPLIT_AT_ONCE; ++j) e[j] = mx4_split_eight(v[j], lane);
+  const int* tiles = plan + 1 + experts + 1;                 // (expert, first slot) of each, in the slots' order
   const size_t part = (size_t)max_tiles * 256 * k_tiles * 128, scale_part = (size_t)max_tiles * 2 * k_tiles * MX4_TILE_BYTES;
-  const __nv_bfloat16* src = x + (size_t)(live ? slot_row[slot] : 0) * width + lane * 8;
-  uint8_t* dst = parts + ((size_t)row * k_tiles * 128 + lane * 8);
-#pragma unroll 4
-  for (int kt = 0; kt < k_tiles; ++kt)
-    mx4_split_eight<WIDE>(src + kt * 128, width - kt * 128 - lane * 8, live, lane, dst + kt * 128, part, scales + mx4_scale_word(row, kt, k_tiles),
-                          scale_part);
+  for (int first = 0; first < top; first += 16) {
+    // a choice a lane: the row of the tiles where it goes, if its slot is in one
+    int to = -1;
+    if (live && first + lane < top) {
+      const int slot = entry_slot[(size_t)row * top + first + lane];
+      int low = 0, high = slot < 0 ? 0 : plan[0];            // the first tile that begins behind the slot is among low .. high
+      while (low < high) {
+        const int middle = (low + high) / 2;
+        if (tiles[2 * middle + 1] <= slot) low = middle + 1;
+        else high = middle;
+      }
+      if (low > 0 && slot >= 0) {
+        const int tile = low - 1, in_tile = slot - tiles[2 * tile + 1];
+        if (in_tile < 256 && slot < plan[1 + tiles[2 * tile] + 1]) to = tile * 256 + in_tile;
+      }
+    }
+    const int count = min(16, top - first);
+    for (int i = 0; i < count; ++i) {
+      const int dst = __shfl_sync(0xffffffffu, to, i, 16);
+      if (dst < 0) continue;
+#pragma unroll
+      for (int j = 0; j < MX4_SPLIT_AT_ONCE; ++j)
+        if (kt0 + j < k_tiles)
+          mx4_store_split(e[j], lane, parts + ((size_t)dst * k_tiles + kt0 + j) * 128 + lane * 8, part, scales + mx4_scale_word(dst, kt0 + j, k_tiles), scale_part);
+    }
+  }
 }
 
 // Eight entries of 128 of a row (lane of 16) as the eight four-bit parts of mx4.cuh, rows of their own from `row` on.
@@ -146,31 +226,9 @@ mx4_parts_slots_kernel(const __nv_bfloat16* __restrict__ x, int width, const int
                            codes, scales);
 }
 
-// Scales of stacked gate and up rows (2 * inner rows a matrix) in groups: `group` gate rows, the `group` up rows of the same features, room for
-// `room` rows (a multiple of 128) a group.  A product tile's scales are whole tiles then, wherever the up rows begin.  Matrices without a slot in
-// the plan are left out.  A thread has the 16 bytes of four rows, 32 apart.
-__global__ void __launch_bounds__(MX4_ROWS_THREADS)
-mx4_gated_scales_kernel(const unsigned* __restrict__ scales, int inner, int group, int room, int groups, int k_tiles, const int* __restrict__ plan,
-                        uint4* __restrict__ out) {
-  srb_launch_dependents();
-  srb_grid_dependency_wait();
-  const int matrix = blockIdx.y;
-  if (plan[1 + matrix] == plan[1 + matrix + 1]) return;
-  const int tiles = groups * (room / 128), item = blockIdx.x * MX4_ROWS_THREADS + threadIdx.x;
-  if (item >= tiles * k_tiles * 32) return;
-  const int kt = item / 32 % k_tiles, tile = item / 32 / k_tiles;
-  const size_t from = (size_t)matrix * mx4_tiles(2 * inner) * k_tiles * MX4_TILE_BYTES;
-  unsigned w[4];
-#pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    const int row = tile * 128 + q * 32 + (item & 31), n = row % room, feature = row / room * group + (n < group ? n : n - group);
-    w[q] = n < 2 * group && feature < inner ? scales[(from + mx4_scale_word(n < group ? feature : inner + feature, kt, k_tiles)) / 4] : 0x7f7f7f7fu;
-  }
-  out[((size_t)(matrix * tiles + tile) * k_tiles + kt) * (MX4_TILE_BYTES / 16) + (item & 31)] = make_uint4(w[0], w[1], w[2], w[3]);
-}
-
 // out[row, :] = sum over the row's choices, in their order, of weight * y[slot, :], in 32 bits, rounded once.  Bound by the bytes of y: four
-// columns a thread, the loads of four choices in flight.
+// columns a thread, the loads of eight choices in flight.
+#define MX4_COMBINE_AT_ONCE 8
 template <bool WIDE>
 __global__ void __launch_bounds__(128)
 mx4_combine_kernel(const float* __restrict__ y, const int* __restrict__ entry_slot, const float* __restrict__ weights, int top, int width,
@@ -182,10 +240,10 @@ mx4_combine_kernel(const float* __restrict__ y, const int* __restrict__ entry_sl
   const int* slots = entry_slot + (size_t)row * top;
   const float* w = weights + (size_t)row * top;
   float sum[4] = {};
-  for (int first = 0; first < top; first += 4) {
-    float v[4][4], by[4];
+  for (int first = 0; first < top; first += MX4_COMBINE_AT_ONCE) {
+    float v[MX4_COMBINE_AT_ONCE][4], by[MX4_COMBINE_AT_ONCE];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
+    for (int k = 0; k < MX4_COMBINE_AT_ONCE; ++k) {
       const int slot = first + k < top ? slots[first + k] : -1;
       by[k] = slot >= 0 ? w[first + k] : 0.f;
       const float* src = y + (size_t)max(slot, 0) * width + i;
@@ -200,7 +258,7 @@ mx4_combine_kernel(const float* __restrict__ y, const int* __restrict__ entry_sl
       }
     }
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
+    for (int k = 0; k < MX4_COMBINE_AT_ONCE; ++k)
 #pragma unroll
       for (int j = 0; j < 4; ++j) sum[j] = fmaf(by[k], v[k][j], sum[j]);
   }
@@ -232,13 +290,6 @@ static inline int mx4_launch_split(const void* x, long long pitch, int rows, int
                            (const __nv_bfloat16*)x, (size_t)pitch, rows, width, parts, scales));
   return SRB_OK;
 }
-static inline int mx4_launch_split_slots(const void* x, int width, const int* plan, const int* slot_row, int experts, int max_tiles, uint8_t* parts,
-                                  uint8_t* scales, cudaStream_t s) {
-  if (max_tiles > 1 << 22) SRB_FAIL("four-bit experts: %d tiles are too many", max_tiles);
-  SRB_CUDA_CALL(srb_launch(mx4_wide(x, width) ? mx4_split_slots_kernel<true> : mx4_split_slots_kernel<false>, dim3(256 / 16 * max_tiles),
-                           dim3(MX4_ROWS_THREADS), 0, s, (const __nv_bfloat16*)x, width, plan, slot_row, experts, max_tiles, parts, scales));
-  return SRB_OK;
-}
 // Eight four-bit parts: codes [8 rows, 64 column tiles] and the tiles of scales of 8 rows rows.
 static inline int mx4_launch_parts(const void* x, long long pitch, int rows, int width, uint8_t* codes, uint8_t* scales, cudaStream_t s) {
   dim3 grid;
@@ -258,12 +309,26 @@ static inline int mx4_launch_parts_slots(const void* x, int width, const int* pl
 static inline size_t mx4_gated_scales_bytes(int matrices, int width, int room, int groups) {
   return (size_t)matrices * groups * (room / 128) * mx4_tiles(width) * MX4_TILE_BYTES;
 }
-static inline int mx4_launch_gated_scales(const void* scales, int matrices, int inner, int width, int group, int room, int groups, const int* plan,
-                                   uint8_t* out, cudaStream_t s) {
-  const long long items = (long long)groups * (room / 128) * mx4_tiles(width) * 32;
-  if (matrices > 65535 || items > 0x3fffffff) SRB_FAIL("four-bit experts: %d matrices of 2 x %d rows of %d are too many", matrices, inner, width);
-  SRB_CUDA_CALL(srb_launch(mx4_gated_scales_kernel, dim3((unsigned)((items + MX4_ROWS_THREADS - 1) / MX4_ROWS_THREADS), matrices),
-                           dim3(MX4_ROWS_THREADS), 0, s, (const unsigned*)scales, inner, group, room, groups, mx4_tiles(width), plan, (uint4*)out));
+static inline int mx4_make_gated_scales(Mx4GatedScales* g, const void* scales, int matrices, int inner, int width, int group, int room, int groups,
+                                        int left_out, uint8_t* out) {
+  const long long items = (long long)groups * (room / 128) * mx4_tiles(width) * 32, blocks = (items + MX4_ROWS_THREADS - 1) / MX4_ROWS_THREADS;
+  if (items > 0x3fffffff || blocks * matrices > 0x3fffffff) SRB_FAIL("four-bit experts: %d matrices of 2 x %d rows of %d are too many", matrices, inner, width);
+  *g = {(const unsigned*)scales, inner, group, room, groups, mx4_tiles(width), (int)blocks, left_out, (uint4*)out};
+  return SRB_OK;
+}
+static inline int mx4_launch_gated_scales(const Mx4GatedScales& g, int matrices, const int* plan, cudaStream_t s) {
+  SRB_CUDA_CALL(srb_launch(mx4_gated_scales_kernel, dim3(g.blocks * matrices), dim3(MX4_ROWS_THREADS), 0, s, g, plan));
+  return SRB_OK;
+}
+// `g`: scales to be regrouped beside it, of `matrices` matrices (none: 0).
+static inline int mx4_launch_split_slots(const void* x, int rows, int width, const int* plan, const int* entry_slot, int top, int experts, int max_tiles,
+                                         uint8_t* parts, uint8_t* scales, const Mx4GatedScales& g, int matrices, cudaStream_t s) {
+  const long long pieces = (mx4_tiles(width) + MX4_SPLIT_AT_ONCE - 1) / MX4_SPLIT_AT_ONCE;
+  const long long blocks = (rows * pieces + MX4_ROWS_THREADS / 16 - 1) / (MX4_ROWS_THREADS / 16);
+  if (max_tiles > 1 << 22 || blocks > 0x3fffffff) SRB_FAIL("four-bit experts: %d rows of %d, %d tiles are too many", rows, width, max_tiles);
+  SRB_CUDA_CALL(srb_launch(mx4_wide(x, width) ? mx4_split_slots_kernel<true> : mx4_split_slots_kernel<false>, dim3((unsigned)(blocks + g.blocks * matrices)),
+                           dim3(MX4_ROWS_THREADS), 0, s, (const __nv_bfloat16*)x, rows, width, plan, entry_slot, top, experts, max_tiles, (int)blocks, parts,
+                           scales, g));
   return SRB_OK;
 }
 static inline int mx4_launch_combine(const float* y, const int* entry_slot, const float* weights, int rows, int top, int width, void* out, cudaStream_t s) {
@@ -289,7 +354,7 @@ struct Mx4Scratch {
 // What a call on the experts has, for both libraries.
 struct Mx4ExpertsCall {
   const void* h;                 // bfloat16 rows of `width`
-  const int *plan, *slot_row;
+  const int* plan;
   const void *up, *up_scales;    // [experts, 2 * inner or inner, width]
   const void *down, *down_scales;// [experts, width, inner]
   float* y;                      // [slots, width]

@@ -28,25 +28,26 @@ MX4_FEW_ROWS = 64
 #: 20, 192 rows 20 and 21, 256 rows 22 and 21; 12,288 x 4,096: 192 rows 48 and 49; 2,048 x 2,048: 192 rows 9 and 13)
 MX4_FEW_ROWS_OF_SMALL = 192
 #: The experts' products run on the kernel for few rows while choices per expert * bytes of an expert's codes stay below this (that kernel reads an expert's
-#: matrices, from L2, for every 8 of its rows; us, it and pairs: 64 experts of 2,048 x 1,408 with 32 choices each 160 and 221, 48 227 and 231; 32 of
-#: 1,024 x 1,024 with 64 82 and 106, 96 109 and 111; 16 of 2,048 x 704 with 64 62 and 84, 96 85 and 91; 8 of 1,024 x 512 with 96 29 and 41, 192 43 and 46)
+#: matrices, from L2, for every 8 of its rows; us, it and the best of the others: 64 experts of 2,048 x 1,408 with 32 choices each 161 and 174, 40 189
+#: and 189, 48 226 and 215; 32 of 1,024 x 1,024 with 64 83 and 100, 96 109 and 100; 8 of 1,024 x 512 with 96 30 and 38, 192 43 and 38)
 MX4_FEW_BYTES = 160 << 20
 #: above it, from this many experts on, they are divided on the device, those with up to MX4_FEW_SLOTS rows going to the kernel for few rows all the same: a tile
-#: of 256 rows costs the pairs as much with one row (all on pairs and divided, choices spread unevenly: 64 experts of 2,048 x 1,408 with 48 each 231 and 199,
-#: 192 376 and 356, and 433 and 392 again and again, where the chip's power limit counts; 32 of 1,024 x 1,024 with 64 106 and 94; but 8 of 1,024 x 512
-#: with 48 44 and 57: three launches more)
-MX4_DIVIDE_EXPERTS = 32
+#: of 256 rows costs the pairs as much with one row (all on pairs and divided: 128 experts of 2,048 x 768 with 96 choices each 335 and 309 where some have
+#: many more than others, 317 and 350 spread evenly; 64 of 2,048 x 1,408 with 192, very uneven, 431 and 390 again and again, where the chip's power
+#: limit counts; 48 of 1,024 x 1,024 with 192 192 and 189, evenly 172 and 181; but 32 of 2,048 x 1,408 with 96 144 and 155: three launches more)
+MX4_DIVIDE_EXPERTS = 64
 MX4_FEW_SLOTS = 48
 
 _P, _I, _L, _F = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_float
 _LINEAR = (_P, _L, _P, _P, _P, _P, _P, _L, _I, _I, _I, _I, _P, _P, _P)
 _EXPERTS = (_P,) * 8 + (_I,) * 7 + (_F, _P, _P, _P)
+_EXPERTS_PAIR = (_P,) * 8 + (_I,) * 9 + (_F, _P, _P, _P)
 #: entry points by library and their arguments, declared once: a small call costs as long on the host as on the device
 _SIGNATURES = {
     "mx4": {"srb_mx4_quantize": (_P, _L, _L, _I, _I, _I, _P, _P, _I, _P), "srb_mx4_dequantize": (_P, _P, _I, _I, _I, _P, _I, _P)},
     "gemm_mx4": {"srb_mx4_linear": _LINEAR, "srb_mx4_experts": _EXPERTS, "srb_mx4_linear_scratch": (_I,) * 2,
                  "srb_mx4_experts_scratch": (_I,) * 5, "srb_mx4_experts_tile": (), "srb_mx4_combine": (_P, _P, _P, _I, _I, _I, _P, _P)},
-    "gemm_mx4_pair": {"srb_mx4_linear_pair": _LINEAR, "srb_mx4_experts_pair": _EXPERTS, "srb_mx4_linear_pair_scratch": (_I,) * 2,
+    "gemm_mx4_pair": {"srb_mx4_linear_pair": _LINEAR, "srb_mx4_experts_pair": _EXPERTS_PAIR, "srb_mx4_linear_pair_scratch": (_I,) * 2,
                       "srb_mx4_experts_pair_scratch": (_I,) * 5, "srb_mx4_experts_pair_tile": (),
                       "srb_mx4_divide_plan": (_P, _I, _I, _I, _I, _I, _P, _P, _P, _P)},
     "route_groups": {"srb_route_groups": (_P, _L, _I, _I, _P, _I, _I, _I, _I, _I, _I, _F, _F, _P, _P, _P)},
@@ -361,15 +362,16 @@ def chosen_experts_mx4(h: torch.Tensor, chosen: torch.Tensor, weights: torch.Ten
     _check(moe, moe.srb_moe_plan_of(_P(chosen.data_ptr()), rows, top, experts, tile, _P(plan), _P(slot_row), _P(entry_slot), None, None, _P(error),
                                     stream if isinstance(stream, _P) else _P(stream)))
     matrices = (w_gate_up.codes.data_ptr(), w_gate_up.scales.data_ptr(), w_down.codes.data_ptr(), w_down.scales.data_ptr(), y)
-    sizes = (entries, experts, width, inner, gated, act_code, activation_param)
+    sizes = (experts, width, inner, gated, act_code, activation_param)
     few_plan = pair_plan = plan
     if divided:
         few_plan, pair_plan = at + few_plan_at, at + pair_plan_at
         _check(pair, pair.srb_mx4_divide_plan(plan, experts, MX4_FEW_SLOTS, few_tile, few_tiles, tiles, few_plan, pair_plan, error, stream))
     if few_tiles:
-        _check(lib, lib.srb_mx4_experts(h.data_ptr(), few_plan, slot_row, *matrices, few_tiles, *sizes, at + few_at, error, stream),
+        _check(lib, lib.srb_mx4_experts(h.data_ptr(), few_plan, slot_row, *matrices, few_tiles, entries, *sizes, at + few_at, error, stream),
                3 + int(gated and inner % 128 != 0))
     if many:
-        _check(pair, pair.srb_mx4_experts_pair(h.data_ptr(), pair_plan, slot_row, *matrices, tiles, *sizes, at + pair_at, error, stream), 3 + int(gated))
+        _check(pair, pair.srb_mx4_experts_pair(h.data_ptr(), pair_plan, entry_slot, *matrices, tiles, rows, top, MX4_FEW_SLOTS if divided else 0, *sizes,
+                                               at + pair_at, error, stream), 3)
     _check(lib, lib.srb_mx4_combine(y, entry_slot, weights.data_ptr(), rows, top, width, out.data_ptr(), stream))
     return out

@@ -496,6 +496,18 @@ def test_experts_chosen_twice_by_nobody_and_outside(rows):
     assert (check_experts(h, everywhere, weights, up, down) == 0).all()
 
 
+@pytest.mark.parametrize("kernels", KERNELS)
+@pytest.mark.parametrize("rows,experts,width,inner,top", [(40, 24, 136, 72, 20), (90, 5, 192, 96, 17), (300, 3, 256, 128, 33)])
+def test_many_choices_on_each_kernel_some_outside_and_some_twice(rows, experts, width, inner, top, kernels, monkeypatch):
+    for name, value in KERNELS[kernels].items():
+        monkeypatch.setattr(mx4, name, value)
+    g = generator(71)
+    h, weights = torch.randn(rows, width, generator=g).bfloat16().cuda(), torch.rand(rows, top, generator=g).cuda()
+    chosen = torch.randint(-2, experts + 2, (rows, top), generator=g, dtype=torch.int32).cuda()
+    chosen[rows // 2] = -1
+    check_experts(h, chosen, weights, random_matrix(72, experts, 2 * inner, width, low=116, high=122), random_matrix(73, experts, width, inner, low=116, high=122))
+
+
 def test_more_tiles_of_experts_than_a_grid_is_high():
     rows, experts, width, inner = 270_000, 64, 128, 64
     h = torch.randn(rows, width, generator=generator(61)).bfloat16().cuda()
