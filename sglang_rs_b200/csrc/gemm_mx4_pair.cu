@@ -8,7 +8,8 @@
 //
 // CTA r of a pair has 128 rows of X (the M side) and 96 rows of W (half of the N side) in shared memory, and in tensor memory two
 // buffers of 192 columns of sums for its rows of X, a row a lane, beside 128 columns of scales (256 columns of sums twice would leave none).  Scales
-// go from shared to tensor memory ahead of a step's products, in the same queue; steps use places in turn.
+// go from shared to tensor memory ahead of a step's products, in the same queue: products wait for the copies issued ahead of them, copies not for the
+// products, so each stage has a place for scales of its own, which is free when the stage is.
 //
 // Over experts (GROUPED) a tile is up to 256 slots of one expert (the plan of csrc/moe.cu); X and the parts that the gated mode leaves have room
 // for 256 rows a tile, so that a tile's scales are whole tiles.  Gated: the even CTA brings gate rows, the odd one the up rows of the same 96 features,
@@ -17,8 +18,9 @@
 //
 // Bound by the tensor cores under the chip's power limit: 2,048 rows of bfloat16 through 4,096 x 24,576 in 262 us for some milliseconds (1,570 TFLOP/s of
 // the product, twice that of the parts' products: 0.96 of the library's bfloat16 rate), 300 again and again.  Both operands in four bits by what L2 brings,
-// 10.7 TB/s: 91 to 94 us and 109 again and again (4,400 TFLOP/s), 8 us of it the rows' quantising; with 5 stages instead of 6 101, without the
-// copies of scales no less.  Tiles of 384 rows of W in one buffer, which bring X half as often, took the same (260, 93): nothing is multiplied while
+// some 10 TB/s: 95 us (4,300 TFLOP/s), 8 us of it the rows' quantising.  Without the copies of scales it takes no less; a sixth stage with five places for
+// scales, each awaited ahead of its next copies, 109 to 116: tensor memory has no columns for a sixth place.  Tiles of 384 rows of W in one buffer,
+// which bring X half as often, took the same (260, 93 with six stages): nothing is multiplied while
 // they are stored.
 //
 // Warps: 0 TMA, 1 products (even CTA) and tensor memory, 2-13 epilogue: a quarter of the lanes and a third of the columns each.  Waits are
@@ -48,7 +50,7 @@ SRB_DEFINE_PDL_SWITCH()
 #define MXP_ACT 5
 
 template <bool FOUR> struct PairShape {
-  static constexpr int STAGES = FOUR ? 6 : 4;
+  static constexpr int STAGES = FOUR ? 5 : 4;
   static constexpr int PARTS = FOUR ? 1 : 2;
   static constexpr int B_AT = PARTS * MXP_A_BYTES;
   static constexpr int XS_AT = B_AT + MXP_B_BYTES;           // scales of X: two column tiles, or a tile of each part
@@ -57,7 +59,6 @@ template <bool FOUR> struct PairShape {
   static constexpr int TMA_BYTES = FOUR ? STAGE_BYTES : 2 * MXP_A_BYTES + MXP_B_BYTES / 2 + 2048;    // what the barrier counts: codes without the gaps
   static constexpr int THREADS = 32 * (2 + MXP_EPILOGUE_WARPS);
   static constexpr int PLACE_COLUMNS = FOUR ? 24 : 16;       // of scales of a step
-  static constexpr int PLACES = FOUR ? 5 : 4;
 };
 
 struct PairMx4Args {
@@ -149,6 +150,7 @@ mx4_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
                 const __grid_constant__ CUtensorMap map_ws, const __grid_constant__ CUtensorMap map_out, const PairMx4Args a) {
   using Shape = PairShape<FOUR>;
   constexpr int STAGES = Shape::STAGES;
+  static_assert(STAGES * Shape::PLACE_COLUMNS <= 512 - MXP_SUMS, "a place for scales a stage");
   constexpr bool GATED = MODE == MXP_GATED, PARTS = MODE == MXP_GATED || MODE == MXP_ACT;
   extern __shared__ unsigned char smem_unaligned[];
   unsigned char* smem = reinterpret_cast<unsigned char*>(((uintptr_t)smem_unaligned + 1023) & ~(uintptr_t)1023);
@@ -244,7 +246,8 @@ mx4_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
           if (!ok) break;
           tc_fence_after();
           const unsigned stage = smem_u32(smem) + s * Shape::STAGE_BYTES;
-          const unsigned place = tmem + MXP_SUMS + (round % Shape::PLACES) * Shape::PLACE_COLUMNS;
+          // (a place for scales a stage: who took them last is done when the stage is free)
+          const unsigned place = tmem + MXP_SUMS + s * Shape::PLACE_COLUMNS;
           const unsigned long long a_desc = smem_descriptor(stage), b_desc = smem_descriptor(stage + Shape::B_AT);
           if (elect_one()) {
             const unsigned long long xs = scales_descriptor(stage + Shape::XS_AT), ws = scales_descriptor(stage + Shape::WS_AT);

@@ -584,3 +584,31 @@ def test_a_layer_of_experts_in_four_bits(rows):
         graph.replay()
         torch.cuda.synchronize()
         check(results)
+
+
+# ------------------------------------------------------------------------------------------- many steps on pairs
+@pytest.mark.parametrize("four", [False, True])
+@pytest.mark.parametrize("rows,width,features", [(300, 4225, 15400), (257, 8192, 7700)])
+def test_many_steps_and_more_tiles_than_pairs(rows, width, features, four):
+    """Every stage and every place for scales is taken again many times, within a tile and from one to the next: the values, and the same bits
+    beside other work."""
+    g = torch.Generator("cuda").manual_seed(rows)
+    x = (torch.randn(rows, width, generator=g, device="cuda") * torch.exp(torch.randn(width, generator=g, device="cuda"))).bfloat16()
+    # every block with a scale of its own: one that is taken for another is off by powers of two
+    size = torch.exp2(torch.randint(-8, 9, (features, -(-width // 32)), generator=g, device="cuda").float()).repeat_interleave(32, dim=1)[:, :width]
+    matrix = ops.quantize_mx4(torch.randn(features, width, generator=g, device="cuda") * size)
+    x = ops.quantize_mx4(x) if four else x
+    error = word()
+    got = ops.linear_mx4(x, matrix, error, out_dtype=torch.float32)
+    rows_in_64, w = (ops.dequantize_mx4(x, torch.float32) if four else x).double(), ops.dequantize_mx4(matrix, torch.float32).double()
+    want = rows_in_64 @ w.T
+    assert ((got.double() - want).abs() <= room_of(rows_in_64, w, want, torch.float32)).all()
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    torch.cuda.synchronize()
+    results = []
+    for stream in streams:
+        with torch.cuda.stream(stream):
+            results += [ops.linear_mx4(x, matrix, error, out_dtype=torch.float32) for _ in range(5)]
+    torch.cuda.synchronize()
+    ops.raise_on_error_word(error)
+    assert all(torch.equal(got, r) for r in results)
