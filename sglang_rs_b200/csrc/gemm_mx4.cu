@@ -343,7 +343,7 @@ mx4_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
         for (int j = 0; j < AT_ONCE; ++j) {
           if (OUT_PARTS) {
             if (token + j >= t.count) break;
-            float r = srb_gated<true>(a.activation, v[j], GATED ? up[j] : 1.0f, a.act_param);
+            float r = mx4_gated(a.activation, v[j], GATED ? up[j] : 1.0f, a.act_param);
             if (feature >= a.features) r = 0.f;              // what pads the rows of parts
             const unsigned first = mx4_first_scale(__reduce_max_sync(0xffffffffu, __float_as_uint(r) & 0x7fffffffu));
             // part p of eight lanes' features together: lane 8 g + p gets the four bytes of features 8 g .. + 7

@@ -306,10 +306,10 @@ mx4_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
               float up[32];
               tmem_load_32(sums + MXP_HALF + column, up);
 #pragma unroll
-              for (int j = 0; j < 32; ++j) v[j] = srb_gated<true>(a.activation, lane < live ? v[j] : 1.0f, up[j], a.act_param);
+              for (int j = 0; j < 32; ++j) v[j] = mx4_gated(a.activation, lane < live ? v[j] : 1.0f, up[j], a.act_param);
             } else {
 #pragma unroll
-              for (int j = 0; j < 32; ++j) v[j] = srb_gated<true>(a.activation, lane < live ? v[j] : 1.0f, 1.0f, a.act_param);
+              for (int j = 0; j < 32; ++j) v[j] = mx4_gated(a.activation, lane < live ? v[j] : 1.0f, 1.0f, a.act_param);
             }
             if (feature + 32 > a.features) {
 #pragma unroll

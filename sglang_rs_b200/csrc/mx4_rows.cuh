@@ -7,6 +7,13 @@
 
 #define MX4_ROWS_THREADS 256
 
+// act(g) * u in 32 bits.  Sums that are not numbers (a row or a block of weights that is not finite) stay so: the limits of some activations would turn
+// them into numbers (0, or the limit).
+__device__ __forceinline__ float mx4_gated(int activation, float g, float u, float param) {
+  const float r = srb_gated<true>(activation, g, u, param);
+  return isnan(g) || isnan(u) ? __uint_as_float(0x7fc00000u) : r;
+}
+
 template <bool WIDE>
 __device__ __forceinline__ void mx4_load_eight(const __nv_bfloat16* __restrict__ src, int left, bool live, float (&v)[8]) {
 #pragma unroll

@@ -316,7 +316,9 @@ def chosen_experts_mx4(h: torch.Tensor, chosen: torch.Tensor, weights: torch.Ten
     :func:`~sglang_rs_b200.ops.route`); a choice outside the experts adds nothing, one made twice counts twice.
     ``w_gate_up``: a stack [experts, 2 * inner, width], an expert's gate rows over its up rows (``gated`` False: the up matrices
     alone [experts, inner, width], an expert being W_down act(W_up h)); ``w_down`` a stack [experts, width, inner].  Sums are
-    taken in 32 bits; act(gate) * up is rounded once between the two products.  Nothing is decided on the host."""
+    taken in 32 bits; act(gate) * up is rounded once between the two products.  Nothing is decided on the host.  A row with an infinity or
+    something that is not a number, and one whose act(gate) * up is beyond 32 bits, gives a row that is not a number, whatever the
+    activation makes of it."""
     _need(h, "h", torch.bfloat16); _need(chosen, "chosen", torch.int32); _need(weights, "weights", torch.float32)
     _need_mx4(w_gate_up, "w_gate_up", True); _need_mx4(w_down, "w_down", True); _need(error_word, "error_word", torch.int32)
     act_code = activation_code(activation, parametric=True)

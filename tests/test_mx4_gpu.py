@@ -612,3 +612,40 @@ def test_many_steps_and_more_tiles_than_pairs(rows, width, features, four):
     torch.cuda.synchronize()
     ops.raise_on_error_word(error)
     assert all(torch.equal(got, r) for r in results)
+
+
+# ------------------------------------------------------------------------------------------- what is not finite, through every activation
+ACTIVATIONS = [("silu", True, 0.0), ("gelu_tanh", True, 0.0), ("swiglu_clamp", True, 1.5), ("relu2", True, 0.0), ("relu2", False, 0.0), ("silu", False, 0.0),
+               ("gelu_tanh", False, 0.0), ("swiglu_clamp", False, 1.5)]
+
+
+@pytest.mark.parametrize("kernels", KERNELS)
+@pytest.mark.parametrize("name,gated,param", ACTIVATIONS)
+def test_rows_that_are_not_finite_spoil_themselves_through_every_activation(name, gated, param, kernels, monkeypatch):
+    for setting, value in KERNELS[kernels].items():
+        monkeypatch.setattr(mx4, setting, value)
+    h, chosen, weights, up, down = expert_case(66, 70, 4, 160, 96, 2, gated)
+    call = lambda: ops.chosen_experts_mx4(h, chosen, weights, up[0], down[0], name, word(), gated=gated, activation_param=param)
+    clean = call()
+    spoilt = {3: math.nan, 11: math.inf, 40: -math.inf, 69: math.nan}
+    for row, value in spoilt.items():
+        h[row, 9 + row] = value
+    got = call()
+    rows = torch.zeros(70, dtype=torch.bool, device="cuda")
+    rows[list(spoilt)] = True
+    assert got[rows].isnan().all() and torch.equal(got[~rows], clean[~rows])
+
+
+@pytest.mark.parametrize("kernels", KERNELS)
+@pytest.mark.parametrize("name,gated,param", ACTIVATIONS)
+def test_weights_that_are_not_numbers_spoil_the_rows_of_their_expert(name, gated, param, kernels, monkeypatch):
+    for setting, value in KERNELS[kernels].items():
+        monkeypatch.setattr(mx4, setting, value)
+    h, chosen, weights, up, down = expert_case(67, 70, 4, 160, 96, 2, gated)
+    call = lambda matrix: ops.chosen_experts_mx4(h, chosen, weights, matrix, down[0], name, word(), gated=gated, activation_param=param)
+    clean = call(up[0])
+    for row in ((5, 96 + 70) if gated else (5,)):             # a gate row, an up row
+        scales = up[0].scales.clone()
+        scales[2, row // 128, 0, (row % 32) * 16 + row % 128 // 32 * 4 + 1] = 255
+        got, theirs = call(ops.Mx4(up[0].codes, scales, 160)), (chosen == 2).any(1)
+        assert got[theirs].isnan().all() and torch.equal(got[~theirs], clean[~theirs])
