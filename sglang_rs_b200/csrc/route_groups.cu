@@ -60,16 +60,17 @@ __device__ __forceinline__ unsigned long long route_most(unsigned long long key)
 // Whether 32-bit numbers do not tell which of two picks (or sums of two) is larger, `above` being the larger one of them.  `by_logit`: they are the logits
 // themselves, whose order is that of the scores but where 64-bit scores are alike: both 0; sigmoids near 1 (2^-53 apart is e^-36, and logits
 // below 36 that are 1 apart differ by more); logits so near 0 that the exponential does not see them apart (below 1e-5 two may be nearer
-// than 9e-13, and an argument of up to 700 is good to 2e-13).  Otherwise
-// they are off by at most 1.25 2^-22 of the scores that went in (the exponential by 2^-23 of itself, the sum under the division, the division and the sum
-// with the bias by 2^-24 each; 2^-24 more where two picks are added), or, in a softmax, 2^-20: its exponential's argument is off by 2^-24 of its size,
-// which is below 24 where the score is above 2^-34, the sum by 2^-22 and the quick division by 2^-22; smaller picks always count as near.
+// than 9e-13, and an argument of up to 700 is good to 2e-13).  Otherwise they are off by at most 1.75 2^-22 of the scores that went in (the
+// exponential by 1.5 2^-23 of itself, over all floats 1.28 2^-23 at most; the sum under the division, the division, the sum with the bias and that of two
+// picks by 2^-24 each), or, in a softmax, 2^-16: its exponential's argument is off by 2^-24 of its size, which is below 104 where anything is left of
+// the score (6.2e-6 of it), the sum by 2^-24 for each of up to 37 additions (2.2e-6) and as much as its terms (the largest ones have small
+// arguments: 1e-6), the quick division by 2^-22.  Beside that by 2^-126, where 32 bits end.
 __device__ __forceinline__ bool route_near(float above, float below, float bias_most, float most, bool by_logit, int scoring) {
   if (by_logit)
     return !(below - (scoring == ROUTE_SOFTMAX ? most : 0.f) > -700.f) || (fabsf(above) < 1e-5f && above - below < 9e-13f) ||
            (scoring == ROUTE_SIGMOID && above > 16.f && !(above - below >= 1.f && below <= 36.f));
-  const float room = (fabsf(above) + fabsf(below) + 2.f * bias_most) * (scoring == ROUTE_SOFTMAX ? 1.9073486e-6f : 3.6e-7f);
-  return !(above - below > room) || (bias_most == 0.f && below < 5.8207661e-11f);
+  const float room = fmaf(fabsf(above) + fabsf(below) + 2.f * bias_most, scoring == ROUTE_SOFTMAX ? 1.5258789e-5f : 4.3e-7f, 2.3509887e-38f);
+  return !(above - below > room);
 }
 
 // The score of a group whose largest two picks each lane has among its own.

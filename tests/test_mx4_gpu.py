@@ -649,3 +649,28 @@ def test_weights_that_are_not_numbers_spoil_the_rows_of_their_expert(name, gated
         scales[2, row // 128, 0, (row % 32) * 16 + row % 128 // 32 * 4 + 1] = 255
         got, theirs = call(ops.Mx4(up[0].codes, scales, 160)), (chosen == 2).any(1)
         assert got[theirs].isnan().all() and torch.equal(got[~theirs], clean[~theirs])
+
+
+# ------------------------------------------------------------------------------------------- scores where 32 bits say little
+def test_choices_between_small_scores_that_a_small_bias_puts_in_order():
+    """One logit 66 above two others: their scores, some 2e-29, are off by up to 7e-6 of themselves in 32 bits, and biases of 2e-6 of them decide."""
+    g = generator(51)
+    step = 2.0 ** -19
+    most = 46 + torch.randint(0, 256, (600,), generator=g) * 2.0 ** -18
+    second = -20 + torch.randint(0, 16, (600,), generator=g) * step
+    third = second - torch.randint(0, 3, (600,), generator=g) * step
+    logits = torch.stack([most, second, third, torch.full((600,), -40.0)], dim=1)
+    bias = torch.tensor([0.0, 0.0, 2.2e-6 * math.exp(-66.0), 0.0])
+    check_choice(logits.cuda(), dict(experts=4, top=3), bias.cuda())
+
+
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+def test_groups_whose_scores_32_bits_do_not_hold(scoring):
+    """A group's two best scores below the least 32-bit number add up to more than another's one above it."""
+    logits = torch.full((40, 16), -200.0)
+    logits[:, 4] = -88.71 + 0.001 * torch.arange(40)
+    logits[:, 9], logits[:, 10] = -88.8, -88.9
+    if scoring == "softmax":
+        logits[:, 0] = 0.0
+        logits[:, 4:12] -= 15.0
+    check_choice(logits.cuda(), dict(experts=16, top=3, groups=4, top_groups=1 if scoring == "sigmoid" else 2, group_best=2, scoring=scoring), None)
