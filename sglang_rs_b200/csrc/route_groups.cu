@@ -282,6 +282,19 @@ __device__ __noinline__ int route_reorder(const float* __restrict__ z, const flo
   return ordered;
 }
 
+// The weight of the lane's choice in 64 bits, `argument` being that of the exponential.
+__device__ __noinline__ float route_far_weight(double argument, float sum, const GroupRule& rule, int lane) {
+  double weight = 0.0;
+  if (lane < rule.top) weight = rule.scoring == ROUTE_SOFTMAX ? exp(argument) / (double)sum : 1.0 / (1.0 + exp(-argument));
+  if (rule.renormalize) {
+    double all = weight;
+#pragma unroll 1
+    for (int offset = 16; offset > 0; offset >>= 1) all += __shfl_xor_sync(ALL, all, offset);
+    weight /= all + (double)rule.norm_eps;
+  }
+  return (float)(weight * (double)rule.scale);
+}
+
 template <int PER>
 __global__ void __launch_bounds__(32 * ROUTE_WARPS, PER <= 8 ? 10 : 1)
 route_groups_kernel(const float* __restrict__ logits, size_t pitch, int rows, const float* __restrict__ bias, GroupRule rule,
@@ -317,13 +330,19 @@ route_groups_kernel(const float* __restrict__ logits, size_t pitch, int rows, co
     choice = route_choose_exactly(from, bias, rule, shared, lane);
   else if (near)
     choice = route_reorder(from, bias, choice, count, lane);
-  // the chosen scores, a lane each
+  // the chosen scores, a lane each; where 32 bits do not hold one (below e^-87), in 64: divided by their sum they may be anything
+  const float logit = lane < rule.top ? from[choice] : 0.f;
   float weight = 0.f;
-  if (lane < rule.top) weight = rule.scoring == ROUTE_SOFTMAX ? expf(from[choice] - most) / sum : 1.0f / (1.0f + expf(-from[choice]));
-  if (rule.renormalize) weight /= srb_warp_sum(weight) + rule.norm_eps;
+  if (lane < rule.top) weight = rule.scoring == ROUTE_SOFTMAX ? expf(logit - most) / sum : 1.0f / (1.0f + expf(-logit));
+  if (__any_sync(ALL, lane < rule.top && weight < 1e-37f)) {
+    weight = route_far_weight(rule.scoring == ROUTE_SOFTMAX ? (double)logit - (double)most : (double)logit, sum, rule, lane);
+  } else {
+    if (rule.renormalize) weight /= srb_warp_sum(weight) + rule.norm_eps;
+    weight *= rule.scale;
+  }
   if (lane < rule.top) {
     chosen[(size_t)row * rule.top + lane] = choice;
-    weights[(size_t)row * rule.top + lane] = weight * rule.scale;
+    weights[(size_t)row * rule.top + lane] = weight;
   }
 }
 

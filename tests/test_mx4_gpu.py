@@ -674,3 +674,18 @@ def test_groups_whose_scores_32_bits_do_not_hold(scoring):
         logits[:, 0] = 0.0
         logits[:, 4:12] -= 15.0
     check_choice(logits.cuda(), dict(experts=16, top=3, groups=4, top_groups=1 if scoring == "sigmoid" else 2, group_best=2, scoring=scoring), None)
+
+
+@pytest.mark.parametrize("eps", [0.0, 1e-20])
+@pytest.mark.parametrize("low", [-80.0, -88.0, -100.0, -300.0, -600.0])
+def test_renormalised_weights_of_scores_that_32_bits_do_not_hold(low, eps):
+    g = generator(53)
+    logits = low + 2 * torch.randn(50, 32, generator=g)
+    logits[25:, 7] = 1.0
+    check_choice(logits.cuda(), dict(experts=32, top=4, renormalize=True, scoring="sigmoid", eps=eps, scale=2.5), None)
+    # a bias that closes the one expert with a score to speak of
+    bias = torch.zeros(32)
+    bias[7] = -4.0
+    logits[:, 7] = 1.0
+    for scoring in ("softmax", "sigmoid"):
+        check_choice(logits.cuda(), dict(experts=32, top=4, renormalize=True, scoring=scoring, eps=eps), bias.cuda())
