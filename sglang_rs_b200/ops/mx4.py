@@ -296,8 +296,11 @@ def choose_experts(logits: torch.Tensor, top: int, renormalize: bool = False, *,
         _need(choice_bias, "choice_bias", torch.float32)
         if choice_bias.shape != (experts,):
             raise KernelError("choose_experts: one choice bias per expert is needed")
-    if top < 0 or top > 2**31 - 1 or rows * max(top, 1) >= 2**31:
-        raise KernelError(f"choose_experts: {rows} rows of {top} choices")
+    # (what follows counts in 32 bits; the kernel has its own limits below these)
+    if not 0 < top <= experts or rows * top >= 2**31 or max(rows, experts) > MX4_MOST:
+        raise KernelError(f"choose_experts: {rows} rows of {top} choices of {experts} experts")
+    if not (0 < top_groups <= groups <= experts) or group_best not in (1, 2):
+        raise KernelError(f"choose_experts: {experts} experts in {groups} groups, {top_groups} of them open by their {group_best} best")
     here = _here("choose_experts", logits, choice_bias)
     chosen, weights = logits.new_empty((rows, top), dtype=torch.int32), logits.new_empty((rows, top))
     lib = _library("route_groups")

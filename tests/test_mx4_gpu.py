@@ -689,3 +689,10 @@ def test_renormalised_weights_of_scores_that_32_bits_do_not_hold(low, eps):
     logits[:, 7] = 1.0
     for scoring in ("softmax", "sigmoid"):
         check_choice(logits.cuda(), dict(experts=32, top=4, renormalize=True, scoring=scoring, eps=eps), bias.cuda())
+
+
+@pytest.mark.parametrize("options", [dict(groups=2 ** 32 + 1), dict(groups=2 ** 32 + 2, top_groups=2 ** 32 + 1), dict(top_groups=2 ** 32 + 1), dict(group_best=2 ** 32 + 1),
+                                     dict(top=2 ** 32 + 1), dict(top=2 ** 30), dict(groups=0), dict(top_groups=0), dict(groups=-1), dict(group_best=0)])
+def test_numbers_that_32_bits_do_not_hold_are_refused(options):
+    with pytest.raises(ops.KernelError):
+        ops.choose_experts(torch.zeros(1, 8, device="cuda"), **{"top": 2, **options})
