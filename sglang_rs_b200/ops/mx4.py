@@ -236,7 +236,8 @@ def linear_mx4(x, weight: Mx4, error_word: torch.Tensor, *, bias: Optional[torch
 
     Rows of bfloat16 go in as parts that add up to them: every entry exactly where it is at least 2^-14 of the largest of its 32
     neighbours, otherwise to 2^-22 of that one; a few rows, up to 192, also to no less than 2^-129.  A row with an infinity or something
-    that is not a number gives rows that are not numbers.  No result depends on other rows or on timing."""
+    that is not a number gives rows that are not numbers.  The bits of a row's result do not depend on what the other rows hold, nor on
+    timing; they do on how many rows there are, by which the kernel, the parts and the order of the sums are chosen."""
     four = isinstance(x, Mx4)
     if four:
         _need_mx4(x, "x", False)
@@ -319,7 +320,10 @@ def chosen_experts_mx4(h: torch.Tensor, chosen: torch.Tensor, weights: torch.Ten
     :func:`~sglang_rs_b200.ops.route`); a choice outside the experts adds nothing, one made twice counts twice.
     ``w_gate_up``: a stack [experts, 2 * inner, width], an expert's gate rows over its up rows (``gated`` False: the up matrices
     alone [experts, inner, width], an expert being W_down act(W_up h)); ``w_down`` a stack [experts, width, inner].  Sums are
-    taken in 32 bits; act(gate) * up is rounded once between the two products.  Nothing is decided on the host.  A row with an infinity or
+    taken in 32 bits; act(gate) * up is rounded once between the two products: where an expert's rows go through the kernel for many, to
+    a relative 2^-9 (two parts of four significant bits; bfloat16 has 2^-8) or 2^-22 of the largest of 32 neighbours, and through the one for few to
+    2^-23 of that (eight parts).  Which of the two depends on the number of rows and, from 64 experts on, on how many of them chose the
+    expert.  Nothing is decided on the host.  A row with an infinity or
     something that is not a number, and one whose act(gate) * up is beyond 32 bits, gives a row that is not a number, whatever the
     activation makes of it."""
     _need(h, "h", torch.bfloat16); _need(chosen, "chosen", torch.int32); _need(weights, "weights", torch.float32)

@@ -696,3 +696,17 @@ def test_renormalised_weights_of_scores_that_32_bits_do_not_hold(low, eps):
 def test_numbers_that_32_bits_do_not_hold_are_refused(options):
     with pytest.raises(ops.KernelError):
         ops.choose_experts(torch.zeros(1, 8, device="cuda"), **{"top": 2, **options})
+
+
+@pytest.mark.parametrize("four", [False, True])
+@pytest.mark.parametrize("rows,width,features", [(1, 4096, 512), (16, 4096, 512), (17, 4096, 512), (48, 2100, 300), (64, 8192, 130), (65, 4096, 512), (200, 2048, 300)])
+def test_a_row_does_not_depend_on_what_the_others_hold(rows, width, features, four):
+    """K is cut into parts here; the same number of rows, all but one of them others (of other sizes, and not finite)."""
+    x, matrix = rows_of(55, rows, width), random_matrix(56, features, width)[0]
+    call = lambda x: ops.linear_mx4(ops.quantize_mx4(x) if four else x, matrix, word(), out_dtype=torch.float32)
+    all_of_them = call(x)
+    for keep in {0, rows // 2, rows - 1}:
+        other = rows_of(57, rows, width) * 2.0 ** 30
+        other[::3, 5], other[1::7, 9] = math.inf, math.nan
+        other[keep] = x[keep]
+        assert torch.equal(call(other)[keep], all_of_them[keep])
