@@ -71,6 +71,7 @@ struct PairMx4Args {
   int x_lo_row, xs_lo_tile;      // where the second part's rows and tiles of scales begin
   int ws_tiles;                  // row tiles of scales of a matrix
   int tiles_t, tiles_f;
+  int by_element;                // rows of the result that do not start on 16-byte borders: no TMA
   int activation;
   float act_param;
   int* error_word;
@@ -112,6 +113,29 @@ __device__ __forceinline__ void store_16(unsigned at, unsigned a, unsigned b, un
 __device__ __forceinline__ unsigned two_bf16(float low, float high) {
   const __nv_bfloat162 v = __floats2bfloat162_rn(low, high);
   return *reinterpret_cast<const unsigned*>(&v);
+}
+
+// A warp's box (`live` rows of 64 bytes, swizzled) to rows that start anywhere: the lanes take neighbouring entries, a row of 32 bfloat16 at a time or two
+// of 16 floats (2,048 rows of bfloat16 through 4,096 x 24,575: 274 us, 24,576 by TMA 266; both in four bits 97 and 92, through 512 x 24,575 54 and 41).
+template <bool FLOAT>
+__device__ __forceinline__ void pair_store_elements(const PairMx4Args& a, unsigned box, int first, int live, int feature, int lane) {
+  constexpr int WIDTH = FLOAT ? 16 : 32, BYTES = FLOAT ? 4 : 2;
+  const int column = lane % WIDTH;
+  if (feature + column >= a.features) return;
+#pragma unroll 4
+  for (int r = lane / WIDTH; r < live; r += 32 / WIDTH) {
+    const unsigned from = box + r * 64 + ((((unsigned)column * BYTES >> 4) ^ ((unsigned)(r >> 1) & 3u)) << 4) + (column * BYTES & 15);
+    const size_t at = (size_t)(first + r) * a.ldo + feature + column;
+    if (FLOAT) {
+      unsigned v;
+      asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(from) : "memory");
+      reinterpret_cast<unsigned*>(a.out)[at] = v;
+    } else {
+      unsigned short v;
+      asm volatile("ld.shared.b16 %0, [%1];" : "=h"(v) : "r"(from) : "memory");
+      reinterpret_cast<unsigned short*>(a.out)[at] = v;
+    }
+  }
 }
 
 // What a tile is, the same in every role of both CTAs.
@@ -379,6 +403,11 @@ mx4_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
                   store_16(row + ((i ^ turn) << 4), two_bf16(q[0], q[1]), two_bf16(q[2], q[3]), two_bf16(q[4], q[5]), two_bf16(q[6], q[7]));
                 }
               }
+              if (!GROUPED && a.by_element) {
+                __syncwarp();
+                pair_store_elements<MODE == MXP_F32>(a, box, first, live, feature + 16 * half, lane);
+                continue;
+              }
               fence_proxy_async_shared();
               __syncwarp();
               if (lane == 0 && feature + 16 * half < a.features) pair_tma_store(&map_out, box, feature + 16 * half, first);
@@ -424,15 +453,15 @@ extern "C" long long srb_mx4_linear_pair_scratch(int rows, int width) {
   return (long long)scratch.used;
 }
 
-// out's rows are `ldo` elements apart, a multiple of 16 bytes.
+// out's rows are `ldo` elements apart.
 extern "C" int srb_mx4_linear_pair(const void* x, long long ldx, const void* x_scales, const void* w, const void* w_scales, const float* bias, void* out,
                                    long long ldo, int rows, int features, int width, int out_float, void* scratch_memory, int* error_word, void* stream) {
   if (rows <= 0 || features <= 0) return SRB_OK;
   if (width <= 0) SRB_FAIL("mx4_linear_pair: inner size %d must be positive", width);
   if (((uintptr_t)w & 31) || (x_scales && ((uintptr_t)x & 31))) SRB_FAIL("mx4_linear_pair: codes must start on 32-byte borders");
-  if (((uintptr_t)out & 15) || ldo * (out_float ? 4 : 2) % 16) SRB_FAIL("mx4_linear_pair: rows of the result must start on 16-byte borders");
   PairMx4Args a = {};
   a.bias = bias; a.out = out; a.ldo = ldo; a.rows = rows; a.features = a.w_rows = features; a.k_tiles = mx4_tiles(width); a.error_word = error_word;
+  a.by_element = ((uintptr_t)out & 15) != 0 || ldo * (out_float ? 4 : 2) % 16 != 0;
   a.tiles_t = (rows + MXP_TILE - 1) / MXP_TILE; a.tiles_f = (features + MXP_N - 1) / MXP_N; a.ws_tiles = mx4_tiles(features);
   const long long row_tiles = mx4_tiles(rows), tiles = (long long)a.tiles_t * a.tiles_f, scale_tiles = 2 * row_tiles * a.k_tiles;
   if (tiles > 0x3fffffff || 2ll * row_tiles * 128 > 0x7fffffff || scale_tiles > 0x7fffffff || (long long)a.ws_tiles * a.k_tiles > 0x7fffffff)
@@ -451,9 +480,11 @@ extern "C" int srb_mx4_linear_pair(const void* x, long long ldx, const void* x_s
   if (make_bytes_map(&maps[0], x, four ? rows : 2ll * rows, a.k_tiles * (four ? 64 : 128), MXP_ROWS) != SRB_OK ||
       make_scales_map(&maps[1], x_scales, four ? scale_tiles / 2 : scale_tiles, four ? 2 : 1) != SRB_OK ||
       (four ? make_bytes_map(&maps[2], w, features, a.k_tiles * 64, MXP_HALF) : make_codes_map(&maps[2], w, features, a.k_tiles, MXP_HALF)) != SRB_OK ||
-      make_scales_map(&maps[3], w_scales, (long long)a.ws_tiles * a.k_tiles, four ? 2 : 1) != SRB_OK ||
-      make_map(&maps[4], out_float ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, out, rows, features, ldo * (out_float ? 4 : 2),
-               32, out_float ? 16 : 32, CU_TENSOR_MAP_SWIZZLE_64B) != SRB_OK)
+      make_scales_map(&maps[3], w_scales, (long long)a.ws_tiles * a.k_tiles, four ? 2 : 1) != SRB_OK)
+    return SRB_ERR_INVALID;
+  maps[4] = maps[0];
+  if (!a.by_element && make_map(&maps[4], out_float ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, out, rows, features,
+                                ldo * (out_float ? 4 : 2), 32, out_float ? 16 : 32, CU_TENSOR_MAP_SWIZZLE_64B) != SRB_OK)
     return SRB_ERR_INVALID;
   if (four) return out_float ? launch_pair<true, MXP_F32, false>(maps, a, (int)tiles, s) : launch_pair<true, MXP_BF16, false>(maps, a, (int)tiles, s);
   return out_float ? launch_pair<false, MXP_F32, false>(maps, a, (int)tiles, s) : launch_pair<false, MXP_BF16, false>(maps, a, (int)tiles, s);

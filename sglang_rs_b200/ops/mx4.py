@@ -231,8 +231,7 @@ def linear_mx4(x, weight: Mx4, error_word: torch.Tensor, *, bias: Optional[torch
     """y = x @ weight^T (+ bias), sums in 32 bits; bfloat16, or float32 with ``out_dtype``.
 
     ``x``: bfloat16 [rows, width] (dense rows, any pitch), or an :class:`Mx4` of rows: both operands are then multiplied in four
-    bits.  ``weight``: one matrix [features, width]; ``bias`` float32 [features].  Rows of the result may lie further apart than they
-    are long (many rows of a number of features that is no multiple of 8).
+    bits.  ``weight``: one matrix [features, width]; ``bias`` float32 [features].  The result is contiguous.
 
     Rows of bfloat16 go in as parts that add up to them: every entry exactly where it is at least 2^-14 of the largest of its 32
     neighbours, otherwise to 2^-22 of that one; a few rows, up to 192, also to no less than 2^-129.  A row with an infinity or something
@@ -263,18 +262,16 @@ def linear_mx4(x, weight: Mx4, error_word: torch.Tensor, *, bias: Optional[torch
             raise KernelError("linear_mx4: one bias per feature is needed")
     here = _here("linear_mx4", held, codes, weight.scales, bias, error_word)
     many = not _few_rows(rows, features, four)
-    # the kernel for many rows stores rows that start on 16-byte borders
-    pitch = -(-features // 8) * 8 if many else features
-    out = codes.new_empty((rows, pitch), dtype=out_dtype)
+    out = codes.new_empty((rows, features), dtype=out_dtype)
     if rows and features:
         lib = _library("gemm_mx4_pair" if many else "gemm_mx4")
         product, needed = (lib.srb_mx4_linear_pair, lib.srb_mx4_linear_pair_scratch) if many else (lib.srb_mx4_linear, lib.srb_mx4_linear_scratch)
         needed = 0 if four else needed(rows, width)
         scratch = codes.new_empty(needed) if needed else None
         _check(lib, product(held.data_ptr(), held.stride(0), x.scales.data_ptr() if four else None, codes.data_ptr(), weight.scales.data_ptr(),
-                            None if bias is None else bias.data_ptr(), out.data_ptr(), pitch, rows, features, width,
+                            None if bias is None else bias.data_ptr(), out.data_ptr(), features, rows, features, width,
                             out_dtype == torch.float32, scratch.data_ptr() if needed else None, error_word.data_ptr(), _stream(here)), 2 if needed else 1)
-    return out if pitch == features else out[:, :features]
+    return out
 
 
 @traced("routed_experts")

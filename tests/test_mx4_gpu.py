@@ -710,3 +710,20 @@ def test_a_row_does_not_depend_on_what_the_others_hold(rows, width, features, fo
         other[::3, 5], other[1::7, 9] = math.inf, math.nan
         other[keep] = x[keep]
         assert torch.equal(call(other)[keep], all_of_them[keep])
+
+
+@pytest.mark.parametrize("four", [False, True])
+@pytest.mark.parametrize("out_dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows,features", [(3, 129), (65, 7), (70, 33), (200, 129), (257, 199), (300, 1030), (290, 20001), (260, 196)])
+def test_results_are_contiguous_whatever_their_sizes(rows, features, out_dtype, four):
+    x, (matrix, w) = rows_of(58, rows, 200), random_matrix(59, features, 200)
+    bias = torch.randn(features, generator=generator(60)).cuda()
+    assert check_linear(ops.quantize_mx4(x) if four else x, matrix, w, bias, out_dtype).is_contiguous()
+
+
+def test_a_product_feeds_the_experts_however_many_rows_there_are():
+    _, chosen, weights, up, down = expert_case(68, 70, 4, 130, 64, 2)
+    matrix, _ = random_matrix(69, 130, 96)
+    for rows in (8, 70):
+        h = ops.linear_mx4(rows_of(70, rows, 96) * 2.0 ** -8, matrix, word())
+        check_experts(h, chosen[:rows], weights[:rows], up, down)
