@@ -32,9 +32,11 @@ MX4_FEW_ROWS_OF_SMALL = 192
 #: and 189, 48 226 and 215; 32 of 1,024 x 1,024 with 64 83 and 100, 96 109 and 100; 8 of 1,024 x 512 with 96 30 and 38, 192 43 and 38)
 MX4_FEW_BYTES = 160 << 20
 #: above it, from this many experts on, they are divided on the device, those with up to MX4_FEW_SLOTS rows going to the kernel for few rows all the same: a tile
-#: of 256 rows costs the pairs as much with one row (all on pairs and divided: 128 experts of 2,048 x 768 with 96 choices each 335 and 309 where some have
-#: many more than others, 317 and 350 spread evenly; 64 of 2,048 x 1,408 with 192, very uneven, 431 and 390 again and again, where the chip's power
-#: limit counts; 48 of 1,024 x 1,024 with 192 192 and 189, evenly 172 and 181; but 32 of 2,048 x 1,408 with 96 144 and 155: three launches more)
+#: of 256 rows costs the pairs as much with one row.  That pays where some experts have many more rows than others, as routers choose them, and
+#: costs three launches where all have as many (us, all on pairs and divided, from a graph: 64 of 2,048 x 1,408 with 192 choices each 361 and 343,
+#: evenly 285 and 298; 64 of 1,024 x 1,024 with 187 240 and 214, evenly 187 and 199; 128 of 2,048 x 768 with 96 299 and 269, evenly 324 and 346; 256 of
+#: 1,024 x 512 with 256 660 and 605, evenly 614 and 637).  Fewer experts gain less: 48 of 1,024 x 1,024 with 192 192 and 189, evenly 172 and 181; 32 of
+#: 2,048 x 1,408 with 96 lose, 144 and 155.  How even the load is, only the device knows
 MX4_DIVIDE_EXPERTS = 64
 MX4_FEW_SLOTS = 48
 

@@ -727,3 +727,55 @@ def test_a_product_feeds_the_experts_however_many_rows_there_are():
     for rows in (8, 70):
         h = ops.linear_mx4(rows_of(70, rows, 96) * 2.0 ** -8, matrix, word())
         check_experts(h, chosen[:rows], weights[:rows], up, down)
+
+
+@pytest.mark.parametrize("kernels", KERNELS)
+def test_a_thousand_experts_unevenly_loaded_on_each_kernel(kernels, monkeypatch):
+    for setting, value in KERNELS[kernels].items():
+        monkeypatch.setattr(mx4, setting, value)
+    h, _, weights, up, down = expert_case(90, 700, 1000, 64, 32, 3)
+    chosen = (torch.rand(700, 3, generator=generator(91)) ** 6 * 1000).int().cuda()        # some have a hundred rows, most none
+    chosen[:5] = 999
+    check_experts(h, chosen, weights, up, down)
+
+
+@pytest.mark.parametrize("kernels", KERNELS)
+def test_experts_give_the_same_bits_again_and_beside_other_work(kernels, monkeypatch):
+    for setting, value in KERNELS[kernels].items():
+        monkeypatch.setattr(mx4, setting, value)
+    h, chosen, weights, up, down = expert_case(92, 300, 12, 264, 200, 3)
+    error = word()
+    call = lambda: ops.chosen_experts_mx4(h, chosen, weights, up[0], down[0], "silu", error)
+    first = call()
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    torch.cuda.synchronize()
+    results = []
+    for stream in streams:
+        with torch.cuda.stream(stream):
+            results += [call() for _ in range(4)]
+    torch.cuda.synchronize()
+    ops.raise_on_error_word(error)
+    assert all(torch.equal(first, r) for r in results)
+
+
+def test_a_matrix_quantised_right_ahead_of_its_product():
+    """The product's early reads of the matrix come behind the kernel that makes it, eager and captured."""
+    error = word()
+    for rows in (1, 5, 40, 90):
+        x, weights = rows_of(93, rows, 512), [rows_of(94 + i, 3000, 512) for i in range(3)]
+        want = [ops.linear_mx4(x, ops.quantize_mx4(w), error) for w in weights]
+        torch.cuda.synchronize()
+        weight = weights[0].clone()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            result = ops.linear_mx4(x, ops.quantize_mx4(weight), error)
+        for _ in range(3):
+            for w, y in zip(weights, want):
+                weight.copy_(w)
+                graph.replay()
+                torch.cuda.synchronize()
+                assert torch.equal(result, y)
+                matrix = ops.quantize_mx4(w)
+                assert torch.equal(ops.linear_mx4(x, matrix, error), y)
+                del matrix
+    ops.raise_on_error_word(error)
