@@ -22,21 +22,23 @@ MX4_BLOCK = 32
 #: the largest size of a matrix: the kernels count rows and entries in 32 bits, in whole tiles
 MX4_MOST = 2**31 - 2**16
 #: Up to this many rows a product runs on the kernel that has the weights on the M side (csrc/gemm_mx4.cu), above it on pairs of CTAs (us, that kernel and
-#: pairs, 4,096 x 24,576: 64 rows 30 and 36, 96 rows 39 and 37; both operands in four bits 64 rows 19 and 19, 96 rows 23 and 20) ...
+#: pairs, 4,096 x 24,576: 64 rows 30 and 37, 96 rows 39 and 37; both operands in four bits, without the quantising of the rows, 64 rows 15.7 and 16.0, 96 rows
+#: 19 and 17, 4,096 x 4,096: 64 rows 8.3 and 8.6, 96 rows 9.8 and 8.7) ...
 MX4_FEW_ROWS = 64
 #: ... and rows of bfloat16 up to this many there too, where the pairs' tiles would leave half of the pairs idle (4,096 x 4,096: 128 rows 14 and
 #: 20, 192 rows 20 and 21, 256 rows 22 and 21; 12,288 x 4,096: 192 rows 48 and 49; 2,048 x 2,048: 192 rows 9 and 13)
 MX4_FEW_ROWS_OF_SMALL = 192
-#: The experts' products run on the kernel for few rows while choices per expert * bytes of an expert's codes stay below this (that kernel reads an expert's
-#: matrices, from L2, for every 8 of its rows; us, it and the best of the others: 64 experts of 2,048 x 1,408 with 32 choices each 161 and 174, 40 189
-#: and 189, 48 226 and 215; 32 of 1,024 x 1,024 with 64 83 and 100, 96 109 and 100; 8 of 1,024 x 512 with 96 30 and 38, 192 43 and 38)
-MX4_FEW_BYTES = 160 << 20
+#: The experts' products run on the kernel for few rows while choices per expert * bytes of an expert's codes stay below this.  That kernel reads an expert's
+#: matrices, from L2, for every 8 of its rows, and holds what is between the products more finely; it is left where it is clearly the slower one (us, it
+#: and the best of the others: 64 experts of 2,048 x 1,408 with 24 choices each 126 and 136, 32 156 and 144, 40 186 and 157; 32 of 1,024 x 1,024 with 64
+#: 80 and 76, 96 107 and 79; 8 of 1,024 x 512 with 96 30 and 32, 144 36 and 35, 192 43 and 34)
+MX4_FEW_BYTES = 136 << 20
 #: above it, from this many experts on, they are divided on the device, those with up to MX4_FEW_SLOTS rows going to the kernel for few rows all the same: a tile
 #: of 256 rows costs the pairs as much with one row.  That pays where some experts have many more rows than others, as routers choose them, and
-#: costs three launches where all have as many (us, all on pairs and divided, from a graph: 64 of 2,048 x 1,408 with 192 choices each 361 and 343,
-#: evenly 285 and 298; 64 of 1,024 x 1,024 with 187 240 and 214, evenly 187 and 199; 128 of 2,048 x 768 with 96 299 and 269, evenly 324 and 346; 256 of
-#: 1,024 x 512 with 256 660 and 605, evenly 614 and 637).  Fewer experts gain less: 48 of 1,024 x 1,024 with 192 192 and 189, evenly 172 and 181; 32 of
-#: 2,048 x 1,408 with 96 lose, 144 and 155.  How even the load is, only the device knows
+#: costs three launches where all have as many (us, all on pairs and divided, from a graph: 64 of 2,048 x 1,408 with 192 choices each 340 and 319,
+#: evenly 271 and 281; 64 of 1,024 x 1,024 with 187 165 and 165, evenly 144 and 155; 128 of 2,048 x 768 with 96 281 and 251, evenly 303 and 321; 256 of
+#: 1,024 x 512 with 256 483 and 458, evenly 473 and 497).  Fewer experts do not gain: 48 of 1,024 x 1,024 with 192 131 and 140; 32 of 1,024 x 1,024
+#: with 96 79 and 86.  How even the load is, only the device knows
 MX4_DIVIDE_EXPERTS = 64
 MX4_FEW_SLOTS = 48
 
@@ -211,7 +213,8 @@ def quantize_mx4(x: torch.Tensor) -> Mx4:
 
 @traced("quantize")
 def dequantize_mx4(q: Mx4, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
-    """The values that ``q`` stands for, in bfloat16 (exact: a code times a power of two) or float32."""
+    """The values that ``q`` stands for, in bfloat16 or float32: exact in both, a code times a power of two, but for those of 2^128 and above, which
+    scales of 253 and 254 (:func:`quantize_mx4` makes none) can have and which become infinite."""
     _need_mx4(q, "q", None)
     code = dtype_code(dtype)
     codes, width = q.codes, q.width

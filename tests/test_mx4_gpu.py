@@ -779,3 +779,13 @@ def test_a_matrix_quantised_right_ahead_of_its_product():
                 assert torch.equal(ops.linear_mx4(x, matrix, error), y)
                 del matrix
     ops.raise_on_error_word(error)
+
+
+@pytest.mark.parametrize("out", [torch.bfloat16, torch.float32])
+def test_every_scale_and_code_as_values(out):
+    codes = torch.arange(16, dtype=torch.uint8).repeat(256, 2)
+    scales = torch.arange(256, dtype=torch.uint8)[:, None].contiguous()
+    want = pm.values(codes, scales)
+    want = torch.where(want.abs() >= 2.0 ** 128, want.sign() * math.inf, want)
+    got = ops.dequantize_mx4(ops.mx4_from_rows(pm.packed(codes).cuda(), scales.cuda()), out).cpu().double()
+    assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.nan_to_num(7.0), want.nan_to_num(7.0))
