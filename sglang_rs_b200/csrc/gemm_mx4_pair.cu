@@ -14,14 +14,15 @@
 // Over experts (GROUPED) a tile is up to 256 slots of one expert (the plan of csrc/moe.cu); X and the parts that the gated mode leaves have room
 // for 256 rows a tile, so that a tile's scales are whole tiles.  Gated: the even CTA brings gate rows, the odd one the up rows of the same 96 features,
 // whose scales come regrouped (mx4_gated_scales: 96 and 96 rows are no whole tiles; a word a row by cp.async instead kept the tensor cores
-// waiting, 296 us instead of some 215 for the gate/up of 12,288 slots, 64 experts of 2,048 x 1,408).
+// waiting, 296 us instead of some 215 for the gate/up of 12,288 slots, 64 experts of 2,048 x 1,408, as the epilogue then was; those of experts with more
+// than 48 slots take 145 us now, the tensor pipe active 0.73 of them).
 //
-// Bound by the tensor cores under the chip's power limit: 2,048 rows of bfloat16 through 4,096 x 24,576 in 262 us for some milliseconds (1,570 TFLOP/s of
-// the product, twice that of the parts' products: 0.96 of the library's bfloat16 rate), 300 again and again.  Both operands in four bits by what L2 brings,
-// some 10 TB/s: 95 us (4,300 TFLOP/s), 8 us of it the rows' quantising.  Without the copies of scales it takes no less; a sixth stage with five places for
-// scales, each awaited ahead of its next copies, 109 to 116: tensor memory has no columns for a sixth place.  Tiles of 384 rows of W in one buffer,
-// which bring X half as often, took the same (260, 93 with six stages): nothing is multiplied while
-// they are stored.
+// Bound by the tensor cores under the chip's power limit: 2,048 rows of bfloat16 through 4,096 x 24,576 in 262 to 267 us for some milliseconds (1,560
+// TFLOP/s of the product, twice that of the parts' products: 0.95 of the library's bfloat16 rate), 310 again and again.  Both operands in four bits by
+// what L2 brings, 10.3 TB/s: 95 to 97 us and 113 again and again (4,300 TFLOP/s), 8 us of it the rows' quantising.  Without the copies of scales
+// it takes no less; a sixth stage with five places for scales, each awaited ahead of its next copies, 109 to 116: tensor memory has no columns for a
+// sixth place.  Tiles of 384 rows of W in one buffer, which bring X half as often, took the same (260, 93 with six stages): nothing is multiplied
+// while they are stored.
 //
 // Warps: 0 TMA, 1 products (even CTA) and tensor memory, 2-13 epilogue: a quarter of the lanes and a third of the columns each.  Waits are
 // bounded; one that runs out flags SRB_FLAG_WAIT_TIMEOUT.
