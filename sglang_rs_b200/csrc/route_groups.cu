@@ -14,8 +14,7 @@
 //
 // A warp per row, expert lane + 32 j the lane's j-th.  Picks lie in registers as unsigned numbers of the same order, so that a largest one of the
 // warp is one instruction (redux.sync; two for 64 bits) and its lowest index another.  Bound by a row's chain of instructions, some 1,600 for 256
-// experts in 8 groups: 64 rows 6.4 us, 8,192 rows 19 to 20 (their bytes take 1.4; 22 where every
-// doubt costs the whole row); a row that is chosen once more takes 8 to 11 more by itself.
+// experts in 8 groups: 64 rows 6.4 us, 8,192 rows 18.4 to 22 (their bytes take 1.4); a row that is chosen once more takes 8 to 11 more by itself.
 #include "common.cuh"
 #include <math.h>
 
